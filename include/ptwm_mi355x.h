@@ -14,7 +14,7 @@
  * any other negative value an internal error.
  *
  * Device ("_cuda") entry points take device addresses as u64 and a device
- * ordinal.  They run on the library's own per-device stream (the handle the
+ * ordinal.  Those of the codec (sections 1 and 2) run on the library's own per-device stream (the handle the
  * *_stream_handle symbols return) and synchronise it before returning, so
  * the output is complete and visible to any stream when they return
  * (native.rs:152-162).  Input and output must be distinct allocations.
@@ -376,6 +376,61 @@ int64_t ptwm_mi355x_set_profiling(uint32_t device_ordinal, uint32_t on);
 /* Durations of the last profiled call in milliseconds: out3[0] entropy-decode
  * kernel(s), out3[1] merge kernel(s), out3[2] both. */
 int64_t ptwm_mi355x_last_kernel_ms(uint32_t device_ordinal, float *out3);
+
+/* ===================================================================== */
+/* 3. Operators on microscaled (MX) blocks                                */
+/* ===================================================================== */
+
+/* What a program does with MXFP4 tensors once a decode has restored them;
+ * the reference, which stops at the restored bytes, has no counterpart.  A
+ * block is 32 consecutive values of a row with one scale byte b (E8M0):
+ * 2^(b-127), NaN for 255.  Weights are e2m1 codes, two a byte, the first
+ * value in the low nibble, as the nibble chain restores them, with their
+ * scales as a tensor of their own; 8-bit activations are e4m3 codes.
+ *
+ * These calls differ from the codec's in one way: they queue their work on
+ * `stream` (a hipStream_t of the device, 0 = the null stream) and return
+ * without waiting for it.  They hold no state, lock, workspace or scratch,
+ * allocate nothing, and may be captured into a graph.  Addresses need the
+ * alignment of their elements only; strides are between rows, in elements
+ * (weights and scales: bytes).  dtypes are public dtype codes (dtype.rs:79-103):
+ * 1 float32, 4 float16, 6 bfloat16, 29 float8_e4m3fn.  cols is a multiple of
+ * 32.  Returns 0; -1 for arguments that do not fit together (nothing is
+ * queued), -5 for a dtype the operator does not take.  Zero rows or tokens:
+ * 0, and nothing is queued.
+ *
+ * A block of outputs in 8 bits takes the smallest scale 2^(b-127), b >= 0,
+ * with which its largest magnitude is at most 448, e4m3's largest value;
+ * its codes are rounded to nearest, ties to even.  A block that holds an
+ * infinity or NaN gets the scale 255 and the codes 0x7F. */
+
+/* y = s * rsqrt(mean(s^2) + eps) * weight for every row of s = x + residual
+ * (residual 0: s = x), in 32 bits; codes and scales receive y, and sum
+ * (0: not wanted) s in x's dtype.  sum may be x or residual itself. */
+int64_t ptwm_mi355x_rms_norm_mx_cuda(uint32_t dtype, uint64_t x, uint64_t x_stride, uint64_t residual,
+                                     uint64_t residual_stride, uint32_t weight_dtype, uint64_t weight, float eps,
+                                     uint64_t sum, uint64_t sum_stride, uint64_t codes, uint64_t codes_stride,
+                                     uint64_t scales, uint64_t scales_stride, uint64_t rows, uint64_t cols,
+                                     uint64_t stream, uint32_t device_ordinal);
+
+/* y = gate / (1 + exp(-gate)) * up in 32 bits; codes and scales receive y. */
+int64_t ptwm_mi355x_swiglu_mx_cuda(uint32_t dtype, uint64_t gate, uint64_t gate_stride, uint64_t up,
+                                   uint64_t up_stride, uint64_t codes, uint64_t codes_stride, uint64_t scales,
+                                   uint64_t scales_stride, uint64_t rows, uint64_t cols, uint64_t stream,
+                                   uint32_t device_ordinal);
+
+/* out[t, n] = sum over k of x[t, k] * weight[n, k] (+ bias[n]) with sums in
+ * 32 bits and one rounding to out_dtype.  weight: rows x cols/2 bytes of
+ * codes, scales: rows x cols/32 bytes.  x is float32, float16, bfloat16, or
+ * float8_e4m3fn with x_scales (tokens x cols/32 bytes; 0 for the others).
+ * bias (0: none) has out's dtype.  Weights and activations are taken exactly,
+ * down to 2^-133; a code times its scale of 2^128 or more counts as infinite,
+ * and its sums as infinite or NaN. */
+int64_t ptwm_mi355x_mxfp4_linear_cuda(uint32_t x_dtype, uint64_t x, uint64_t x_stride, uint64_t x_scales,
+                                      uint64_t x_scales_stride, uint64_t weight, uint64_t weight_stride,
+                                      uint64_t scales, uint64_t scales_stride, uint32_t out_dtype, uint64_t bias,
+                                      uint64_t out, uint64_t out_stride, uint64_t tokens, uint64_t rows,
+                                      uint64_t cols, uint64_t stream, uint32_t device_ordinal);
 
 #ifdef __cplusplus
 }

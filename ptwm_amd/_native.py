@@ -28,6 +28,7 @@ _RC_NAMES = {
 
 # every symbol the header declares, with its ctypes signature
 _u8p = C.c_void_p
+_u64 = C.c_uint64
 _SIGS = {
     "ptwm_plane_codec_v1_encode": (C.c_int64, [_u8p, C.c_size_t, _u8p, C.c_size_t]),
     "ptwm_plane_codec_v1_decode": (C.c_int64, [_u8p, C.c_size_t, _u8p, C.c_size_t]),
@@ -88,6 +89,12 @@ _SIGS = {
     "ptwm_mi355x_merge_cuda": (
         C.c_int64, [C.c_uint32, C.POINTER(C.c_uint64), C.c_uint32, C.c_size_t, C.c_uint64, C.c_size_t,
                     C.c_uint32]),
+    "ptwm_mi355x_rms_norm_mx_cuda": (
+        C.c_int64, [C.c_uint32, _u64, _u64, _u64, _u64, C.c_uint32, _u64, C.c_float, _u64, _u64, _u64, _u64, _u64,
+                    _u64, _u64, _u64, _u64, C.c_uint32]),
+    "ptwm_mi355x_swiglu_mx_cuda": (C.c_int64, [C.c_uint32] + [_u64] * 11 + [C.c_uint32]),
+    "ptwm_mi355x_mxfp4_linear_cuda": (
+        C.c_int64, [C.c_uint32] + [_u64] * 8 + [C.c_uint32] + [_u64] * 7 + [C.c_uint32]),
 }
 
 

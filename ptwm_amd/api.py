@@ -496,3 +496,146 @@ def container_write(tensors, layout: str = "compact", payloads=None, as_array: b
     check(rc, "container_write")
     del keep
     return out[:n.value] if as_array else out[:n.value].tobytes()
+
+
+# Operators on microscaled (MX) blocks: what a program does with the MXFP4
+# tensors that a decode restored (library additions).  Unlike the codec calls
+# they queue their work on torch's current stream and return without waiting
+# for it, as torch's own operators do.
+
+_MX_DTYPES: dict = {}   # torch dtype -> public dtype code (dtype.rs:79-103)
+_MX_CODES: dict = {}    # torch dtypes that hold one scale or code byte -> what they may hold
+
+
+def _mx_dtypes() -> dict:
+    if not _MX_DTYPES:
+        import torch
+        _MX_CODES.update({"scales": (torch.float8_e8m0fnu, torch.uint8), "codes": (torch.float8_e4m3fn, torch.uint8),
+                          "weight": (torch.uint8, torch.float4_e2m1fn_x2)})
+        _MX_DTYPES.update({torch.float32: 1, torch.float16: 4, torch.bfloat16: 6, torch.float8_e4m3fn: 29})
+    return _MX_DTYPES
+
+
+def _mx_matrix(t, name: str, rows: int, cols: int, device_ordinal: int, dtypes) -> tuple[int, int]:
+    """(address, row stride) of a device matrix of the given size and one of
+    the given dtypes, whose rows are contiguous and do not overlap."""
+    if not t.is_cuda:
+        raise ValueError(f"{name}: tensor is not on a GPU device")
+    if t.get_device() != device_ordinal:
+        raise ValueError(f"{name}: tensor is on device {t.get_device()}, call names device {device_ordinal}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name}: dtype {t.dtype} is not one of {', '.join(str(d) for d in dtypes)}")
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != rows or shape[1] != cols:
+        raise ValueError(f"{name}: shape {tuple(shape)} is not ({rows}, {cols})")
+    stride, inner = t.stride()
+    if (inner != 1 and cols > 1) or (stride < cols and rows > 1):
+        raise ValueError(f"{name}: rows must be contiguous and must not overlap")
+    return t.data_ptr(), stride
+
+
+def _mx_vector(t, name: str, n: int, device_ordinal: int, dtypes) -> int:
+    """Address of a contiguous device vector of n elements."""
+    if not t.is_cuda:
+        raise ValueError(f"{name}: tensor is not on a GPU device")
+    if t.get_device() != device_ordinal:
+        raise ValueError(f"{name}: tensor is on device {t.get_device()}, call names device {device_ordinal}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name}: dtype {t.dtype} is not one of {', '.join(str(d) for d in dtypes)}")
+    if tuple(t.shape) != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name}: expected {n} contiguous elements")
+    return t.data_ptr()
+
+
+def _mx_input(t, name: str, eight_bit: bool) -> tuple[int, int, int]:
+    """(dtype code, rows, columns) of an operator's first input."""
+    if not hasattr(t, "data_ptr"):
+        raise TypeError(f"{name}: expected a device tensor")
+    code = _mx_dtypes().get(t.dtype)
+    if code is None or (code == 29 and not eight_bit):
+        raise TypeError(f"{name}: dtype {t.dtype} is not supported")
+    if t.dim() != 2:
+        raise ValueError(f"{name}: expected a matrix, a row a token")
+    rows, cols = t.shape
+    if cols == 0 or cols % 32:
+        raise ValueError(f"{name}: {cols} columns are not whole blocks of 32")
+    return code, rows, cols
+
+
+def rms_norm_mx_cuda(x, weight, out, out_scales, device_ordinal: int = 0, residual=None, sum_out=None,
+                     eps: float = 1e-6) -> None:
+    """Root-mean-square norm with an output in 8 bits (library addition):
+    ``s = x + residual``, ``y = s * rsqrt(mean(s**2) + eps) * weight`` for
+    every row, in 32 bits.  ``out`` [rows, cols] (float8_e4m3fn or uint8)
+    receives y's codes and ``out_scales`` [rows, cols / 32] (float8_e8m0fnu
+    or uint8) a power of two for each block of 32: the smallest with which
+    the block's largest magnitude is at most 448.  ``sum_out`` receives ``s``
+    in x's dtype and may be ``x`` or ``residual`` itself.  x: float32,
+    float16 or bfloat16, rows at any stride."""
+    code, rows, cols = _mx_input(x, "x", False)
+    same = (x.dtype,)
+    xp, xs = _mx_matrix(x, "x", rows, cols, device_ordinal, same)
+    wcode = _MX_DTYPES.get(weight.dtype)
+    wp = _mx_vector(weight, "weight", cols, device_ordinal, _MX_DTYPES)
+    if wcode == 29:
+        raise TypeError("weight: dtype torch.float8_e4m3fn is not supported")
+    rp = rs = sp = ss = 0
+    if residual is not None:
+        rp, rs = _mx_matrix(residual, "residual", rows, cols, device_ordinal, same)
+    if sum_out is not None:
+        sp, ss = _mx_matrix(sum_out, "sum_out", rows, cols, device_ordinal, same)
+    op, os_ = _mx_matrix(out, "out", rows, cols, device_ordinal, _MX_CODES["codes"])
+    cp, cs = _mx_matrix(out_scales, "out_scales", rows, cols // 32, device_ordinal, _MX_CODES["scales"])
+    if rows:
+        check(lib().ptwm_mi355x_rms_norm_mx_cuda(code, xp, xs, rp, rs, wcode, wp, eps, sp, ss, op, os_, cp, cs, rows,
+                                                 cols, _current_raw_stream(device_ordinal), device_ordinal),
+              "rms_norm_mx_cuda")
+
+
+def swiglu_mx_cuda(gate, up, out, out_scales, device_ordinal: int = 0) -> None:
+    """Gated activation with an output in 8 bits (library addition):
+    ``y = gate / (1 + exp(-gate)) * up`` in 32 bits, to ``out`` and
+    ``out_scales`` as :func:`rms_norm_mx_cuda` writes them.  gate and up:
+    float32, float16 or bfloat16, rows at any stride (the halves of one
+    matrix, say)."""
+    code, rows, cols = _mx_input(gate, "gate", False)
+    same = (gate.dtype,)
+    gp, gs = _mx_matrix(gate, "gate", rows, cols, device_ordinal, same)
+    up_, us = _mx_matrix(up, "up", rows, cols, device_ordinal, same)
+    op, os_ = _mx_matrix(out, "out", rows, cols, device_ordinal, _MX_CODES["codes"])
+    cp, cs = _mx_matrix(out_scales, "out_scales", rows, cols // 32, device_ordinal, _MX_CODES["scales"])
+    if rows:
+        check(lib().ptwm_mi355x_swiglu_mx_cuda(code, gp, gs, up_, us, op, os_, cp, cs, rows, cols,
+                                               _current_raw_stream(device_ordinal), device_ordinal), "swiglu_mx_cuda")
+
+
+def mxfp4_linear_cuda(x, weight, scales, out, device_ordinal: int = 0, x_scales=None, bias=None) -> None:
+    """``out = x @ W.T (+ bias)`` with MXFP4 weights (library addition):
+    ``weight`` [rows, cols / 2] holds e2m1 codes, the first of two in the low
+    nibble, and ``scales`` [rows, cols / 32] their E8M0 bytes, as a decode
+    restores them.  x [tokens, cols] is float32, float16, bfloat16, or
+    float8_e4m3fn with ``x_scales`` [tokens, cols / 32]; out [tokens, rows]
+    is float32, float16 or bfloat16, bias [rows] of out's dtype.  Sums are
+    held in 32 bits.  Rows may lie at any stride, but are contiguous."""
+    code, tokens, cols = _mx_input(x, "x", True)
+    xp, xs = _mx_matrix(x, "x", tokens, cols, device_ordinal, (x.dtype,))
+    if weight.dim() != 2:
+        raise ValueError("weight: expected a matrix, a row an output")
+    rows = weight.shape[0]
+    wp, ws = _mx_matrix(weight, "weight", rows, cols // 2, device_ordinal, _MX_CODES["weight"])
+    sp, ss = _mx_matrix(scales, "scales", rows, cols // 32, device_ordinal, _MX_CODES["scales"])
+    if (code == 29) != (x_scales is not None):
+        raise ValueError("x_scales: wanted with float8_e4m3fn activations, and only there")
+    cp = cs = bp = 0
+    if x_scales is not None:
+        cp, cs = _mx_matrix(x_scales, "x_scales", tokens, cols // 32, device_ordinal, _MX_CODES["scales"])
+    ocode = _MX_DTYPES.get(out.dtype)
+    op, os_ = _mx_matrix(out, "out", tokens, rows, device_ordinal, _MX_DTYPES)
+    if ocode == 29:
+        raise TypeError("out: dtype torch.float8_e4m3fn is not supported")
+    if bias is not None:
+        bp = _mx_vector(bias, "bias", rows, device_ordinal, (out.dtype,))
+    if tokens and rows:
+        check(lib().ptwm_mi355x_mxfp4_linear_cuda(code, xp, xs, cp, cs, wp, ws, sp, ss, ocode, bp, op, os_, tokens,
+                                                  rows, cols, _current_raw_stream(device_ordinal), device_ordinal),
+              "mxfp4_linear_cuda")

@@ -13,6 +13,7 @@
 #include "decode_sync.h"
 #include "ilv_host.h"
 #include "integrity.h"
+#include "mx_ops.h"
 #include "plane_ops.h"
 #include "ref_encode.h"
 #include "runtime.h"
@@ -197,6 +198,32 @@ int64_t ilv_decode_payload(DevCtx& ctx, uint64_t in_dev, size_t in_len, uint64_t
   }
   return (int64_t)expected;
 }
+
+// The operators on MX blocks need no context: they queue on the stream that
+// the caller names.  Makes the device current where it is not.
+struct OnDevice {
+  int prev = -1;
+  bool ok = false;
+  explicit OnDevice(uint32_t ord) {
+    if (ord > 0x7FFFFFFFu || hipGetDevice(&prev) != hipSuccess) return;
+    ok = prev == (int)ord || hipSetDevice((int)ord) == hipSuccess;
+    if (prev == (int)ord) prev = -1;
+  }
+  ~OnDevice() {
+    if (prev >= 0) (void)hipSetDevice(prev);
+  }
+};
+
+bool mx_float(uint32_t type) { return type == kTypeF32 || type == kTypeF16 || type == kTypeBf16; }
+
+// A row-major operand of `cols` elements a row: an address, and rows that do
+// not overlap.
+bool mx_rows(const MxRows& r, uint64_t rows, uint64_t cols) { return r.ptr && (rows <= 1 || r.stride >= cols); }
+
+int64_t mx_launched(hipError_t e) { return e == hipSuccess ? kOk : kInternal; }
+
+// Rows and columns that 32-bit grids and column indexes hold.
+constexpr uint64_t kMxMaxRows = 0x7FFFFFFF, kMxMaxCols = 1u << 30;
 
 // Host-buffer entry points stage through device memory on device 0.
 constexpr uint32_t kHostDevice = 0;
@@ -1082,6 +1109,61 @@ int64_t ptwm_mi355x_last_kernel_ms(uint32_t device_ordinal, float* out3) {
   if (!ds.ok) return kInvalidInput;
   for (int i = 0; i < 3; ++i) out3[i] = ds.ctx->last_ms[i];
   return 0;
+}
+
+int64_t ptwm_mi355x_rms_norm_mx_cuda(uint32_t dtype, uint64_t x, uint64_t x_stride, uint64_t residual,
+                                     uint64_t residual_stride, uint32_t weight_dtype, uint64_t weight, float eps,
+                                     uint64_t sum, uint64_t sum_stride, uint64_t codes, uint64_t codes_stride,
+                                     uint64_t scales, uint64_t scales_stride, uint64_t rows, uint64_t cols,
+                                     uint64_t stream, uint32_t device_ordinal) {
+  if (!mx_float(dtype) || !mx_float(weight_dtype)) return kUnsupported;
+  if (rows > kMxMaxRows || cols == 0 || cols > kMxMaxCols || cols % kMxBlock) return kInvalidInput;
+  if (rows == 0) return kOk;
+  const MxNormArgs a{{x, x_stride}, {residual, residual_stride}, {sum, sum_stride}, {codes, codes_stride},
+                     {scales, scales_stride}, weight, rows, (uint32_t)cols, eps};
+  if (!mx_rows(a.x, rows, cols) || !mx_rows(a.codes, rows, cols) || !mx_rows(a.scales, rows, cols / kMxBlock) ||
+      !weight || (residual && !mx_rows(a.residual, rows, cols)) || (sum && !mx_rows(a.sum, rows, cols)))
+    return kInvalidInput;
+  OnDevice on(device_ordinal);
+  if (!on.ok) return kInvalidInput;
+  return mx_launched(launch_rms_norm_mx(dtype, weight_dtype, a, reinterpret_cast<hipStream_t>(stream)));
+}
+
+int64_t ptwm_mi355x_swiglu_mx_cuda(uint32_t dtype, uint64_t gate, uint64_t gate_stride, uint64_t up,
+                                   uint64_t up_stride, uint64_t codes, uint64_t codes_stride, uint64_t scales,
+                                   uint64_t scales_stride, uint64_t rows, uint64_t cols, uint64_t stream,
+                                   uint32_t device_ordinal) {
+  if (!mx_float(dtype)) return kUnsupported;
+  if (rows > kMxMaxRows || cols == 0 || cols > kMxMaxCols || cols % kMxBlock) return kInvalidInput;
+  if (rows == 0) return kOk;
+  const MxSwigluArgs a{{gate, gate_stride}, {up, up_stride}, {codes, codes_stride}, {scales, scales_stride}, rows,
+                       (uint32_t)cols};
+  if (!mx_rows(a.gate, rows, cols) || !mx_rows(a.up, rows, cols) || !mx_rows(a.codes, rows, cols) ||
+      !mx_rows(a.scales, rows, cols / kMxBlock))
+    return kInvalidInput;
+  OnDevice on(device_ordinal);
+  if (!on.ok) return kInvalidInput;
+  return mx_launched(launch_swiglu_mx(dtype, a, reinterpret_cast<hipStream_t>(stream)));
+}
+
+int64_t ptwm_mi355x_mxfp4_linear_cuda(uint32_t x_dtype, uint64_t x, uint64_t x_stride, uint64_t x_scales,
+                                      uint64_t x_scales_stride, uint64_t weight, uint64_t weight_stride,
+                                      uint64_t scales, uint64_t scales_stride, uint32_t out_dtype, uint64_t bias,
+                                      uint64_t out, uint64_t out_stride, uint64_t tokens, uint64_t rows,
+                                      uint64_t cols, uint64_t stream, uint32_t device_ordinal) {
+  if ((!mx_float(x_dtype) && x_dtype != kTypeE4m3) || !mx_float(out_dtype)) return kUnsupported;
+  if (tokens > kMxMaxRows || rows > kMxMaxRows || cols == 0 || cols > kMxMaxCols || cols % kMxBlock)
+    return kInvalidInput;
+  if (tokens == 0 || rows == 0) return kOk;
+  const MxLinearArgs a{{x, x_stride}, {x_scales, x_scales_stride}, {weight, weight_stride}, {scales, scales_stride},
+                       {out, out_stride}, bias, tokens, (uint32_t)rows, (uint32_t)cols};
+  if (!mx_rows(a.x, tokens, cols) || !mx_rows(a.weight, rows, cols / 2) ||
+      !mx_rows(a.scales, rows, cols / kMxBlock) || !mx_rows(a.out, tokens, rows) ||
+      (x_dtype == kTypeE4m3) != (x_scales != 0) || (x_scales && !mx_rows(a.x_scales, tokens, cols / kMxBlock)))
+    return kInvalidInput;
+  OnDevice on(device_ordinal);
+  if (!on.ok) return kInvalidInput;
+  return mx_launched(launch_mxfp4_linear(x_dtype, out_dtype, a, reinterpret_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"
