@@ -37,6 +37,16 @@ __device__ __forceinline__ void st4(uint64_t a, uint32_t v) {
   ((__attribute__((address_space(1))) Bytes4*)(uintptr_t)a)->v = v;
 }
 
+// A uniform address and 32-bit offsets from it.
+typedef const __attribute__((address_space(1))) uint8_t* GlobalBytes;
+__device__ __forceinline__ GlobalBytes global_bytes(uint64_t a) { return (GlobalBytes)(uintptr_t)a; }
+__device__ __forceinline__ u32x4 ld16(GlobalBytes p, uint32_t at) {
+  return ((const __attribute__((address_space(1))) Bytes16*)(p + at))->v;
+}
+__device__ __forceinline__ uint32_t ld4(GlobalBytes p, uint32_t at) {
+  return ((const __attribute__((address_space(1))) Bytes4*)(p + at))->v;
+}
+
 __host__ __device__ constexpr uint32_t type_bytes(uint32_t type) {
   return type == kTypeF32 ? 4 : type == kTypeE4m3 ? 1 : 2;
 }
