@@ -1156,14 +1156,14 @@ int64_t ptwm_mi355x_mxfp4_linear_cuda(uint32_t x_dtype, uint64_t x, uint64_t x_s
     return kInvalidInput;
   if (tokens == 0 || rows == 0) return kOk;
   const MxLinearArgs a{{x, x_stride}, {x_scales, x_scales_stride}, {weight, weight_stride}, {scales, scales_stride},
-                       {out, out_stride}, bias, tokens, (uint32_t)rows, (uint32_t)cols};
+                       {out, out_stride}, bias, tokens, (uint32_t)rows, (uint32_t)cols, out_dtype};
   if (!mx_rows(a.x, tokens, cols) || !mx_rows(a.weight, rows, cols / 2) ||
       !mx_rows(a.scales, rows, cols / kMxBlock) || !mx_rows(a.out, tokens, rows) ||
       (x_dtype == kTypeE4m3) != (x_scales != 0) || (x_scales && !mx_rows(a.x_scales, tokens, cols / kMxBlock)))
     return kInvalidInput;
   OnDevice on(device_ordinal);
   if (!on.ok) return kInvalidInput;
-  return mx_launched(launch_mxfp4_linear(x_dtype, out_dtype, a, reinterpret_cast<hipStream_t>(stream)));
+  return mx_launched(launch_mxfp4_linear(x_dtype, a, reinterpret_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -68,9 +68,11 @@ __device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t w, float scale, bool h
 }
 
 // Eight values as bf16 parts, each cut from what the ones before it leave
-// (truncation, so nothing rounds up to infinity); the rest of an infinity or
-// NaN is zero, which keeps it what it is in the sum.  scale: of e4m3 codes,
-// read for its exponent only (byte 0 is 2^-127, 255 is NaN).
+// (truncation, so nothing rounds up to infinity).  The parts before the last
+// are finite, so an infinity or NaN is the last one, where it stays what it
+// is: NaN's highest mantissa bit is set by the subtraction.  scale: of e4m3
+// codes, read for its exponent only (byte 0 is 2^-127, 255 is NaN).
+constexpr float kBf16Max = 0x1.FEp127f;
 template <uint32_t T>
 __device__ __forceinline__ void parts_of_raw(const Raw8<T>& r, float scale, u32x4 (&p)[parts_of(T)]) {
   if constexpr (T == kTypeBf16) {
@@ -93,19 +95,21 @@ __device__ __forceinline__ void parts_of_raw(const Raw8<T>& r, float scale, u32x
       }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)  // a NaN whose cut would read as an infinity
-      if (v[i] != v[i]) v[i] = bits_f32(0x7FC00000u);
-#pragma unroll
     for (int j = 0; j < parts_of(T); ++j) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t b0 = f32_bits(v[2 * i]), b1 = f32_bits(v[2 * i + 1]);
-        p[j][i] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
-        if (j + 1 < parts_of(T)) {
-          const float h0 = bits_f32(b0 & 0xFFFF0000u), h1 = bits_f32(b1 & 0xFFFF0000u);
-          v[2 * i] = __builtin_isfinite(h0) ? v[2 * i] - h0 : 0.0f;
-          v[2 * i + 1] = __builtin_isfinite(h1) ? v[2 * i + 1] - h1 : 0.0f;
+        uint32_t b[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float& x = v[2 * i + e];
+          if (j + 1 < parts_of(T)) {
+            b[e] = f32_bits(__builtin_amdgcn_fmed3f(x, -kBf16Max, kBf16Max)) & 0xFFFF0000u;
+            x -= bits_f32(b[e]);
+          } else {
+            b[e] = f32_bits(x);
+          }
         }
+        p[j][i] = __builtin_amdgcn_perm(b[1], b[0], 0x07060302u);
       }
     }
   }
@@ -130,37 +134,40 @@ __device__ __forceinline__ f32x16 mfma32(bf16x8 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// The bias of outputs n .. n+3, zero past the last one or without a bias.
+// Outputs n .. n+3 of token t with their bias, those that exist.
 template <uint32_t OT>
-__device__ __forceinline__ void load_bias(const MxLinearArgs& a, uint32_t n, float (&b)[4]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    b[j] = a.bias && n + j < a.rows ? load1<OT>(a.bias + (uint64_t)(n + j) * type_bytes(OT)) : 0.0f;
-}
-
-// Outputs n .. n+3 of token t, those that exist.
-template <uint32_t OT>
-__device__ __forceinline__ void store4(const MxLinearArgs& a, uint64_t t, uint32_t n, f32x4 v, const float (&b)[4]) {
+__device__ __forceinline__ void store4_as(const MxLinearArgs& a, uint64_t t, uint32_t n, f32x4 v) {
   const uint64_t at = a.out.ptr + (t * a.out.stride + n) * type_bytes(OT);
-  float o[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) o[j] = v[j] + b[j];
   if (n + 3 < a.rows) {
+    if (a.bias) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += load1<OT>(a.bias + (uint64_t)(n + j) * type_bytes(OT));
+    }
     if constexpr (OT == kTypeF32)
-      st16(at, u32x4_make(f32_bits(o[0]), f32_bits(o[1]), f32_bits(o[2]), f32_bits(o[3])));
+      st16(at, __builtin_bit_cast(u32x4, v));
     else
-      st8(at, pack2<OT>(o[0], o[1]) | (uint64_t)pack2<OT>(o[2], o[3]) << 32);
+      st8(at, pack2<OT>(v[0], v[1]) | (uint64_t)pack2<OT>(v[2], v[3]) << 32);
   } else {
 #pragma unroll
     for (int j = 0; j < 3; ++j)
-      if (n + j < a.rows) store1<OT>(at + j * type_bytes(OT), o[j]);
+      if (n + j < a.rows)
+        store1<OT>(at + j * type_bytes(OT),
+                   a.bias ? v[j] + load1<OT>(a.bias + (uint64_t)(n + j) * type_bytes(OT)) : v[j]);
   }
+}
+__device__ __forceinline__ void store4(const MxLinearArgs& a, uint64_t t, uint32_t n, f32x4 v) {
+  if (a.out_type == kTypeBf16)
+    store4_as<kTypeBf16>(a, t, n, v);
+  else if (a.out_type == kTypeF16)
+    store4_as<kTypeF16>(a, t, n, v);
+  else
+    store4_as<kTypeF32>(a, t, n, v);
 }
 
 // A 16x16 tile of outputs by one workgroup, whose wavefronts take turns in
 // steps of 128 values (four blocks) along the rows and add up in LDS.  Lane l
 // holds weight row l % 16 and block l / 16 of the step, and token l % 16.
-template <uint32_t T, uint32_t OT>
+template <uint32_t T>
 __global__ __launch_bounds__(256) void mxfp4_linear_kernel(MxLinearArgs a) {
   __shared__ float part[4][16][17];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, i = lane & 15;
@@ -199,277 +206,418 @@ __global__ __launch_bounds__(256) void mxfp4_linear_kernel(MxLinearArgs a) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) part[wave][i][q * 4 + j] = acc[j];
   __syncthreads();
-  const uint32_t on = threadIdx.x & 15, ot = threadIdx.x >> 4;
-  if (n0 + on < a.rows && t0 + ot < a.tokens) {
-    float v = part[0][ot][on] + part[1][ot][on] + part[2][ot][on] + part[3][ot][on];
-    if (a.bias) v += load1<OT>(a.bias + (uint64_t)(n0 + on) * type_bytes(OT));
-    store1<OT>(a.out.ptr + ((t0 + ot) * a.out.stride + n0 + on) * type_bytes(OT), v);
+  if (threadIdx.x < 64) {
+    const uint32_t ot = threadIdx.x >> 2, on = (threadIdx.x & 3) * 4;
+    f32x4 v = {};
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += part[g][ot][on + j];
+    if (t0 + ot < a.tokens) store4(a, t0 + ot, n0 + on, v);
   }
 }
 
-// Many tokens: a tile of 128 * RT weight rows and 32 * CT tokens by one
-// workgroup of four wavefronts, 32 * RT rows each.
+// A tile of 32 * RT * RG weight rows and 32 * CT tokens by one workgroup of
+// RG * KG wavefronts: RG groups of 32 * RT rows each, and KG groups that take
+// turns in steps of 128 values (four blocks) along the rows and add up in LDS
+// at the end.
 //
-// A step takes 128 values (four blocks) of every row.  The tokens' share goes
-// through LDS as bf16 parts, two steps deep; every wavefront reads all of it.
-// bf16 whose rows lie at multiples of 16 bytes goes there by itself (DMA),
-// other types through registers, both while the step before is multiplied.
-// The weights of a wavefront are its own: they go from memory to registers as
-// codes, one step ahead, and are widened there.  Within a step the order
-// along k is free as long as both operands follow it: lane l's share of
-// weight row l % 32 is blocks l / 32 and 2 + l / 32, a 16-byte load each, and
-// product f of four takes a block's values 8f .. 8f+7.  A token's 16 chunks of
-// eight values (256 bytes, every bank once) are stored at chunk ^ token % 16,
-// so 16 lanes that read one chunk of 16 tokens meet 16 different groups of
-// four banks.
+// The tokens' share of a step goes through LDS; the RG wavefronts of a K group
+// load it together and each reads all of it (with RG = 1 a wavefront waits for
+// nobody until the end).  Values go there one step ahead, as they are, and are
+// widened or split as they are read (RAW), or through registers as bf16 parts,
+// where several wavefronts would split the same f16 or f32 values.  Rows are
+// held in 16-byte chunks, chunk ^ row in place (place()), so the 16 lanes that
+// read one chunk of 16 rows at a time meet every bank once.
 //
-// A row's 64 bytes of codes are requested in one go and its four scales as
-// one word: requests to the L2, a segment of one row each, bound an earlier
-// form that took them piece by piece.  Offsets within a tile are 32 bits on
-// top of uniform addresses (tiles_fit()), which is what leaves registers for
-// the operands in flight.
-template <uint32_t T, uint32_t OT, int RT, int CT, bool DMA>
-__global__ __launch_bounds__(256, 2) void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
+// The weights of a wavefront are its own.  Their codes go to LDS by DMA one
+// step ahead, four lanes to a row's 64 bytes, and are read and widened in the
+// matrix instruction's order, a row a lane: loading them in that order
+// straight to registers costs the address unit a cycle a lane (measured: 16
+// bytes a cycle and CU, against 60 this way).  A row's scales of a step are one
+// word, loaded by one lane and exchanged between the halves.  Within a step
+// the order along k is free as long as both operands follow it: lane l's share
+// of weight row l % 32 is blocks l / 32 and 2 + l / 32, and product f of four
+// takes a block's values 8f .. 8f+7.
+//
+// What goes to LDS as it is goes by DMA where it lies at multiples of 16 bytes
+// (ALIGNED) and through registers otherwise, to the same places: results do
+// not depend on how operands lie.  Offsets within a tile are 32 bits on top of uniform addresses
+// (tiles_fit()), which is what leaves registers for the operands in flight.
+
+// The place of 16-byte chunk c of row t among rows of S chunks.
+template <uint32_t S>
+__device__ __forceinline__ uint32_t place(uint32_t t, uint32_t c) {
+  constexpr uint32_t per = S < 16 ? 16 / S : 1;  // rows that meet all banks together
+  return t * S + (c ^ (t / per & (S < 16 ? S - 1 : 15)));
+}
+
+template <uint32_t T, int RT, int CT, int RG, int KG, bool RAW, bool ALIGNED>
+__global__ __launch_bounds__(64 * RG * KG, RG * KG <= 4 ? 1 + (RT * CT * RG > 16) : RG * KG / 4)
+void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
+  static_assert(RAW || parts_of(T) > 1, "what needs no split goes as it is");
   constexpr int P = parts_of(T);
-  constexpr uint32_t kTokens = 32 * CT, kRows = 128 * RT;
-  // a thread's pieces of the tokens' share: 16 e4m3 codes (two chunks) or one chunk each
-  constexpr int C8 = T == kTypeE4m3 ? 2 : 1, J = 2 * CT / C8;
-  constexpr uint32_t kPer = 16 / C8;  // pieces of a token
-  // two variables, so that a read of one does not wait for what is on its way to the other
-  __shared__ u32x4 even[P * kTokens * 16], odd[P * kTokens * 16];
+  constexpr uint32_t kTokens = 32 * CT, kRows = 32 * RT * RG, kLoaders = 64 * RG;
+  constexpr uint32_t S = RAW ? 8 * type_bytes(T) : 16;       // 16-byte chunks of a row (and part) in LDS
+  constexpr uint32_t kStage = (RAW ? 1 : P) * kTokens * S;   // chunks of a stage
+  // a thread's pieces of the tokens' share: a chunk as it is, or eight values to split
+  constexpr uint32_t kPer = RAW ? S : 16;                     // pieces of a token
+  constexpr uint32_t kPiece = RAW ? 16 : 8 * type_bytes(T);  // bytes of a piece
+  constexpr uint32_t kBlockPieces = kMxBlock * type_bytes(T) / kPiece;
+  constexpr int J = kTokens * kPer / kLoaders;
+  constexpr uint32_t kTokenStep = kLoaders / kPer;
+  constexpr uint32_t kCodes = 32 * RT * 4;  // chunks of a wavefront's weight codes
+  constexpr int XS = CT < 2 ? 1 : CT / 2;   // words of token scales of a lane
+  // variables of their own, so that a read of one does not wait for what is on its way to another
+  __shared__ u32x4 even_all[KG * kStage], odd_all[KG * kStage], codes_all[RG * KG * kCodes];
   const uint32_t lane = threadIdx.x & 63, h = lane >> 5, i = lane & 31;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t group = wave / RG, rg = wave % RG, loader = rg * 64 + lane;
+  u32x4* const even = even_all + group * kStage;
+  u32x4* const odd = odd_all + group * kStage;
+  u32x4* const codes = codes_all + wave * kCodes;
   const uint32_t row_tiles = (a.rows + kRows - 1) / kRows;
-  const uint32_t n0 = blockIdx.x % row_tiles * kRows + wave * 32 * RT;
+  const uint32_t n0 = blockIdx.x % row_tiles * kRows + rg * 32 * RT;
   const uint64_t t0 = (uint64_t)(blockIdx.x / row_tiles) * kTokens;
-  const uint32_t blocks = a.cols / kMxBlock, steps = (blocks + 3) / 4, tail = blocks & 3;
+  const uint32_t tokens = (uint32_t)min(a.tokens - t0, (uint64_t)kTokens);
+  const uint32_t blocks = a.cols / kMxBlock, steps = (blocks + 3) / 4, rounds = (steps + KG - 1) / KG;
   // a wavefront past the last row, or a lane's row or token past it, takes the last one and stores nothing
   const uint32_t nb = min(n0, a.rows - 1);
-  GlobalBytes w = global_bytes(a.weight.ptr + nb * a.weight.stride);
-  GlobalBytes s = global_bytes(a.scales.ptr + nb * a.scales.stride);
-  GlobalBytes x = global_bytes(a.x.ptr + t0 * a.x.stride * type_bytes(T));
-  GlobalBytes xsc = global_bytes(a.x_scales.ptr + t0 * a.x_scales.stride);
-  uint32_t wo[RT], so[RT], xo[J], xso[J];
+  const GlobalBytes w0 = global_bytes(a.weight.ptr + nb * a.weight.stride);
+  const GlobalBytes s0 = global_bytes(a.scales.ptr + nb * a.scales.stride);
+  const GlobalBytes x0 = global_bytes(a.x.ptr + t0 * a.x.stride * type_bytes(T));
+  const GlobalBytes c0 = global_bytes(a.x_scales.ptr + t0 * a.x_scales.stride);
+  uint32_t wo[2 * RT], xo[J], co[XS];
+  const uint32_t code_chunk = (lane & 3) ^ (lane >> 4);
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const uint32_t n = min(r * 32 + i, a.rows - 1 - nb);
-    wo[r] = n * (uint32_t)a.weight.stride;
-    so[r] = n * (uint32_t)a.scales.stride;
-  }
-  // through registers, thread by thread: its chunk's place in LDS is swizzled; by DMA the place is the lane's and the
-  // chunk is swizzled
-  const uint32_t token = threadIdx.x / kPer;
-  const uint32_t chunk = DMA ? (threadIdx.x & 15) ^ (token & 15) : threadIdx.x % kPer * C8;
+  for (int r = 0; r < 2 * RT; ++r)
+    wo[r] = min(r * 16 + lane / 4, a.rows - 1 - nb) * (uint32_t)a.weight.stride;
+  uint32_t so = min(RT == 2 ? lane : i, a.rows - 1 - nb) * (uint32_t)a.scales.stride;
+#pragma unroll
+  for (int c = 0; c < XS; ++c)
+    if constexpr (T == kTypeE4m3)
+      co[c] = min(CT < 2 ? i : c * 64 + lane, tokens - 1) * (uint32_t)a.x_scales.stride;
+  // by DMA a piece's place in LDS is the lane's and the piece follows from it, through registers the other way round
+  const uint32_t token = loader / kPer;
+  auto token_of = [&](int j) { return token + j * kTokenStep; };
+  auto piece_of = [&](int j) {
+    return RAW ? place<S>(token_of(j), loader % kPer) - token_of(j) * S : loader % kPer;
+  };
 #pragma unroll
   for (int j = 0; j < J; ++j) {
-    const uint32_t t = (uint32_t)min((uint64_t)(token + j * (256 / kPer)), a.tokens - 1 - t0);
-    xo[j] = (t * (uint32_t)a.x.stride + chunk * 8) * type_bytes(T);
-    if constexpr (T == kTypeE4m3) xso[j] = t * (uint32_t)a.x_scales.stride + chunk / 4;
+    const uint32_t t = min(token_of(j), tokens - 1);
+    xo[j] = t * (uint32_t)a.x.stride * type_bytes(T) + piece_of(j) * kPiece;
   }
-  u32x4 wv[2][2][RT];
-  uint32_t sv[2][RT];
-  // past a row's end, in the last step, its last block is loaded again, and cleared at its use; a word of scales
-  // ends where the row does
-  const uint32_t w_at[2] = {tail ? min(h, tail - 1) * 16 : h * 16, tail ? min(2 + h, tail - 1) * 16 : 32 + h * 16};
-  const uint32_t s_over = tail ? 4 - tail : 0;
-  const uint32_t x_over = tail && chunk / 4 >= tail ? chunk / 4 + 1 - tail : 0;  // never more blocks than lie before
-  auto load_weights = [&](int set, bool last) {
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      asm("" : "+v"(wo[r]), "+v"(so[r]));
-#pragma unroll
-      for (int m = 0; m < 2; ++m) wv[set][m][r] = ld16(w, wo[r] + (last ? w_at[m] : h * 16 + m * 32));
-    }
-#pragma unroll
-    for (int r = 0; r < RT; ++r) sv[set][r] = ld4(last ? s - s_over : s, so[r]);
+  const uint32_t loads = (tokens + kTokenStep - 1) / kTokenStep;  // of J, the ones with a token
+  // In the last round a group's step may end past the row or lie past it.  Loads then repeat the row's last step and
+  // block, and what they bring is cleared at its use; a word of scales ends where the row does.
+  struct Step {
+    uint32_t at;    // the step that is loaded
+    uint32_t left;  // blocks of it that count, up to four
+    uint32_t in;    // blocks of it that exist, one to four
   };
-  Raw8<T> raw[J][C8];
-  uint32_t xs[J];
-  auto load_tokens = [&](u32x4* stage, bool last) {
-    const uint32_t over = last ? x_over : 0;
+  auto step_of = [&](uint32_t round) {
+    const uint32_t want = round * KG + group;
+    Step p;
+    p.at = min(want, steps - 1);
+    p.in = min(blocks - p.at * 4, 4u);
+    p.left = want < steps ? p.in : 0;
+    return p;
+  };
+  u32x4 wr[2 * RT];     // codes on their way through registers
+  uint32_t sv, cv[XS];  // scales of a row and of tokens, a byte a block
+  auto load_weights = [&](const Step& p) {
+    GlobalBytes w = w0 + (uint64_t)p.at * 64, s = s0 + ((uint64_t)p.at * 4 + p.in - 4);
+    asm("" : "+s"(w), "+s"(s));  // kept uniform: otherwise the loop carries a 64-bit address for every load and lane
+#pragma unroll
+    for (int r = 0; r < 2 * RT; ++r) {
+      asm("" : "+v"(wo[r]));
+      const uint32_t at = wo[r] + min(code_chunk, p.in - 1) * 16;
+      if constexpr (ALIGNED)
+        __builtin_amdgcn_global_load_lds(w + at, (__attribute__((address_space(3))) void*)(codes + r * 64), 16, 0, 0);
+      else
+        wr[r] = ld16(w, at);
+    }
+    asm("" : "+v"(so));
+    sv = ld4(s, so);
+  };
+  Raw8<T> raw[J];  // values on their way through registers
+  u32x4 xr[J];
+  auto load_tokens = [&](u32x4* stage, const Step& p) {
+    GlobalBytes x = x0 + (uint64_t)p.at * (128 * type_bytes(T));
+    GlobalBytes c = c0 + ((uint64_t)p.at * 4 + p.in - 4);
+    asm("" : "+s"(x), "+s"(c));
+    if constexpr (T == kTypeE4m3) {
+#pragma unroll
+      for (int k = 0; k < XS; ++k) {
+        asm("" : "+v"(co[k]));
+        cv[k] = ld4(c, co[k]);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < J; ++j) {
+      if (RAW && ALIGNED && RG == 1 && j && (uint32_t)j >= loads) break;
       asm("" : "+v"(xo[j]));
+      const uint32_t b = piece_of(j) / kBlockPieces;
+      const uint32_t over = b - min(b, p.in - 1);  // blocks to go back: at least as many lie before
       const uint32_t at = xo[j] - over * (kMxBlock * type_bytes(T));
-      if constexpr (DMA) {
-        __builtin_amdgcn_global_load_lds(x + at, (__attribute__((address_space(3))) void*)(stage + j * 256 + wave * 64),
-                                         16, 0, 0);
-      } else if constexpr (T == kTypeE4m3) {
-        asm("" : "+v"(xso[j]));
-        const u32x4 v = ld16(x, at);
-        raw[j][0].w = v[0] | (uint64_t)v[1] << 32;
-        raw[j][1].w = v[2] | (uint64_t)v[3] << 32;
-        xs[j] = xsc[xso[j] - over];
+      if constexpr (RAW && ALIGNED) {
+        __builtin_amdgcn_global_load_lds(
+            x + at, (__attribute__((address_space(3))) void*)(stage + j * kLoaders + rg * 64), 16, 0, 0);
+      } else if constexpr (RAW) {
+        xr[j] = ld16(x, at);
       } else {
-        raw[j][0] = load_raw8<T>(x, at);
+        raw[j] = load_raw8<T>(x, at);
       }
     }
   };
-  auto store_tokens = [&](u32x4* stage) {
-    if constexpr (!DMA) {
+  auto store = [&](u32x4* stage) {  // what came through registers
+    if constexpr (!ALIGNED) {
+#pragma unroll
+      for (int r = 0; r < 2 * RT; ++r) codes[r * 64 + lane] = wr[r];
+    }
+    if constexpr (RAW && !ALIGNED) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) stage[j * kLoaders + loader] = xr[j];
+    }
+    if constexpr (!RAW) {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        const uint32_t t = token + j * (256 / kPer);
+        u32x4 p[P];
+        parts_of_raw<T>(raw[j], 1.0f, p);
 #pragma unroll
-        for (int g = 0; g < C8; ++g) {
-          u32x4 p[P];
-          parts_of_raw<T>(raw[j][g], T == kTypeE4m3 ? scale_f32(xs[j]) : 1.0f, p);
-#pragma unroll
-          for (int part = 0; part < P; ++part)
-            stage[(part * kTokens + t) * 16 + ((chunk + g) ^ (t & 15))] = p[part];
-        }
+        for (int part = 0; part < P; ++part)
+          stage[part * kTokens * S + place<S>(token_of(j), piece_of(j))] = p[part];
       }
     }
+  };
+  auto meet = [&] {
+    // a barrier waits for no DMA: each wavefront waits for its own, requested a step ago, before all meet
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if constexpr (RG > 1)
+      __syncthreads();
+    else
+      __builtin_amdgcn_wave_barrier();
   };
   f32x16 acc[RT][CT] = {};
-  // one step from one stage, while the next one's operands are on their way to the other; the last step stands alone,
-  // so that the loop has no branch at which all loads in flight would be waited for
-  auto multiply = [&](uint32_t step, auto set, u32x4* now, u32x4* next, auto last) {
-    const bool next_last = step + 2 == steps;
-    w += 64, s += 4, x += 128 * type_bytes(T), xsc += 4;  // of the next step
-    // kept uniform: without this the loop carries a 64-bit address for every load and lane
-    asm("" : "+s"(w), "+s"(s), "+s"(x), "+s"(xsc));
-    // a barrier waits for no DMA: each wavefront waits for its own, requested a step ago, before all meet
-    if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if constexpr (last)
-      if (tail) {  // what lies past the rows' ends
-        for (uint32_t at = threadIdx.x; at < P * kTokens * 16; at += 256)
-          if (((at & 15) ^ (at >> 4 & 15)) >= tail * 4) now[at] = u32x4{};
-        __syncthreads();
+  // one step from one stage, while the next one's operands are on their way; the last step stands alone, so that the
+  // loop has no branch at which all loads in flight would be waited for
+  auto multiply = [&](uint32_t round, u32x4* now, u32x4* next, auto last) {
+    meet();
+    const Step p = step_of(round);
+    if constexpr (last) {
+      if (p.left < 4) {
+        constexpr uint32_t kBlockChunks = S / 4;
+        for (uint32_t at = loader; at < kStage; at += kLoaders) {
+          const uint32_t t = at / S % kTokens;
+          if ((place<S>(t, at % S) - t * S) / kBlockChunks >= p.left) now[at] = u32x4{};
+        }
+        if constexpr (RG > 1) __syncthreads();
       }
-    if constexpr (!last) {
-      load_tokens(next, next_last);
-      load_weights(set ^ 1, next_last);
     }
-    // part p of product u of eight (block pair u / 4, values 8 (u % 4) ..): read one ahead
-    u32x4 x8[2][CT];
+    u32x4 wv[2][RT];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) wv[m][r] = codes[(r * 32 + i) * 4 + ((2 * m + h) ^ (i >> 2 & 3))];
+    // the word of row or token 32 k + l % 32 in lane l, from the lanes that loaded it
+    uint32_t sn[RT], cn[CT];
+    if constexpr (RT == 2) {
+      const auto both = __builtin_amdgcn_permlane32_swap(sv, sv, false, false);
+      sn[0] = both[0], sn[1] = both[1];
+    } else {
+      sn[0] = sv;
+    }
+    if constexpr (T == kTypeE4m3) {
+#pragma unroll
+      for (int k = 0; k < XS; ++k) {
+        if constexpr (CT < 2) {
+          cn[0] = cv[0];
+        } else {
+          const auto both = __builtin_amdgcn_permlane32_swap(cv[k], cv[k], false, false);
+          cn[2 * k] = both[0], cn[2 * k + 1] = both[1];
+        }
+      }
+    }
+    // Product u of eight takes values 8 (u % 4) .. of block pair u / 4.  Chunks are read one ahead: G of them for
+    // every kEach products (two for f32; one of e4m3 serves two), P times in parts.
+    constexpr int G = RAW && T == kTypeF32 ? 2 : 1, kEach = T == kTypeE4m3 ? 2 : 1;
+    constexpr int kParts = RAW ? 1 : P, kReads = 8 / kEach * kParts;
+    u32x4 x8[2][CT][G];
     auto read = [&](int v) {
-      const int u = v / P, part = P - 1 - v % P;
+      const int u = v / kParts * kEach, part = kParts - 1 - v % kParts;
+      const uint32_t chunk = ((u / 4 * 2 + h) * 4 + u % 4) * G / kEach;
 #pragma unroll
       for (int c = 0; c < CT; ++c)
-        x8[v & 1][c] = now[(part * kTokens + c * 32 + i) * 16 + (((u / 4 * 2 + h) * 4 + u % 4) ^ (i & 15))];
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+          x8[v & 1][c][g] = now[part * kTokens * S + place<S>(c * 32 + i, chunk + g)];
     };
     read(0);
+    if constexpr (!last) {
+      // the codes are in registers before new ones may arrive in their place
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      const Step q = step_of(round + 1);
+      load_weights(q);
+      load_tokens(next, q);
+    }
     bf16x8 w8[RT];
-    float sf[RT];
+    float sf[RT], cf[CT];
 #pragma unroll
-    for (int v = 0; v < 8 * P; ++v) {
-      const int u = v / P, m = u / 4;
+    for (int v = 0; v < 8 * kParts; ++v) {
+      const int u = v / kParts, m = u / 4, rd = v / kEach;
       // what is requested stays ahead of the products it hides behind
-      if (v + 1 < 8 * P) read(v + 1);
-      if (v % P == 0) {
-        const bool in = !last || tail == 0 || 2 * m + h < tail;
+      if (v % kEach == 0 && rd + 1 < kReads) read(rd + 1);
+      if (v % kParts == 0) {
+        const bool in = !last || 2 * m + h < p.left;
+        const uint32_t byte = 2 * m + h + (last ? 4 - p.in : 0);
+        const uint32_t shift = 8 * (byte & 3);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-          if (u % 4 == 0) {
-            const uint32_t byte = 2 * m + h + (last ? s_over : 0);
-            sf[r] = scale_f32(in ? sv[set][r] >> (8 * (byte & 3)) & 0xFF : 127);
-          }
-          w8[r] = weights8(in ? wv[set][m][r][u & 3] : 0, sf[r]);
+          if (u % 4 == 0) sf[r] = scale_f32(in ? sn[r] >> shift & 0xFF : 127);
+          w8[r] = weights8(in ? wv[m][r][u & 3] : 0, sf[r]);
+        }
+        if constexpr (T == kTypeE4m3) {
+#pragma unroll
+          for (int c = 0; c < CT; ++c)
+            if (u % 4 == 0) cf[c] = scale_f32(in ? cn[c] >> shift & 0xFF : 127);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int c = 0; c < CT; ++c)
+      for (int c = 0; c < CT; ++c) {
+        if constexpr (RAW) {
+          Raw8<T> r8;
+          if constexpr (T == kTypeE4m3) {
+            const uint32_t lo = x8[rd & 1][c][0][u % 2 * 2], hi = x8[rd & 1][c][0][u % 2 * 2 + 1];
+            r8.w = lo | (uint64_t)hi << 32;
+          } else {
 #pragma unroll
-        for (int r = 0; r < RT; ++r) acc[r][c] = mfma32(w8[r], x8[v & 1][c], acc[r][c]);
+            for (int g = 0; g < G; ++g) r8.w[g] = x8[rd & 1][c][g];
+          }
+          u32x4 b[P];
+          parts_of_raw<T>(r8, cf[c], b);
+#pragma unroll
+          for (int part = P - 1; part >= 0; --part)
+#pragma unroll
+            for (int r = 0; r < RT; ++r) acc[r][c] = mfma32(w8[r], b[part], acc[r][c]);
+        } else {
+#pragma unroll
+          for (int r = 0; r < RT; ++r) acc[r][c] = mfma32(w8[r], x8[rd & 1][c][0], acc[r][c]);
+        }
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (!last) store_tokens(next);
+    if constexpr (!last) store(next);
   };
-  constexpr std::integral_constant<int, 0> k0{};
-  constexpr std::integral_constant<int, 1> k1{};
-  load_tokens(even, steps == 1);
-  load_weights(0, steps == 1);
-  store_tokens(even);
-  uint32_t step = 0;
-  for (; step + 2 < steps; step += 2) {
-    multiply(step, k0, even, odd, std::false_type{});
-    multiply(step + 1, k1, odd, even, std::false_type{});
+  load_weights(step_of(0));
+  load_tokens(even, step_of(0));
+  store(even);
+  uint32_t round = 0;
+  for (; round + 2 < rounds; round += 2) {
+    multiply(round, even, odd, std::false_type{});
+    multiply(round + 1, odd, even, std::false_type{});
   }
   u32x4* stage = even;
-  if (step + 2 == steps) {
-    multiply(step++, k0, even, odd, std::false_type{});
-#pragma unroll
-    for (int r = 0; r < RT; ++r) wv[0][0][r] = wv[1][0][r], wv[0][1][r] = wv[1][1][r], sv[0][r] = sv[1][r];
+  if (round + 2 == rounds) {
+    multiply(round++, even, odd, std::false_type{});
     stage = odd;
   }
-  multiply(step, k0, stage, stage, std::true_type{});
+  multiply(round, stage, stage, std::true_type{});
+
   // lane l holds token l % 32 and rows 8 j + 4 (l / 32) .. + 3, j = 0 .. 3
+  constexpr int kQuads = RT * CT * 4;
+  auto write = [&](int quad, f32x4 v) {
+    const int r = quad / (CT * 4), c = quad / 4 % CT, j = quad % 4;
+    const uint64_t t = t0 + c * 32 + i;
+    if (t < a.tokens) store4(a, t, n0 + r * 32 + j * 8 + h * 4, v);
+  };
+  auto quad_of = [&](int quad) {
+    const int r = quad / (CT * 4), c = quad / 4 % CT, j = quad % 4;
+    return f32x4{acc[r][c][4 * j], acc[r][c][4 * j + 1], acc[r][c][4 * j + 2], acc[r][c][4 * j + 3]};
+  };
+  if constexpr (KG == 1) {
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
+    for (int quad = 0; quad < kQuads; ++quad) write(quad, quad_of(quad));
+  } else {
+    // the groups' sums take the place of their stages, in the order of the groups
+    constexpr uint32_t kFit = kStage / 64;
+    static_assert(RG == 1 && kQuads <= 2 * kFit, "a K group is a wavefront");
+    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t n = n0 + r * 32 + j * 8 + h * 4;
-      float bias[4];
-      load_bias<OT>(a, n, bias);
+    for (uint32_t quad = 0; quad < kQuads; ++quad)
+      (quad < kFit ? even + quad * 64 : odd + (quad - kFit) * 64)[lane] = __builtin_bit_cast(u32x4, quad_of(quad));
+    __syncthreads();
+    for (uint32_t quad = wave; quad < kQuads; quad += KG) {
+      const u32x4* from = quad < kFit ? even_all + quad * 64 : odd_all + (quad - kFit) * 64;
+      f32x4 v = {};
 #pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        const uint64_t t = t0 + c * 32 + i;
-        const f32x4 v = {acc[r][c][4 * j], acc[r][c][4 * j + 1], acc[r][c][4 * j + 2], acc[r][c][4 * j + 3]};
-        if (t < a.tokens) store4<OT>(a, t, n, v, bias);
-      }
+      for (int g = 0; g < KG; ++g) v += __builtin_bit_cast(f32x4, from[g * kStage + lane]);
+      write(quad, v);
     }
+  }
 }
 
-// Whether a tile's rows and tokens lie within 32-bit offsets, and a row's scales fill a word.
+// Whether a tile's rows and tokens lie within 32-bit offsets and a row's scales fill a word.
 bool tiles_fit(const MxLinearArgs& a) {
-  return a.cols >= 128 && a.weight.stride < (1u << 23) && a.x.stride < (1u << 23) && a.scales.stride < (1u << 23) &&
-         a.x_scales.stride < (1u << 23);
+  return a.cols >= 128 && a.weight.stride < (1u << 23) && a.x.stride < (1u << 23) && a.scales.stride < (1u << 23) && a.x_scales.stride < (1u << 23);
 }
 
-template <uint32_t T, int RT, int CT>
-hipError_t tiles_of(uint32_t out_type, const MxLinearArgs& a, hipStream_t stream) {
-  const uint64_t tiles =
-      (uint64_t)((a.rows + 128 * RT - 1) / (128 * RT)) * ((a.tokens + 32 * CT - 1) / (32 * CT));
+template <uint32_t T, int RT, int CT, int RG, int KG, bool RAW>
+hipError_t tiles_of(const MxLinearArgs& a, hipStream_t stream) {
+  constexpr uint32_t kRows = 32 * RT * RG, kTokens = 32 * CT;
+  const uint64_t tiles = (uint64_t)((a.rows + kRows - 1) / kRows) * ((a.tokens + kTokens - 1) / kTokens);
   if (tiles > 0x7FFFFFFFu) return hipErrorInvalidValue;
-  const dim3 grid((uint32_t)tiles), block(256);
-  if constexpr (T == kTypeBf16) {
-    if (a.x.ptr % 16 == 0 && a.x.stride % 8 == 0)
-      switch (out_type) {
-        case kTypeF32: hipLaunchKernelGGL((mxfp4_linear_tiles_kernel<T, kTypeF32, RT, CT, true>), grid, block, 0, stream, a); return hipGetLastError();
-        case kTypeF16: hipLaunchKernelGGL((mxfp4_linear_tiles_kernel<T, kTypeF16, RT, CT, true>), grid, block, 0, stream, a); return hipGetLastError();
-        case kTypeBf16: hipLaunchKernelGGL((mxfp4_linear_tiles_kernel<T, kTypeBf16, RT, CT, true>), grid, block, 0, stream, a); return hipGetLastError();
-        default: return hipErrorInvalidValue;
-      }
-  }
-  switch (out_type) {
-    case kTypeF32: hipLaunchKernelGGL((mxfp4_linear_tiles_kernel<T, kTypeF32, RT, CT, false>), grid, block, 0, stream, a); break;
-    case kTypeF16: hipLaunchKernelGGL((mxfp4_linear_tiles_kernel<T, kTypeF16, RT, CT, false>), grid, block, 0, stream, a); break;
-    case kTypeBf16: hipLaunchKernelGGL((mxfp4_linear_tiles_kernel<T, kTypeBf16, RT, CT, false>), grid, block, 0, stream, a); break;
-    default: return hipErrorInvalidValue;
-  }
+  const bool aligned = a.weight.ptr % 16 == 0 && a.weight.stride % 16 == 0 &&
+                       (!RAW || (a.x.ptr % 16 == 0 && a.x.stride * type_bytes(T) % 16 == 0));
+  const auto kernel = aligned ? mxfp4_linear_tiles_kernel<T, RT, CT, RG, KG, RAW, true>
+                              : mxfp4_linear_tiles_kernel<T, RT, CT, RG, KG, RAW, false>;
+  hipLaunchKernelGGL(kernel, dim3((uint32_t)tiles), dim3(64 * RG * KG), 0, stream, a);
   return hipGetLastError();
 }
 
-// 32s of tokens of a workgroup's tile, by the LDS that their parts take.
 template <uint32_t T>
-constexpr int kTileTokens = T == kTypeF32 ? 1 : T == kTypeF16 ? 2 : 4;
+hipError_t tiles_by_size(const MxLinearArgs& a, hipStream_t stream) {
+  constexpr bool kPlain = parts_of(T) == 1;
+  constexpr int CT = T == kTypeF32 ? 1 : T == kTypeF16 ? 2 : 4, KG = T == kTypeF32 ? 4 : 8;
+  auto count = [&](uint64_t rows, uint64_t tokens) {
+    return ((a.rows + rows - 1) / rows) * ((a.tokens + tokens - 1) / tokens);
+  };
+  // Tiles of 256 rows where there are enough for the 256 CUs, otherwise smaller ones whose wavefronts share the length
+  // of the rows: measured (us, 256-row tiles against the one taken) 512x14336x4096 bf16 (224 tiles) 68 and 100,
+  // 256x14336x4096 bf16 (112) 63 and 50, e4m3 66 and 41, 100x4096x4096 e4m3 (16) 63 and 8.9.
+  if (count(256, 32 * CT) >= 160) return tiles_of<T, 2, CT, 4, 1, kPlain>(a, stream);
+  // As many wavefronts to a tile as LDS holds where each tile has a CU of its own: 45x1354x960 bf16 (86 tiles of 32
+  // rows) 4.0 and 4.8 with four, 100x4096x4096 e4m3 (256 of 64 rows) 8.9 and 9.3.
+  if (count(32, 32) <= 128) return tiles_of<T, 1, 1, 1, KG, true>(a, stream);
+  // Few tokens read each weight once, and more, smaller tiles keep more of them in flight: 1x14336x4096 bf16 7.7 and
+  // 8.2 with 64 rows.
+  if (a.tokens <= 16 && count(32, 32) <= 512) return tiles_of<T, 1, 1, 1, 4, true>(a, stream);
+  if (count(64, 32) <= 256) return tiles_of<T, 2, 1, 1, KG, true>(a, stream);
+  // Two workgroups share a CU's LDS with 64 tokens of e4m3, with 32 of the others: 700x3000x2048 bf16 21 and 26 with
+  // 64 tokens, 256x14336x4096 e4m3 41 and 48 with 32.
+  if constexpr (T == kTypeE4m3)
+    if (a.tokens > 32) return tiles_of<T, 2, 2, 1, 4, true>(a, stream);
+  return tiles_of<T, 2, 1, 1, 4, true>(a, stream);
+}
 
 template <uint32_t T>
-hipError_t linear_of(uint32_t out_type, const MxLinearArgs& a, hipStream_t stream) {
-  if (a.tokens > 64 && tiles_fit(a)) return tiles_of<T, 2, kTileTokens<T>>(out_type, a, stream);
+hipError_t linear_of(const MxLinearArgs& a, hipStream_t stream) {
+  if (tiles_fit(a)) return tiles_by_size<T>(a, stream);
   const uint64_t tiles = (uint64_t)((a.rows + 15) / 16) * ((a.tokens + 15) / 16);
   if (tiles > 0x7FFFFFFFu) return hipErrorInvalidValue;
-  const dim3 grid((uint32_t)tiles), block(256);
-  switch (out_type) {
-    case kTypeF32: hipLaunchKernelGGL((mxfp4_linear_kernel<T, kTypeF32>), grid, block, 0, stream, a); break;
-    case kTypeF16: hipLaunchKernelGGL((mxfp4_linear_kernel<T, kTypeF16>), grid, block, 0, stream, a); break;
-    case kTypeBf16: hipLaunchKernelGGL((mxfp4_linear_kernel<T, kTypeBf16>), grid, block, 0, stream, a); break;
-    default: return hipErrorInvalidValue;
-  }
+  hipLaunchKernelGGL(mxfp4_linear_kernel<T>, dim3((uint32_t)tiles), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_mxfp4_linear(uint32_t x_type, uint32_t out_type, const MxLinearArgs& a, hipStream_t stream) {
+hipError_t launch_mxfp4_linear(uint32_t x_type, const MxLinearArgs& a, hipStream_t stream) {
   switch (x_type) {
-    case kTypeF32: return linear_of<kTypeF32>(out_type, a, stream);
-    case kTypeF16: return linear_of<kTypeF16>(out_type, a, stream);
-    case kTypeBf16: return linear_of<kTypeBf16>(out_type, a, stream);
-    case kTypeE4m3: return linear_of<kTypeE4m3>(out_type, a, stream);
+    case kTypeF32: return linear_of<kTypeF32>(a, stream);
+    case kTypeF16: return linear_of<kTypeF16>(a, stream);
+    case kTypeBf16: return linear_of<kTypeBf16>(a, stream);
+    case kTypeE4m3: return linear_of<kTypeE4m3>(a, stream);
     default: return hipErrorInvalidValue;
   }
 }

@@ -42,11 +42,12 @@ struct MxLinearArgs {
   uint64_t tokens;
   uint32_t rows;   // output features
   uint32_t cols;   // input features, a multiple of kMxBlock
+  uint32_t out_type;
 };
 
 // Each queues its work on `stream` of the current device and returns.
 hipError_t launch_rms_norm_mx(uint32_t type, uint32_t weight_type, const MxNormArgs& a, hipStream_t stream);
 hipError_t launch_swiglu_mx(uint32_t type, const MxSwigluArgs& a, hipStream_t stream);
-hipError_t launch_mxfp4_linear(uint32_t x_type, uint32_t out_type, const MxLinearArgs& a, hipStream_t stream);
+hipError_t launch_mxfp4_linear(uint32_t x_type, const MxLinearArgs& a, hipStream_t stream);
 
 }  // namespace ptwm
