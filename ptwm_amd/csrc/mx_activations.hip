@@ -87,14 +87,12 @@ __global__ __launch_bounds__(256) void swiglu_mx_kernel(MxSwigluArgs a) {
 
 template <uint32_t T>
 hipError_t norm_of(uint32_t weight_type, const MxNormArgs& a, hipStream_t stream) {
-  const dim3 grid((uint32_t)a.rows), block(kNormThreads);
   switch (weight_type) {
-    case kTypeF32: hipLaunchKernelGGL((rms_norm_mx_kernel<T, kTypeF32>), grid, block, 0, stream, a); break;
-    case kTypeF16: hipLaunchKernelGGL((rms_norm_mx_kernel<T, kTypeF16>), grid, block, 0, stream, a); break;
-    case kTypeBf16: hipLaunchKernelGGL((rms_norm_mx_kernel<T, kTypeBf16>), grid, block, 0, stream, a); break;
+    case kTypeF32: return launch(rms_norm_mx_kernel<T, kTypeF32>, a.rows, kNormThreads, a, stream);
+    case kTypeF16: return launch(rms_norm_mx_kernel<T, kTypeF16>, a.rows, kNormThreads, a, stream);
+    case kTypeBf16: return launch(rms_norm_mx_kernel<T, kTypeBf16>, a.rows, kNormThreads, a, stream);
     default: return hipErrorInvalidValue;
   }
-  return hipGetLastError();
 }
 
 }  // namespace
@@ -110,14 +108,12 @@ hipError_t launch_rms_norm_mx(uint32_t type, uint32_t weight_type, const MxNormA
 
 hipError_t launch_swiglu_mx(uint32_t type, const MxSwigluArgs& a, hipStream_t stream) {
   const uint64_t groups = (a.rows * (a.cols / 8) + 255) / 256;
-  const dim3 grid((uint32_t)groups), block(256);
   switch (type) {
-    case kTypeF32: hipLaunchKernelGGL(swiglu_mx_kernel<kTypeF32>, grid, block, 0, stream, a); break;
-    case kTypeF16: hipLaunchKernelGGL(swiglu_mx_kernel<kTypeF16>, grid, block, 0, stream, a); break;
-    case kTypeBf16: hipLaunchKernelGGL(swiglu_mx_kernel<kTypeBf16>, grid, block, 0, stream, a); break;
+    case kTypeF32: return launch(swiglu_mx_kernel<kTypeF32>, groups, 256, a, stream);
+    case kTypeF16: return launch(swiglu_mx_kernel<kTypeF16>, groups, 256, a, stream);
+    case kTypeBf16: return launch(swiglu_mx_kernel<kTypeBf16>, groups, 256, a, stream);
     default: return hipErrorInvalidValue;
   }
-  return hipGetLastError();
 }
 
 }  // namespace ptwm

@@ -6,6 +6,14 @@
 
 namespace ptwm {
 
+// One launch with one argument; the triple chevrons' way keeps a stack of configurations besides.
+template <typename A>
+hipError_t launch(void (*kernel)(A), uint64_t groups, uint32_t threads, const A& a, hipStream_t stream) {
+  if (groups > 0x7FFFFFFFu) return hipErrorInvalidValue;
+  void* args[] = {const_cast<A*>(&a)};
+  return hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3((uint32_t)groups), dim3(threads), args, 0, stream);
+}
+
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));

@@ -567,13 +567,11 @@ template <uint32_t T, int RT, int CT, int RG, int KG, bool RAW>
 hipError_t tiles_of(const MxLinearArgs& a, hipStream_t stream) {
   constexpr uint32_t kRows = 32 * RT * RG, kTokens = 32 * CT;
   const uint64_t tiles = (uint64_t)((a.rows + kRows - 1) / kRows) * ((a.tokens + kTokens - 1) / kTokens);
-  if (tiles > 0x7FFFFFFFu) return hipErrorInvalidValue;
   const bool aligned = a.weight.ptr % 16 == 0 && a.weight.stride % 16 == 0 &&
                        (!RAW || (a.x.ptr % 16 == 0 && a.x.stride * type_bytes(T) % 16 == 0));
-  const auto kernel = aligned ? mxfp4_linear_tiles_kernel<T, RT, CT, RG, KG, RAW, true>
-                              : mxfp4_linear_tiles_kernel<T, RT, CT, RG, KG, RAW, false>;
-  hipLaunchKernelGGL(kernel, dim3((uint32_t)tiles), dim3(64 * RG * KG), 0, stream, a);
-  return hipGetLastError();
+  return launch(aligned ? mxfp4_linear_tiles_kernel<T, RT, CT, RG, KG, RAW, true>
+                        : mxfp4_linear_tiles_kernel<T, RT, CT, RG, KG, RAW, false>,
+                tiles, 64 * RG * KG, a, stream);
 }
 
 template <uint32_t T>
@@ -605,9 +603,7 @@ template <uint32_t T>
 hipError_t linear_of(const MxLinearArgs& a, hipStream_t stream) {
   if (tiles_fit(a)) return tiles_by_size<T>(a, stream);
   const uint64_t tiles = (uint64_t)((a.rows + 15) / 16) * ((a.tokens + 15) / 16);
-  if (tiles > 0x7FFFFFFFu) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(mxfp4_linear_kernel<T>, dim3((uint32_t)tiles), dim3(256), 0, stream, a);
-  return hipGetLastError();
+  return launch(mxfp4_linear_kernel<T>, tiles, 256, a, stream);
 }
 
 }  // namespace
