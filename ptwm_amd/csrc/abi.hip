@@ -1120,13 +1120,13 @@ int64_t ptwm_mi355x_rms_norm_mx_cuda(uint32_t dtype, uint64_t x, uint64_t x_stri
   if (rows > kMxMaxRows || cols == 0 || cols > kMxMaxCols || cols % kMxBlock) return kInvalidInput;
   if (rows == 0) return kOk;
   const MxNormArgs a{{x, x_stride}, {residual, residual_stride}, {sum, sum_stride}, {codes, codes_stride},
-                     {scales, scales_stride}, weight, rows, (uint32_t)cols, eps};
+                     {scales, scales_stride}, weight, rows, (uint32_t)cols, eps, weight_dtype};
   if (!mx_rows(a.x, rows, cols) || !mx_rows(a.codes, rows, cols) || !mx_rows(a.scales, rows, cols / kMxBlock) ||
       !weight || (residual && !mx_rows(a.residual, rows, cols)) || (sum && !mx_rows(a.sum, rows, cols)))
     return kInvalidInput;
   OnDevice on(device_ordinal);
   if (!on.ok) return kInvalidInput;
-  return mx_launched(launch_rms_norm_mx(dtype, weight_dtype, a, reinterpret_cast<hipStream_t>(stream)));
+  return mx_launched(launch_rms_norm_mx(dtype, a, reinterpret_cast<hipStream_t>(stream)));
 }
 
 int64_t ptwm_mi355x_swiglu_mx_cuda(uint32_t dtype, uint64_t gate, uint64_t gate_stride, uint64_t up,

@@ -12,7 +12,7 @@
 namespace ptwm {
 namespace {
 
-constexpr uint32_t kNormThreads = 256;
+constexpr uint32_t kThreads = 256;
 
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
@@ -20,57 +20,117 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
+__device__ __forceinline__ void load_weight8(const MxNormArgs& a, uint32_t c, float (&v)[8]) {
+  if (a.weight_type == kTypeBf16)
+    load8<kTypeBf16>(a.weight + (uint64_t)c * 2, v);
+  else if (a.weight_type == kTypeF16)
+    load8<kTypeF16>(a.weight + (uint64_t)c * 2, v);
+  else
+    load8<kTypeF32>(a.weight + (uint64_t)c * 4, v);
+}
+
+// Codes and scale of a row's values c .. c+7.
+__device__ __forceinline__ void store_codes(const MxRows& codes, const MxRows& scales, uint64_t row, uint64_t c,
+                                            const float (&v)[8]) {
+  uint32_t lo, hi;
+  const uint32_t b = quantise8(v, lo, hi);
+  st8(codes.ptr + row * codes.stride + c, lo | (uint64_t)hi << 32);
+  if ((threadIdx.x & 3) == 0) g_st<uint8_t>(scales.ptr + row * scales.stride + c / kMxBlock, (uint8_t)b);
+}
+
 // s = x + residual, y = s * rsqrt(mean(s^2) + eps) * weight in 32 bits; sum
-// receives s in x's type, codes and scales receive y.  One workgroup a row.
-template <uint32_t T, uint32_t WT>
-__global__ __launch_bounds__(kNormThreads) void rms_norm_mx_kernel(MxNormArgs a) {
-  __shared__ float part[kNormThreads / 64];
-  const uint64_t row = blockIdx.x;
+// receives s in x's type, codes and scales receive y.  W wavefronts to a row,
+// which they hold in registers in CH pieces of 8 values a thread, so each
+// input is read once, all of it requested before any is used; with CH = 0 rows
+// of any length are read twice.
+template <uint32_t T, int W, int CH>
+__global__ __launch_bounds__(W > 4 ? 64 * W : kThreads) void rms_norm_mx_kernel(MxNormArgs a) {
+  constexpr uint32_t kRowThreads = 64 * W, kRows = W > 4 ? 1 : 4 / W;
+  __shared__ float part[W];
+  const uint64_t row = (uint64_t)blockIdx.x * kRows + threadIdx.x / kRowThreads;
+  if (kRows > 1 && row >= a.rows) return;  // whole wavefronts, which meet no other
+  const uint32_t first = threadIdx.x % kRowThreads * 8;
   const uint64_t x = a.x.ptr + row * a.x.stride * type_bytes(T);
   const uint64_t r = a.residual.ptr + row * a.residual.stride * type_bytes(T);
-  auto load = [&](uint32_t c, float(&v)[8]) {
-    load8<T>(x + (uint64_t)c * type_bytes(T), v);
+  constexpr int N = CH ? CH : 1;
+  Raw8<T> xv[N], rv[N];
+  float v[N][8], w[N][8], total = 0;
+  auto request = [&](int k, uint32_t c) {
+    xv[k] = load_raw8<T>(x + (uint64_t)c * type_bytes(T));
+    if (a.residual.ptr) rv[k] = load_raw8<T>(r + (uint64_t)c * type_bytes(T));
+  };
+  auto take = [&](int k) {
+    values_of<T>(xv[k], v[k]);
     if (a.residual.ptr) {
-      float w[8];
-      load8<T>(r + (uint64_t)c * type_bytes(T), w);
+      float u[8];
+      values_of<T>(rv[k], u);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] += w[i];
+      for (int i = 0; i < 8; ++i) v[k][i] += u[i];
     }
   };
-  float total = 0;
-  for (uint32_t c = threadIdx.x * 8; c < a.cols; c += kNormThreads * 8) {
-    float v[8];
-    load(c, v);
+  auto add = [&](int k) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) total += v[i] * v[i];
+    for (int i = 0; i < 8; ++i) total += v[k][i] * v[k][i];
+  };
+  if constexpr (CH > 0) {
+    // past the row's end its last piece is loaded again and not used
+#pragma unroll
+    for (int k = 0; k < CH; ++k) request(k, min(first + k * kRowThreads * 8, a.cols - 8));
+#pragma unroll
+    for (int k = 0; k < CH; ++k) load_weight8(a, min(first + k * kRowThreads * 8, a.cols - 8), w[k]);
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      take(k);
+      if (first + k * kRowThreads * 8 < a.cols) add(k);
+    }
+  } else {
+    for (uint32_t c = first; c < a.cols; c += kRowThreads * 8) {
+      request(0, c);
+      take(0);
+      add(0);
+    }
   }
   total = wave_sum(total);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = total;
-  __syncthreads();
-  total = 0;
+  if constexpr (kRows == 1) {
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = total;
+    __syncthreads();
+    total = 0;
 #pragma unroll
-  for (uint32_t i = 0; i < kNormThreads / 64; ++i) total += part[i];
+    for (int i = 0; i < W; ++i) total += part[i];
+  }
   const float scale = 1.0f / sqrtf(total / (float)a.cols + a.eps);
-  // the sum is written here, after its last read: it may be x or the residual
-  for (uint32_t c = threadIdx.x * 8; c < a.cols; c += kNormThreads * 8) {
-    float v[8], w[8];
-    load(c, v);
-    if (a.sum.ptr) store8<T>(a.sum.ptr + (row * a.sum.stride + c) * type_bytes(T), v);
-    load8<WT>(a.weight + (uint64_t)c * type_bytes(WT), w);
+  auto finish = [&](uint32_t c, float(&y)[8], const float(&g)[8]) {
+    if (a.sum.ptr) store8<T>(a.sum.ptr + (row * a.sum.stride + c) * type_bytes(T), y);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = v[i] * scale * w[i];
-    uint32_t lo, hi;
-    const uint32_t b = quantise8(v, lo, hi);
-    st8(a.codes.ptr + row * a.codes.stride + c, lo | (uint64_t)hi << 32);
-    if ((threadIdx.x & 3) == 0) g_st<uint8_t>(a.scales.ptr + row * a.scales.stride + c / kMxBlock, (uint8_t)b);
+    for (int i = 0; i < 8; ++i) y[i] = y[i] * scale * g[i];
+    store_codes(a.codes, a.scales, row, c, y);
+  };
+  // the sum is written after the last read of its place: it may be x or the residual
+  if constexpr (CH > 0) {
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const uint32_t c = first + k * kRowThreads * 8;
+      if (c < a.cols) finish(c, v[k], w[k]);
+    }
+  } else {
+    for (uint32_t c = first; c < a.cols; c += kRowThreads * 8) {
+      request(0, c);
+      load_weight8(a, c, w[0]);
+      take(0);
+      finish(c, v[0], w[0]);
+    }
   }
 }
 
-// y = gate / (1 + exp(-gate)) * up in 32 bits.
+// y = gate / (1 + exp(-gate)) * up in 32 bits.  The exponential and the
+// reciprocal are the hardware's, each within a unit in the last place: with
+// the library's exact forms the arithmetic took longer than the memory
+// (2048x14336 bf16: 35 us).  The reciprocal is taken of a quarter, so that it
+// stays a normal number as far as the exponential is finite.
 template <uint32_t T>
-__global__ __launch_bounds__(256) void swiglu_mx_kernel(MxSwigluArgs a) {
+__global__ __launch_bounds__(kThreads) void swiglu_mx_kernel(MxSwigluArgs a) {
   const uint32_t per_row = a.cols / 8;
-  const uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  const uint64_t at = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
   const uint64_t row = at / per_row;
   if (row >= a.rows) return;
   const uint64_t c = (at - row * per_row) * 8;
@@ -78,40 +138,49 @@ __global__ __launch_bounds__(256) void swiglu_mx_kernel(MxSwigluArgs a) {
   load8<T>(a.gate.ptr + (row * a.gate.stride + c) * type_bytes(T), g);
   load8<T>(a.up.ptr + (row * a.up.stride + c) * type_bytes(T), u);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) g[i] = g[i] / (1.0f + expf(-g[i])) * u[i];
-  uint32_t lo, hi;
-  const uint32_t b = quantise8(g, lo, hi);
-  st8(a.codes.ptr + row * a.codes.stride + c, lo | (uint64_t)hi << 32);
-  if ((threadIdx.x & 3) == 0) g_st<uint8_t>(a.scales.ptr + row * a.scales.stride + c / kMxBlock, (uint8_t)b);
+  for (int i = 0; i < 8; ++i) {
+    const float e = __builtin_amdgcn_exp2f(g[i] * -1.4426950408889634f);
+    g[i] = g[i] * 0.25f * __builtin_amdgcn_rcpf(__builtin_fmaf(e, 0.25f, 0.25f)) * u[i];
+  }
+  store_codes(a.codes, a.scales, row, c, g);
+}
+
+template <uint32_t T, int W, int CH>
+hipError_t norm_by(const MxNormArgs& a, hipStream_t stream) {
+  constexpr int kRows = W > 4 ? 1 : 4 / W;
+  return launch(rms_norm_mx_kernel<T, W, CH>, (a.rows + kRows - 1) / kRows, W > 4 ? 64 * W : kThreads, a, stream);
 }
 
 template <uint32_t T>
-hipError_t norm_of(uint32_t weight_type, const MxNormArgs& a, hipStream_t stream) {
-  switch (weight_type) {
-    case kTypeF32: return launch(rms_norm_mx_kernel<T, kTypeF32>, a.rows, kNormThreads, a, stream);
-    case kTypeF16: return launch(rms_norm_mx_kernel<T, kTypeF16>, a.rows, kNormThreads, a, stream);
-    case kTypeBf16: return launch(rms_norm_mx_kernel<T, kTypeBf16>, a.rows, kNormThreads, a, stream);
-    default: return hipErrorInvalidValue;
-  }
+hipError_t norm_of(const MxNormArgs& a, hipStream_t stream) {
+  // Few pieces a thread: measured (us, against four wavefronts with as many pieces as it takes) 1x4096 bf16 2.7 and 2.9,
+  // 2048x4096 11.3 and 11.5, 64x14336 4.4 and 8.4, 2048x8192 25.5 and 27.4.
+  if (a.cols <= 512) return norm_by<T, 1, 1>(a, stream);
+  if (a.cols <= 1024) return norm_by<T, 1, 2>(a, stream);
+  if (a.cols <= 2048) return norm_by<T, 4, 1>(a, stream);
+  if (a.cols <= 4096) return norm_by<T, 8, 1>(a, stream);
+  if (a.cols <= 8192) return norm_by<T, 16, 1>(a, stream);
+  if (a.cols <= 16384) return norm_by<T, 16, 2>(a, stream);
+  return norm_by<T, 16, 0>(a, stream);
 }
 
 }  // namespace
 
-hipError_t launch_rms_norm_mx(uint32_t type, uint32_t weight_type, const MxNormArgs& a, hipStream_t stream) {
+hipError_t launch_rms_norm_mx(uint32_t type, const MxNormArgs& a, hipStream_t stream) {
   switch (type) {
-    case kTypeF32: return norm_of<kTypeF32>(weight_type, a, stream);
-    case kTypeF16: return norm_of<kTypeF16>(weight_type, a, stream);
-    case kTypeBf16: return norm_of<kTypeBf16>(weight_type, a, stream);
+    case kTypeF32: return norm_of<kTypeF32>(a, stream);
+    case kTypeF16: return norm_of<kTypeF16>(a, stream);
+    case kTypeBf16: return norm_of<kTypeBf16>(a, stream);
     default: return hipErrorInvalidValue;
   }
 }
 
 hipError_t launch_swiglu_mx(uint32_t type, const MxSwigluArgs& a, hipStream_t stream) {
-  const uint64_t groups = (a.rows * (a.cols / 8) + 255) / 256;
+  const uint64_t groups = (a.rows * (a.cols / 8) + kThreads - 1) / kThreads;
   switch (type) {
-    case kTypeF32: return launch(swiglu_mx_kernel<kTypeF32>, groups, 256, a, stream);
-    case kTypeF16: return launch(swiglu_mx_kernel<kTypeF16>, groups, 256, a, stream);
-    case kTypeBf16: return launch(swiglu_mx_kernel<kTypeBf16>, groups, 256, a, stream);
+    case kTypeF32: return launch(swiglu_mx_kernel<kTypeF32>, groups, kThreads, a, stream);
+    case kTypeF16: return launch(swiglu_mx_kernel<kTypeF16>, groups, kThreads, a, stream);
+    case kTypeBf16: return launch(swiglu_mx_kernel<kTypeBf16>, groups, kThreads, a, stream);
     default: return hipErrorInvalidValue;
   }
 }

@@ -62,28 +62,53 @@ __host__ __device__ constexpr uint32_t type_bytes(uint32_t type) {
 __device__ __forceinline__ float bits_f32(uint32_t b) { return __builtin_bit_cast(float, b); }
 __device__ __forceinline__ uint32_t f32_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
 
-// Eight consecutive values of type T at address a, in 32 bits.
+// Eight consecutive values of type T as they lie in memory, and in 32 bits.
 template <uint32_t T>
-__device__ __forceinline__ void load8(uint64_t a, float (&v)[8]) {
-  const u32x4 w = ld16(a);
-  if constexpr (T == kTypeF32) {
-    const u32x4 z = ld16(a + 16);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = bits_f32(w[i]), v[4 + i] = bits_f32(z[i]);
+struct Raw8 {
+  u32x4 w[T == kTypeF32 ? 2 : 1];
+};
+template <>
+struct Raw8<kTypeE4m3> {
+  uint64_t w;
+};
+template <uint32_t T>
+__device__ __forceinline__ Raw8<T> load_raw8(uint64_t a) {
+  Raw8<T> r;
+  if constexpr (T == kTypeE4m3) {
+    r.w = ld8(a);
   } else {
+    r.w[0] = ld16(a);
+    if constexpr (T == kTypeF32) r.w[1] = ld16(a + 16);
+  }
+  return r;
+}
+template <uint32_t T>
+__device__ __forceinline__ Raw8<T> load_raw8(GlobalBytes p, uint32_t at) {
+  Raw8<T> r;
+  r.w[0] = ld16(p, at);
+  if constexpr (T == kTypeF32) r.w[1] = ld16(p, at + 16);
+  return r;
+}
+template <uint32_t T>
+__device__ __forceinline__ void values_of(const Raw8<T>& r, float (&v)[8]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t both = w[i];
-      if constexpr (T == kTypeBf16) {
-        v[2 * i] = bits_f32(both << 16);
-        v[2 * i + 1] = bits_f32(both & 0xFFFF0000u);
-      } else {
-        const f16x2 h = __builtin_bit_cast(f16x2, both);
-        v[2 * i] = (float)h[0];
-        v[2 * i + 1] = (float)h[1];
-      }
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a = r.w[0][i];
+    if constexpr (T == kTypeF32) {
+      const uint32_t b = r.w[1][i];
+      v[i] = bits_f32(a), v[4 + i] = bits_f32(b);
+    } else if constexpr (T == kTypeBf16) {
+      v[2 * i] = bits_f32(a << 16);
+      v[2 * i + 1] = bits_f32(a & 0xFFFF0000u);
+    } else {
+      const f16x2 h = __builtin_bit_cast(f16x2, a);
+      v[2 * i] = (float)h[0], v[2 * i + 1] = (float)h[1];
     }
   }
+}
+template <uint32_t T>
+__device__ __forceinline__ void load8(uint64_t a, float (&v)[8]) {
+  values_of<T>(load_raw8<T>(a), v);
 }
 
 // Two values rounded to nearest even in a 16-bit type.

@@ -33,35 +33,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 // bf16 parts that hold a value of type T exactly.
 constexpr int parts_of(uint32_t type) { return type == kTypeF32 ? 3 : type == kTypeF16 ? 2 : 1; }
 
-// Eight values of type T as they lie in memory.
-template <uint32_t T>
-struct Raw8 {
-  u32x4 w[T == kTypeF32 ? 2 : 1];
-};
-template <>
-struct Raw8<kTypeE4m3> {
-  uint64_t w;
-};
-template <uint32_t T>
-__device__ __forceinline__ Raw8<T> load_raw8(uint64_t a) {
-  Raw8<T> r;
-  if constexpr (T == kTypeE4m3) {
-    r.w = ld8(a);
-  } else {
-    r.w[0] = ld16(a);
-    if constexpr (T == kTypeF32) r.w[1] = ld16(a + 16);
-  }
-  return r;
-}
-
-template <uint32_t T>
-__device__ __forceinline__ Raw8<T> load_raw8(GlobalBytes p, uint32_t at) {
-  Raw8<T> r;
-  r.w[0] = ld16(p, at);
-  if constexpr (T == kTypeF32) r.w[1] = ld16(p, at + 16);
-  return r;
-}
-
 __device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t w, float scale, bool high) {
   return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))
               : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
@@ -83,17 +54,7 @@ __device__ __forceinline__ void parts_of_raw(const Raw8<T>& r, float scale, u32x
                       bf16_of_e4m3(hi, scale, true));
   } else {
     float v[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (T == kTypeF32) {
-        const uint32_t a = r.w[0][i], b = r.w[1][i];
-        v[i] = bits_f32(a), v[4 + i] = bits_f32(b);
-      } else {
-        const uint32_t both = r.w[0][i];
-        const f16x2 h = __builtin_bit_cast(f16x2, both);
-        v[2 * i] = (float)h[0], v[2 * i + 1] = (float)h[1];
-      }
-    }
+    values_of<T>(r, v);
 #pragma unroll
     for (int j = 0; j < parts_of(T); ++j) {
 #pragma unroll

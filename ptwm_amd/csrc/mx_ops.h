@@ -28,6 +28,7 @@ struct MxNormArgs {
   uint64_t rows;
   uint32_t cols;
   float eps;
+  uint32_t weight_type;
 };
 
 struct MxSwigluArgs {
@@ -46,7 +47,7 @@ struct MxLinearArgs {
 };
 
 // Each queues its work on `stream` of the current device and returns.
-hipError_t launch_rms_norm_mx(uint32_t type, uint32_t weight_type, const MxNormArgs& a, hipStream_t stream);
+hipError_t launch_rms_norm_mx(uint32_t type, const MxNormArgs& a, hipStream_t stream);
 hipError_t launch_swiglu_mx(uint32_t type, const MxSwigluArgs& a, hipStream_t stream);
 hipError_t launch_mxfp4_linear(uint32_t x_type, const MxLinearArgs& a, hipStream_t stream);
 
