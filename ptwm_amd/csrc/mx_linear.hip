@@ -287,49 +287,47 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
   };
   u32x4 wr[2 * RT];     // codes on their way through registers
   uint32_t sv, cv[XS];  // scales of a row and of tokens, a byte a block
-  auto load_weights = [&](const Step& p) {
-    GlobalBytes w = w0 + (uint64_t)p.at * 64, s = s0 + ((uint64_t)p.at * 4 + p.in - 4);
-    asm("" : "+s"(w), "+s"(s));  // kept uniform: otherwise the loop carries a 64-bit address for every load and lane
-#pragma unroll
-    for (int r = 0; r < 2 * RT; ++r) {
+  Raw8<T> raw[J];  // values on their way through registers
+  u32x4 xr[J];
+  // request k of the kRequests that bring a step: the words of scales, the codes, the tokens' pieces
+  constexpr int kScales = 1 + (T == kTypeE4m3 ? XS : 0), kRequests = kScales + 2 * RT + J;
+  auto request = [&](int k, const Step& p, u32x4* stage) {
+    if (k < kScales) {
+      GlobalBytes g = (k ? c0 : s0) + ((uint64_t)p.at * 4 + p.in - 4);
+      asm("" : "+s"(g));  // kept uniform: otherwise the loop carries a 64-bit address for every load and lane
+      if (k == 0) {
+        asm("" : "+v"(so));
+        sv = ld4(g, so);
+      } else {
+        asm("" : "+v"(co[k - 1]));
+        cv[k - 1] = ld4(g, co[k - 1]);
+      }
+    } else if (k < kScales + 2 * RT) {
+      const int r = k - kScales;
+      GlobalBytes w = w0 + (uint64_t)p.at * 64;
+      asm("" : "+s"(w));
       asm("" : "+v"(wo[r]));
       const uint32_t at = wo[r] + min(code_chunk, p.in - 1) * 16;
       if constexpr (ALIGNED)
         __builtin_amdgcn_global_load_lds(w + at, (__attribute__((address_space(3))) void*)(codes + r * 64), 16, 0, 0);
       else
         wr[r] = ld16(w, at);
-    }
-    asm("" : "+v"(so));
-    sv = ld4(s, so);
-  };
-  Raw8<T> raw[J];  // values on their way through registers
-  u32x4 xr[J];
-  auto load_tokens = [&](u32x4* stage, const Step& p) {
-    GlobalBytes x = x0 + (uint64_t)p.at * (128 * type_bytes(T));
-    GlobalBytes c = c0 + ((uint64_t)p.at * 4 + p.in - 4);
-    asm("" : "+s"(x), "+s"(c));
-    if constexpr (T == kTypeE4m3) {
-#pragma unroll
-      for (int k = 0; k < XS; ++k) {
-        asm("" : "+v"(co[k]));
-        cv[k] = ld4(c, co[k]);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      if (RAW && ALIGNED && RG == 1 && j && (uint32_t)j >= loads) break;
+    } else {
+      const int j = k - kScales - 2 * RT;
+      if (RAW && ALIGNED && RG == 1 && j && (uint32_t)j >= loads) return;  // no token of the batch
+      GlobalBytes x = x0 + (uint64_t)p.at * (128 * type_bytes(T));
+      asm("" : "+s"(x));
       asm("" : "+v"(xo[j]));
       const uint32_t b = piece_of(j) / kBlockPieces;
       const uint32_t over = b - min(b, p.in - 1);  // blocks to go back: at least as many lie before
       const uint32_t at = xo[j] - over * (kMxBlock * type_bytes(T));
-      if constexpr (RAW && ALIGNED) {
+      if constexpr (RAW && ALIGNED)
         __builtin_amdgcn_global_load_lds(
             x + at, (__attribute__((address_space(3))) void*)(stage + j * kLoaders + rg * 64), 16, 0, 0);
-      } else if constexpr (RAW) {
+      else if constexpr (RAW)
         xr[j] = ld16(x, at);
-      } else {
+      else
         raw[j] = load_raw8<T>(x, at);
-      }
     }
   };
   auto store = [&](u32x4* stage) {  // what came through registers
@@ -418,33 +416,42 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
     if constexpr (!last) {
       // the codes are in registers before new ones may arrive in their place
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      const Step q = step_of(round + 1);
-      load_weights(q);
-      load_tokens(next, q);
     }
-    bf16x8 w8[RT];
+    const Step q = step_of(round + 1);
+    bf16x8 w8[2][RT];
     float sf[RT], cf[CT];
+    auto widen = [&](int u) {  // the weights of product u
+      const int m = u / 4;
+      const bool in = !last || 2 * m + h < p.left;
+      const uint32_t shift = 8 * ((2 * m + h + (last ? 4 - p.in : 0)) & 3);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        if (u % 4 == 0) sf[r] = scale_f32(in ? sn[r] >> shift & 0xFF : 127);
+        w8[u & 1][r] = weights8(in ? wv[m][r][u & 3] : 0, sf[r]);
+      }
+    };
+    widen(0);
 #pragma unroll
     for (int v = 0; v < 8 * kParts; ++v) {
       const int u = v / kParts, m = u / 4, rd = v / kEach;
       // what is requested stays ahead of the products it hides behind
       if (v % kEach == 0 && rd + 1 < kReads) read(rd + 1);
-      if (v % kParts == 0) {
-        const bool in = !last || 2 * m + h < p.left;
-        const uint32_t byte = 2 * m + h + (last ? 4 - p.in : 0);
-        const uint32_t shift = 8 * (byte & 3);
+      if constexpr (!last) {
+        // Large tiles spread the next step's requests over the first half of the products: all at once they hold the
+        // wavefront up, and its products with it, until the address unit has taken them (512x14336x4096 bf16: 71 us,
+        // 62 this way).  Where the weights' way from memory is what takes time they go out at once.
+        constexpr int kOver = (RG > 1 ? 4 : 1) * kParts;
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          if (u % 4 == 0) sf[r] = scale_f32(in ? sn[r] >> shift & 0xFF : 127);
-          w8[r] = weights8(in ? wv[m][r][u & 3] : 0, sf[r]);
-        }
-        if constexpr (T == kTypeE4m3) {
-#pragma unroll
-          for (int c = 0; c < CT; ++c)
-            if (u % 4 == 0) cf[c] = scale_f32(in ? cn[c] >> shift & 0xFF : 127);
-        }
+        for (int k = v * kRequests / kOver; k < (v + 1) * kRequests / kOver && k < kRequests; ++k) request(k, q, next);
       }
       __builtin_amdgcn_sched_barrier(0);
+      if constexpr (T == kTypeE4m3) {
+        const bool in = !last || 2 * m + h < p.left;
+        const uint32_t shift = 8 * ((2 * m + h + (last ? 4 - p.in : 0)) & 3);
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+          if (u % 4 == 0) cf[c] = scale_f32(in ? cn[c] >> shift & 0xFF : 127);
+      }
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
         if constexpr (RAW) {
@@ -461,18 +468,26 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
 #pragma unroll
           for (int part = P - 1; part >= 0; --part)
 #pragma unroll
-            for (int r = 0; r < RT; ++r) acc[r][c] = mfma32(w8[r], b[part], acc[r][c]);
+            for (int r = 0; r < RT; ++r) acc[r][c] = mfma32(w8[u & 1][r], b[part], acc[r][c]);
         } else {
 #pragma unroll
-          for (int r = 0; r < RT; ++r) acc[r][c] = mfma32(w8[r], x8[rd & 1][c][0], acc[r][c]);
+          for (int r = 0; r < RT; ++r) acc[r][c] = mfma32(w8[u & 1][r], x8[rd & 1][c][0], acc[r][c]);
         }
+      }
+      // the next product's weights are widened while the matrix unit works: an instruction of it takes the time of
+      // about six others, and the wavefront is free in between
+      if (v % kParts == kParts - 1 && u < 7) widen(u + 1);
+#pragma unroll
+      for (int k = 0; k < CT * RT * (RAW ? P : 1); ++k) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
+        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // up to four others
       }
       __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr (!last) store(next);
   };
-  load_weights(step_of(0));
-  load_tokens(even, step_of(0));
+#pragma unroll
+  for (int k = 0; k < kRequests; ++k) request(k, step_of(0), even);
   store(even);
   uint32_t round = 0;
   for (; round + 2 < rounds; round += 2) {
@@ -542,10 +557,14 @@ hipError_t tiles_by_size(const MxLinearArgs& a, hipStream_t stream) {
   auto count = [&](uint64_t rows, uint64_t tokens) {
     return ((a.rows + rows - 1) / rows) * ((a.tokens + tokens - 1) / tokens);
   };
-  // Tiles of 256 rows where there are enough for the 256 CUs, otherwise smaller ones whose wavefronts share the length
-  // of the rows: measured (us, 256-row tiles against the one taken) 512x14336x4096 bf16 (224 tiles) 68 and 100,
-  // 256x14336x4096 bf16 (112) 63 and 50, e4m3 66 and 41, 100x4096x4096 e4m3 (16) 63 and 8.9.
+  // Tiles of 256 rows where there are enough for the 256 CUs, with half the tokens where there are not, then smaller
+  // ones whose wavefronts share the length of the rows: measured (us; 256 rows and 128 tokens, 64 tokens, shared)
+  // 512x14336x4096 bf16 (224 tiles of 128) 62, 68, 98; 256x14336x4096 bf16 (112 of 128, 224 of 64) 52, 36, 55;
+  // 1024x4096x4096 bf16 (128, 256) 50, 38, 54; 128x14336x4096 bf16 (56, 112) 49, 32, 30; 200x5000x5120 e4m3 (40, 80)
+  // 61, 41, 24.
   if (count(256, 32 * CT) >= 160) return tiles_of<T, 2, CT, 4, 1, kPlain>(a, stream);
+  if constexpr (kPlain)
+    if (count(256, 64) >= 160) return tiles_of<T, 2, 2, 4, 1, kPlain>(a, stream);
   // As many wavefronts to a tile as LDS holds where each tile has a CU of its own: 45x1354x960 bf16 (86 tiles of 32
   // rows) 4.0 and 4.8 with four, 100x4096x4096 e4m3 (256 of 64 rows) 8.9 and 9.3.
   if (count(32, 32) <= 128) return tiles_of<T, 1, 1, 1, KG, true>(a, stream);
