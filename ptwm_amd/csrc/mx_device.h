@@ -8,10 +8,12 @@ namespace ptwm {
 
 // One launch with one argument; the triple chevrons' way keeps a stack of configurations besides.
 template <typename A>
-hipError_t launch(void (*kernel)(A), uint64_t groups, uint32_t threads, const A& a, hipStream_t stream) {
+hipError_t launch(void (*kernel)(A), uint64_t groups, uint32_t threads, const A& a, hipStream_t stream,
+                  uint32_t shared = 0) {
   if (groups > 0x7FFFFFFFu) return hipErrorInvalidValue;
   void* args[] = {const_cast<A*>(&a)};
-  return hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3((uint32_t)groups), dim3(threads), args, 0, stream);
+  return hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3((uint32_t)groups), dim3(threads), args, shared,
+                         stream);
 }
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));

@@ -27,6 +27,7 @@
 namespace ptwm {
 namespace {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
@@ -178,10 +179,10 @@ __global__ __launch_bounds__(256) void mxfp4_linear_kernel(MxLinearArgs a) {
   }
 }
 
-// A tile of 32 * RT * RG weight rows and 32 * CT tokens by one workgroup of
-// RG * KG wavefronts: RG groups of 32 * RT rows each, and KG groups that take
+// A tile of ROWS * RG weight rows and 32 * CT tokens by one workgroup of
+// RG * KG wavefronts: RG groups of ROWS rows each, and KG groups that take
 // turns in steps of 128 values (four blocks) along the rows and add up in LDS
-// at the end.
+// at the end.  ROWS is 64, 32, or 16 (half of the matrix instruction is idle).
 //
 // The tokens' share of a step goes through LDS; the RG wavefronts of a K group
 // load it together and each reads all of it (with RG = 1 a wavefront waits for
@@ -213,12 +214,13 @@ __device__ __forceinline__ uint32_t place(uint32_t t, uint32_t c) {
   return t * S + (c ^ (t / per & (S < 16 ? S - 1 : 15)));
 }
 
-template <uint32_t T, int RT, int CT, int RG, int KG, bool RAW, bool ALIGNED>
-__global__ __launch_bounds__(64 * RG * KG, RG * KG <= 4 ? 1 + (RT * CT * RG > 16) : RG * KG / 4)
+template <uint32_t T, int ROWS, int CT, int RG, int KG, bool RAW, bool ALIGNED>
+__global__ __launch_bounds__(64 * RG * KG, RG * KG <= 4 ? 1 + (ROWS * CT * RG > 512) : RG * KG / 4)
 void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
   static_assert(RAW || parts_of(T) > 1, "what needs no split goes as it is");
-  constexpr int P = parts_of(T);
-  constexpr uint32_t kTokens = 32 * CT, kRows = 32 * RT * RG, kLoaders = 64 * RG;
+  constexpr int P = parts_of(T), RT = ROWS < 32 ? 1 : ROWS / 32, R16 = ROWS / 16;
+  constexpr uint32_t kRowMask = ROWS < 32 ? ROWS - 1 : 31;
+  constexpr uint32_t kTokens = 32 * CT, kRows = ROWS * RG, kLoaders = 64 * RG;
   constexpr uint32_t S = RAW ? 8 * type_bytes(T) : 16;       // 16-byte chunks of a row (and part) in LDS
   constexpr uint32_t kStage = (RAW ? 1 : P) * kTokens * S;   // chunks of a stage
   // a thread's pieces of the tokens' share: a chunk as it is, or eight values to split
@@ -227,7 +229,7 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
   constexpr uint32_t kBlockPieces = kMxBlock * type_bytes(T) / kPiece;
   constexpr int J = kTokens * kPer / kLoaders;
   constexpr uint32_t kTokenStep = kLoaders / kPer;
-  constexpr uint32_t kCodes = 32 * RT * 4;  // chunks of a wavefront's weight codes
+  constexpr uint32_t kCodes = ROWS * 4;  // chunks of a wavefront's weight codes
   constexpr int XS = CT < 2 ? 1 : CT / 2;   // words of token scales of a lane
   // variables of their own, so that a read of one does not wait for what is on its way to another
   __shared__ u32x4 even_all[KG * kStage], odd_all[KG * kStage], codes_all[RG * KG * kCodes];
@@ -238,7 +240,7 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
   u32x4* const odd = odd_all + group * kStage;
   u32x4* const codes = codes_all + wave * kCodes;
   const uint32_t row_tiles = (a.rows + kRows - 1) / kRows;
-  const uint32_t n0 = blockIdx.x % row_tiles * kRows + rg * 32 * RT;
+  const uint32_t n0 = blockIdx.x % row_tiles * kRows + rg * ROWS;
   const uint64_t t0 = (uint64_t)(blockIdx.x / row_tiles) * kTokens;
   const uint32_t tokens = (uint32_t)min(a.tokens - t0, (uint64_t)kTokens);
   const uint32_t blocks = a.cols / kMxBlock, steps = (blocks + 3) / 4, rounds = (steps + KG - 1) / KG;
@@ -248,12 +250,12 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
   const GlobalBytes s0 = global_bytes(a.scales.ptr + nb * a.scales.stride);
   const GlobalBytes x0 = global_bytes(a.x.ptr + t0 * a.x.stride * type_bytes(T));
   const GlobalBytes c0 = global_bytes(a.x_scales.ptr + t0 * a.x_scales.stride);
-  uint32_t wo[2 * RT], xo[J], co[XS];
+  uint32_t wo[R16], xo[J], co[XS];
   const uint32_t code_chunk = (lane & 3) ^ (lane >> 4);
 #pragma unroll
-  for (int r = 0; r < 2 * RT; ++r)
+  for (int r = 0; r < R16; ++r)
     wo[r] = min(r * 16 + lane / 4, a.rows - 1 - nb) * (uint32_t)a.weight.stride;
-  uint32_t so = min(RT == 2 ? lane : i, a.rows - 1 - nb) * (uint32_t)a.scales.stride;
+  uint32_t so = min(RT == 2 ? lane : i & kRowMask, a.rows - 1 - nb) * (uint32_t)a.scales.stride;
 #pragma unroll
   for (int c = 0; c < XS; ++c)
     if constexpr (T == kTypeE4m3)
@@ -285,12 +287,12 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
     p.left = want < steps ? p.in : 0;
     return p;
   };
-  u32x4 wr[2 * RT];     // codes on their way through registers
+  u32x4 wr[R16];        // codes on their way through registers
   uint32_t sv, cv[XS];  // scales of a row and of tokens, a byte a block
   Raw8<T> raw[J];  // values on their way through registers
   u32x4 xr[J];
   // request k of the kRequests that bring a step: the words of scales, the codes, the tokens' pieces
-  constexpr int kScales = 1 + (T == kTypeE4m3 ? XS : 0), kRequests = kScales + 2 * RT + J;
+  constexpr int kScales = 1 + (T == kTypeE4m3 ? XS : 0), kRequests = kScales + R16 + J;
   auto request = [&](int k, const Step& p, u32x4* stage) {
     if (k < kScales) {
       GlobalBytes g = (k ? c0 : s0) + ((uint64_t)p.at * 4 + p.in - 4);
@@ -302,7 +304,7 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
         asm("" : "+v"(co[k - 1]));
         cv[k - 1] = ld4(g, co[k - 1]);
       }
-    } else if (k < kScales + 2 * RT) {
+    } else if (k < kScales + R16) {
       const int r = k - kScales;
       GlobalBytes w = w0 + (uint64_t)p.at * 64;
       asm("" : "+s"(w));
@@ -313,7 +315,7 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
       else
         wr[r] = ld16(w, at);
     } else {
-      const int j = k - kScales - 2 * RT;
+      const int j = k - kScales - R16;
       if (RAW && ALIGNED && RG == 1 && j && (uint32_t)j >= loads) return;  // no token of the batch
       GlobalBytes x = x0 + (uint64_t)p.at * (128 * type_bytes(T));
       asm("" : "+s"(x));
@@ -333,7 +335,7 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
   auto store = [&](u32x4* stage) {  // what came through registers
     if constexpr (!ALIGNED) {
 #pragma unroll
-      for (int r = 0; r < 2 * RT; ++r) codes[r * 64 + lane] = wr[r];
+      for (int r = 0; r < R16; ++r) codes[r * 64 + lane] = wr[r];
     }
     if constexpr (RAW && !ALIGNED) {
 #pragma unroll
@@ -378,7 +380,7 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int r = 0; r < RT; ++r) wv[m][r] = codes[(r * 32 + i) * 4 + ((2 * m + h) ^ (i >> 2 & 3))];
+      for (int r = 0; r < RT; ++r) wv[m][r] = codes[(r * 32 + (i & kRowMask)) * 4 + ((2 * m + h) ^ (i >> 2 & 3))];
     // the word of row or token 32 k + l % 32 in lane l, from the lanes that loaded it
     uint32_t sn[RT], cn[CT];
     if constexpr (RT == 2) {
@@ -502,14 +504,14 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
   multiply(round, stage, stage, std::true_type{});
 
   // lane l holds token l % 32 and rows 8 j + 4 (l / 32) .. + 3, j = 0 .. 3
-  constexpr int kQuads = RT * CT * 4;
+  constexpr int kSub = ROWS < 32 ? ROWS / 8 : 4, kQuads = RT * CT * kSub;
   auto write = [&](int quad, f32x4 v) {
-    const int r = quad / (CT * 4), c = quad / 4 % CT, j = quad % 4;
+    const int r = quad / (CT * kSub), c = quad / kSub % CT, j = quad % kSub;
     const uint64_t t = t0 + c * 32 + i;
     if (t < a.tokens) store4(a, t, n0 + r * 32 + j * 8 + h * 4, v);
   };
   auto quad_of = [&](int quad) {
-    const int r = quad / (CT * 4), c = quad / 4 % CT, j = quad % 4;
+    const int r = quad / (CT * kSub), c = quad / kSub % CT, j = quad % kSub;
     return f32x4{acc[r][c][4 * j], acc[r][c][4 * j + 1], acc[r][c][4 * j + 2], acc[r][c][4 * j + 3]};
   };
   if constexpr (KG == 1) {
@@ -534,20 +536,174 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
   }
 }
 
+// One or a few tokens (NT): 16 weight rows by one workgroup of W wavefronts,
+// without the matrix instruction, whose other columns would be idle.  The
+// tokens lie in LDS in 32 bits, zeros past their ends.  A wavefront takes every
+// W-th step of 128 values; a lane holds block l % 4 of it in row l / 4, so that
+// codes and scales come from memory in the order in which they lie, straight
+// to registers, kDepth steps ahead.  A lane's 32 products are summed by fused
+// multiply-adds in 32 bits, in eight sums, the four lanes of a row and the
+// wavefronts at the end.
+//
+// The weights are read once.  16 widening instructions and 32 * NT
+// multiply-adds for 1 KiB of codes (a wavefront's 64 lanes) let a CU take 15
+// bytes a cycle with one token, more than its share of what memory gives; what
+// is left above that time is the way of the first and the last bytes.
+constexpr int kFewWaves = 8;
+
+template <uint32_t T, int NT>
+__global__ __launch_bounds__(64 * kFewWaves) void mxfp4_linear_few_kernel(MxLinearArgs a) {
+  constexpr int kDepth = 4, W = kFewWaves;
+  extern __shared__ f32x4 few_x[];  // NT rows of whole steps
+  __shared__ float part[W][NT][16];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane & 3;
+  const uint32_t n0 = blockIdx.x * 16;
+  const uint32_t blocks = a.cols / kMxBlock, steps = (blocks + 3) / 4;
+  const GlobalBytes w0 = global_bytes(a.weight.ptr + n0 * a.weight.stride);
+  const GlobalBytes s0 = global_bytes(a.scales.ptr + n0 * a.scales.stride);
+  const uint32_t row = min(lane / 4, a.rows - 1 - n0);
+  const uint32_t wo = row * (uint32_t)a.weight.stride, so = row * (uint32_t)a.scales.stride;
+  u32x4 wv[kDepth];
+  uint32_t sv[kDepth];
+  auto request = [&](int d, uint32_t step) {
+    const uint32_t b = min(step * 4 + q, blocks - 1);  // past the end the last block again, against zeros
+    wv[d] = ld16(w0, wo + b * 16);
+    sv[d] = s0[so + b];
+  };
+  // the tokens' first values are asked for before the weights, behind which they would wait
+  Raw8<T> raw[NT];
+  uint32_t byte[NT];
+  auto ask = [&](uint32_t k) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const uint64_t at = min((uint64_t)t, a.tokens - 1);
+      const uint32_t c = min(k, a.cols - 8);
+      raw[t] = load_raw8<T>(a.x.ptr + (at * a.x.stride + c) * type_bytes(T));
+      if constexpr (T == kTypeE4m3) byte[t] = g_ld<uint8_t>(a.x_scales.ptr + at * a.x_scales.stride + c / kMxBlock);
+    }
+  };
+  auto take = [&](uint32_t k) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float v[8];
+      if constexpr (T == kTypeE4m3) {
+        u32x4 p[1];
+        parts_of_raw<T>(raw[t], scale_f32(byte[t]), p);
+        values_of<kTypeBf16>(Raw8<kTypeBf16>{{p[0]}}, v);
+      } else {
+        values_of<T>(raw[t], v);
+      }
+      const bool in = k < a.cols;
+      f32x4* const to = few_x + t * steps * 32 + k / 4;
+      to[0] = in ? f32x4{v[0], v[1], v[2], v[3]} : f32x4{};
+      to[1] = in ? f32x4{v[4], v[5], v[6], v[7]} : f32x4{};
+    }
+  };
+  uint32_t k = threadIdx.x * 8;
+  ask(k);
+#pragma unroll
+  for (int d = 0; d < kDepth; ++d) request(d, wave + d * W);
+  while (k < steps * 128) {
+    take(k);
+    k += 64 * W * 8;
+    if (k < steps * 128) ask(k);
+  }
+  __syncthreads();
+  f32x4 acc[NT][2] = {};
+  for (uint32_t step = wave; step < steps; step += kDepth * W) {
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+      const uint32_t now = step + d * W;
+      if (now >= steps) break;
+      const bool in = now * 4 + q < blocks;
+      const u32x4 wn = wv[d];
+      const float sf = scale_f32(in ? sv[d] : 127);
+      request(d, now + kDepth * W);
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {  // eight values
+        f32x4 x[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            x[t][e] = few_x[t * steps * 32 + now * 32 + q * 8 + f * 2 + e];
+        const uint32_t c = wn[f];
+        const f32x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, sf, 0);
+        const f32x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, sf, 1);
+        const f32x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, sf, 2);
+        const f32x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, sf, 3);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            acc[t][e][0] = __builtin_fmaf(e ? p2[0] : p0[0], x[t][e][0], acc[t][e][0]);
+            acc[t][e][1] = __builtin_fmaf(e ? p2[1] : p0[1], x[t][e][1], acc[t][e][1]);
+            acc[t][e][2] = __builtin_fmaf(e ? p3[0] : p1[0], x[t][e][2], acc[t][e][2]);
+            acc[t][e][3] = __builtin_fmaf(e ? p3[1] : p1[1], x[t][e][3], acc[t][e][3]);
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const f32x4 s4 = acc[t][0] + acc[t][1];
+    float v = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+    v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true));
+    v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true));
+    if (q == 0) part[wave][t][lane / 4] = v;
+  }
+  __syncthreads();
+  if (threadIdx.x < 4 * NT) {
+    const uint32_t t = threadIdx.x / 4, n = threadIdx.x % 4 * 4;
+    f32x4 v = {};
+#pragma unroll
+    for (int g = 0; g < W; ++g)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += part[g][t][n + j];
+    if (t < a.tokens) store4(a, t, n0 + n, v);
+  }
+}
+
 // Whether a tile's rows and tokens lie within 32-bit offsets and a row's scales fill a word.
 bool tiles_fit(const MxLinearArgs& a) {
   return a.cols >= 128 && a.weight.stride < (1u << 23) && a.x.stride < (1u << 23) && a.scales.stride < (1u << 23) && a.x_scales.stride < (1u << 23);
 }
 
-template <uint32_t T, int RT, int CT, int RG, int KG, bool RAW>
+template <uint32_t T, int ROWS, int CT, int RG, int KG, bool RAW>
 hipError_t tiles_of(const MxLinearArgs& a, hipStream_t stream) {
-  constexpr uint32_t kRows = 32 * RT * RG, kTokens = 32 * CT;
+  constexpr uint32_t kRows = ROWS * RG, kTokens = 32 * CT;
   const uint64_t tiles = (uint64_t)((a.rows + kRows - 1) / kRows) * ((a.tokens + kTokens - 1) / kTokens);
   const bool aligned = a.weight.ptr % 16 == 0 && a.weight.stride % 16 == 0 &&
                        (!RAW || (a.x.ptr % 16 == 0 && a.x.stride * type_bytes(T) % 16 == 0));
-  return launch(aligned ? mxfp4_linear_tiles_kernel<T, RT, CT, RG, KG, RAW, true>
-                        : mxfp4_linear_tiles_kernel<T, RT, CT, RG, KG, RAW, false>,
+  return launch(aligned ? mxfp4_linear_tiles_kernel<T, ROWS, CT, RG, KG, RAW, true>
+                        : mxfp4_linear_tiles_kernel<T, ROWS, CT, RG, KG, RAW, false>,
                 tiles, 64 * RG * KG, a, stream);
+}
+
+// LDS that the few tokens' kernel takes: NT tokens in 32 bits, whole steps.
+constexpr uint64_t few_bytes(uint64_t cols, uint64_t nt) { return (cols + 127) / 128 * 128 * nt * 4; }
+
+template <uint32_t T, int NT>
+hipError_t few_of(const MxLinearArgs& a, hipStream_t stream) {
+  return launch(mxfp4_linear_few_kernel<T, NT>, (a.rows + 15) / 16, 64 * kFewWaves, a, stream,
+                (uint32_t)few_bytes(a.cols, NT));
+}
+
+// Whether the few tokens' kernel takes the call, and with what outcome.  Its LDS is kept to 60 KiB.  One token of f16
+// or f32: measured (us, this kernel and the tiles) 1x14336x4096 f32 9.6 and 29, f16 9.4 and 17, 1x4096x4096 f32 3.8 and
+// 15.  One of bf16 or e4m3 where there are few rows: 1x4096x14336 e4m3 9.0 and 11.2, 1x1024x4096 bf16 3.7 and 5.1,
+// 1x8192x8192 10.7 and 10.5, 1x14336x4096 9.5 and 8.0.  Two of f16 or f32, up to four of f32, whose splitting costs the
+// tiles most: 2x1024x4096 f32 4.8 and 15, 4x1024x3584 f32 6.5 and 13, bf16 6.5 and 5.5.
+template <uint32_t T>
+bool few_taken(const MxLinearArgs& a, hipStream_t stream, hipError_t& e) {
+  constexpr int P = parts_of(T);
+  const auto fits = [&](uint64_t nt) { return a.tokens <= nt && few_bytes(a.cols, nt) <= 60 * 1024; };
+  if (fits(1) && (P > 1 || a.rows <= 6144)) return e = few_of<T, 1>(a, stream), true;
+  if constexpr (P > 1)
+    if (fits(2)) return e = few_of<T, 2>(a, stream), true;
+  if constexpr (P > 2)
+    if (fits(4)) return e = few_of<T, 4>(a, stream), true;
+  return false;
 }
 
 template <uint32_t T>
@@ -562,26 +718,27 @@ hipError_t tiles_by_size(const MxLinearArgs& a, hipStream_t stream) {
   // 512x14336x4096 bf16 (224 tiles of 128) 62, 68, 98; 256x14336x4096 bf16 (112 of 128, 224 of 64) 52, 36, 55;
   // 1024x4096x4096 bf16 (128, 256) 50, 38, 54; 128x14336x4096 bf16 (56, 112) 49, 32, 30; 200x5000x5120 e4m3 (40, 80)
   // 61, 41, 24.
-  if (count(256, 32 * CT) >= 160) return tiles_of<T, 2, CT, 4, 1, kPlain>(a, stream);
+  if (count(256, 32 * CT) >= 160) return tiles_of<T, 64, CT, 4, 1, kPlain>(a, stream);
   if constexpr (kPlain)
-    if (count(256, 64) >= 160) return tiles_of<T, 2, 2, 4, 1, kPlain>(a, stream);
+    if (count(256, 64) >= 160) return tiles_of<T, 64, 2, 4, 1, kPlain>(a, stream);
   // As many wavefronts to a tile as LDS holds where each tile has a CU of its own: 45x1354x960 bf16 (86 tiles of 32
   // rows) 4.0 and 4.8 with four, 100x4096x4096 e4m3 (256 of 64 rows) 8.9 and 9.3.
-  if (count(32, 32) <= 128) return tiles_of<T, 1, 1, 1, KG, true>(a, stream);
+  if (count(32, 32) <= 128) return tiles_of<T, 32, 1, 1, KG, true>(a, stream);
   // Few tokens read each weight once, and more, smaller tiles keep more of them in flight: 1x14336x4096 bf16 7.7 and
   // 8.2 with 64 rows.
-  if (a.tokens <= 16 && count(32, 32) <= 512) return tiles_of<T, 1, 1, 1, 4, true>(a, stream);
-  if (count(64, 32) <= 256) return tiles_of<T, 2, 1, 1, KG, true>(a, stream);
+  if (a.tokens <= 16 && count(32, 32) <= 512) return tiles_of<T, 32, 1, 1, 4, true>(a, stream);
+  if (count(64, 32) <= 256) return tiles_of<T, 64, 1, 1, KG, true>(a, stream);
   // Two workgroups share a CU's LDS with 64 tokens of e4m3, with 32 of the others: 700x3000x2048 bf16 21 and 26 with
   // 64 tokens, 256x14336x4096 e4m3 41 and 48 with 32.
   if constexpr (T == kTypeE4m3)
-    if (a.tokens > 32) return tiles_of<T, 2, 2, 1, 4, true>(a, stream);
-  return tiles_of<T, 2, 1, 1, 4, true>(a, stream);
+    if (a.tokens > 32) return tiles_of<T, 64, 2, 1, 4, true>(a, stream);
+  return tiles_of<T, 64, 1, 1, 4, true>(a, stream);
 }
 
 template <uint32_t T>
 hipError_t linear_of(const MxLinearArgs& a, hipStream_t stream) {
-  if (tiles_fit(a)) return tiles_by_size<T>(a, stream);
+  hipError_t e = hipSuccess;
+  if (tiles_fit(a)) return few_taken<T>(a, stream, e) ? e : tiles_by_size<T>(a, stream);
   const uint64_t tiles = (uint64_t)((a.rows + 15) / 16) * ((a.tokens + 15) / 16);
   return launch(mxfp4_linear_kernel<T>, tiles, 256, a, stream);
 }
