@@ -182,7 +182,7 @@ __global__ __launch_bounds__(256) void mxfp4_linear_kernel(MxLinearArgs a) {
 // A tile of ROWS * RG weight rows and 32 * CT tokens by one workgroup of
 // RG * KG wavefronts: RG groups of ROWS rows each, and KG groups that take
 // turns in steps of 128 values (four blocks) along the rows and add up in LDS
-// at the end.  ROWS is 64, 32, or 16 (half of the matrix instruction is idle).
+// at the end.  ROWS is 64 or 32.
 //
 // The tokens' share of a step goes through LDS; the RG wavefronts of a K group
 // load it together and each reads all of it (with RG = 1 a wavefront waits for
@@ -218,8 +218,7 @@ template <uint32_t T, int ROWS, int CT, int RG, int KG, bool RAW, bool ALIGNED>
 __global__ __launch_bounds__(64 * RG * KG, RG * KG <= 4 ? 1 + (ROWS * CT * RG > 512) : RG * KG / 4)
 void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
   static_assert(RAW || parts_of(T) > 1, "what needs no split goes as it is");
-  constexpr int P = parts_of(T), RT = ROWS < 32 ? 1 : ROWS / 32, R16 = ROWS / 16;
-  constexpr uint32_t kRowMask = ROWS < 32 ? ROWS - 1 : 31;
+  constexpr int P = parts_of(T), RT = ROWS / 32, R16 = ROWS / 16;
   constexpr uint32_t kTokens = 32 * CT, kRows = ROWS * RG, kLoaders = 64 * RG;
   constexpr uint32_t S = RAW ? 8 * type_bytes(T) : 16;       // 16-byte chunks of a row (and part) in LDS
   constexpr uint32_t kStage = (RAW ? 1 : P) * kTokens * S;   // chunks of a stage
@@ -255,7 +254,7 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
 #pragma unroll
   for (int r = 0; r < R16; ++r)
     wo[r] = min(r * 16 + lane / 4, a.rows - 1 - nb) * (uint32_t)a.weight.stride;
-  uint32_t so = min(RT == 2 ? lane : i & kRowMask, a.rows - 1 - nb) * (uint32_t)a.scales.stride;
+  uint32_t so = min(RT == 2 ? lane : i, a.rows - 1 - nb) * (uint32_t)a.scales.stride;
 #pragma unroll
   for (int c = 0; c < XS; ++c)
     if constexpr (T == kTypeE4m3)
@@ -380,7 +379,7 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int r = 0; r < RT; ++r) wv[m][r] = codes[(r * 32 + (i & kRowMask)) * 4 + ((2 * m + h) ^ (i >> 2 & 3))];
+      for (int r = 0; r < RT; ++r) wv[m][r] = codes[(r * 32 + i) * 4 + ((2 * m + h) ^ (i >> 2 & 3))];
     // the word of row or token 32 k + l % 32 in lane l, from the lanes that loaded it
     uint32_t sn[RT], cn[CT];
     if constexpr (RT == 2) {
@@ -504,14 +503,14 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
   multiply(round, stage, stage, std::true_type{});
 
   // lane l holds token l % 32 and rows 8 j + 4 (l / 32) .. + 3, j = 0 .. 3
-  constexpr int kSub = ROWS < 32 ? ROWS / 8 : 4, kQuads = RT * CT * kSub;
+  constexpr int kQuads = RT * CT * 4;
   auto write = [&](int quad, f32x4 v) {
-    const int r = quad / (CT * kSub), c = quad / kSub % CT, j = quad % kSub;
+    const int r = quad / (CT * 4), c = quad / 4 % CT, j = quad % 4;
     const uint64_t t = t0 + c * 32 + i;
     if (t < a.tokens) store4(a, t, n0 + r * 32 + j * 8 + h * 4, v);
   };
   auto quad_of = [&](int quad) {
-    const int r = quad / (CT * kSub), c = quad / kSub % CT, j = quad % kSub;
+    const int r = quad / (CT * 4), c = quad / 4 % CT, j = quad % 4;
     return f32x4{acc[r][c][4 * j], acc[r][c][4 * j + 1], acc[r][c][4 * j + 2], acc[r][c][4 * j + 3]};
   };
   if constexpr (KG == 1) {

@@ -70,6 +70,19 @@ def test_linear_sizes(tokens, rows, cols, kind):
     P.check_linear(o, x, xs, codes, scales, b)
 
 
+# Where the sizes choose another kernel: rows about the limit for one token, LDS about its limit for one, two and four
+# tokens, and enough tiles for the large and the middle ones, with row ends inside a step.
+@pytest.mark.parametrize("kind", TYPES + [F8], ids=str)
+@pytest.mark.parametrize("tokens,rows,cols", [(1, 6144, 160), (1, 6145, 160), (1, 17, 15360), (1, 17, 15392),
+                                              (2, 33, 7680), (2, 33, 7712), (4, 100, 3840), (3, 100, 3872),
+                                              (5, 40, 2016), (1300, 4100, 192), (1100, 5001, 96), (700, 4500, 160),
+                                              (1290, 4110, 416), (640, 4099, 352), (90, 8200, 1184)])
+def test_linear_choices(tokens, rows, cols, kind):
+    x, xs, codes, scales, b, o = linear_case(tokens, rows, cols, kind, torch.float32, True, gen(tokens, rows, cols, 3))
+    api.mxfp4_linear_cuda(x, codes, scales, o, 0, x_scales=xs, bias=b)
+    P.check_linear(o, x, xs, codes, scales, b)
+
+
 @pytest.mark.parametrize("out", TYPES, ids=str)
 @pytest.mark.parametrize("kind", TYPES + [F8], ids=str)
 @pytest.mark.parametrize("tokens", [1, 5, 48, 160])
