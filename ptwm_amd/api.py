@@ -501,153 +501,23 @@ def container_write(tensors, layout: str = "compact", payloads=None, as_array: b
 # Operators on microscaled (MX) blocks: what a program does with the MXFP4
 # tensors that a decode restored (library additions).  Unlike the codec calls
 # they queue their work on torch's current stream and return without waiting
-# for it, as torch's own operators do.  A call of the smallest sizes costs the
-# host more than the GPU, so the checks take the short way where all is well.
-
-class _Mx:
-    """What the operators look up, filled by the first call."""
-
-    codes = scales = weight = e4m3 = ()   # torch dtypes of codes, scales, weights and 8-bit activations
-    real: dict = {}                # torch dtype -> public dtype code (dtype.rs:79-103)
-    norm = swiglu = linear = stream = None   # entry points, and torch's current stream of a device
-
-    @classmethod
-    def load(cls) -> None:
-        import torch
-        L = lib()
-        cls.norm, cls.swiglu = L.ptwm_mi355x_rms_norm_mx_cuda, L.ptwm_mi355x_swiglu_mx_cuda
-        cls.linear = L.ptwm_mi355x_mxfp4_linear_cuda
-        cls.scales, cls.codes = (torch.float8_e8m0fnu, torch.uint8), (torch.float8_e4m3fn, torch.uint8)
-        cls.weight = (torch.uint8, torch.float4_e2m1fn_x2)
-        cls.real = {torch.bfloat16: 6, torch.float16: 4, torch.float32: 1}
-        cls.e4m3 = (torch.float8_e4m3fn,)
-        cls.stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or _current_raw_stream
+# for it, as torch's own operators do.  Their checks are native
+# (csrc/mx_python.cpp), because the smallest calls cost the host more than the
+# GPU; the module, which needs torch, is loaded at their first use.
+_MX = ("rms_norm_mx_cuda", "swiglu_mx_cuda", "mxfp4_linear_cuda")
 
 
-def _mx_refuse(t, name: str, shape: tuple, device_ordinal: int, dtypes):
-    """Raises for an operand that _mx_matrix or _mx_vector did not take."""
-    if not hasattr(t, "data_ptr") or not hasattr(t, "get_device"):
-        raise TypeError(f"{name}: expected a device tensor")
-    if t.dtype not in dtypes:
-        raise TypeError(f"{name}: dtype {t.dtype} is not one of {', '.join(str(d) for d in dtypes)}")
-    if not t.is_cuda:
-        raise ValueError(f"{name}: tensor is not on a GPU device")
-    if t.get_device() != device_ordinal:
-        raise ValueError(f"{name}: tensor is on device {t.get_device()}, call names device {device_ordinal}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name}: shape {tuple(t.shape)} is not {shape}")
-    raise ValueError(f"{name}: rows must be contiguous and must not overlap")
+def __getattr__(name: str):
+    if name not in _MX:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    import torch  # noqa: F401  (its libraries are the module's)
 
-
-def _mx_matrix(t, name: str, rows: int, cols: int, device_ordinal: int, dtypes) -> tuple[int, int]:
-    """(address, row stride) of a device matrix of the given size and one of
-    the given dtypes, whose rows are contiguous and do not overlap."""
+    lib()
     try:
-        if t.get_device() == device_ordinal and t.dtype in dtypes and t.shape == (rows, cols):
-            stride, inner = t.stride()
-            if (inner == 1 or cols <= 1) and (stride >= cols or rows <= 1):
-                return t.data_ptr(), stride
-    except AttributeError:
-        pass
-    _mx_refuse(t, name, (rows, cols), device_ordinal, dtypes)
-
-
-def _mx_vector(t, name: str, n: int, device_ordinal: int, dtypes) -> int:
-    """Address of a contiguous device vector of n elements."""
-    try:
-        if t.get_device() == device_ordinal and t.dtype in dtypes and t.shape == (n,) and t.is_contiguous():
-            return t.data_ptr()
-    except AttributeError:
-        pass
-    _mx_refuse(t, name, (n,), device_ordinal, dtypes)
-
-
-def _mx_size(t, name: str) -> tuple[int, int]:
-    """Rows and columns of an operator's first input: whole blocks of 32."""
-    if _Mx.linear is None:
-        _Mx.load()
-    shape = getattr(t, "shape", None)
-    if shape is None:
-        raise TypeError(f"{name}: expected a device tensor")
-    if len(shape) != 2:
-        raise ValueError(f"{name}: expected a matrix, a row a token")
-    if shape[1] == 0 or shape[1] % 32:
-        raise ValueError(f"{name}: {shape[1]} columns are not whole blocks of 32")
-    return shape
-
-
-def rms_norm_mx_cuda(x, weight, out, out_scales, device_ordinal: int = 0, residual=None, sum_out=None,
-                     eps: float = 1e-6) -> None:
-    """Root-mean-square norm with an output in 8 bits (library addition):
-    ``s = x + residual``, ``y = s * rsqrt(mean(s**2) + eps) * weight`` for
-    every row, in 32 bits.  ``out`` [rows, cols] (float8_e4m3fn or uint8)
-    receives y's codes and ``out_scales`` [rows, cols / 32] (float8_e8m0fnu
-    or uint8) a power of two for each block of 32: the smallest with which
-    the block's largest magnitude is at most 448.  ``sum_out`` receives ``s``
-    in x's dtype and may be ``x`` or ``residual`` itself.  x: float32,
-    float16 or bfloat16, rows at any stride; weight: any of the three."""
-    rows, cols = _mx_size(x, "x")
-    xp, xs = _mx_matrix(x, "x", rows, cols, device_ordinal, _Mx.real)
-    wp = _mx_vector(weight, "weight", cols, device_ordinal, _Mx.real)
-    rp = rs = sp = ss = 0
-    if residual is not None:
-        rp, rs = _mx_matrix(residual, "residual", rows, cols, device_ordinal, (x.dtype,))
-    if sum_out is not None:
-        sp, ss = _mx_matrix(sum_out, "sum_out", rows, cols, device_ordinal, (x.dtype,))
-    op, os_ = _mx_matrix(out, "out", rows, cols, device_ordinal, _Mx.codes)
-    cp, cs = _mx_matrix(out_scales, "out_scales", rows, cols // 32, device_ordinal, _Mx.scales)
-    if rows:
-        rc = _Mx.norm(_Mx.real[x.dtype], xp, xs, rp, rs, _Mx.real[weight.dtype], wp, eps, sp, ss, op, os_, cp, cs,
-                      rows, cols, _Mx.stream(device_ordinal), device_ordinal)
-        if rc:
-            check(rc, "rms_norm_mx_cuda")
-
-
-def swiglu_mx_cuda(gate, up, out, out_scales, device_ordinal: int = 0) -> None:
-    """Gated activation with an output in 8 bits (library addition):
-    ``y = gate / (1 + exp(-gate)) * up`` in 32 bits, to ``out`` and
-    ``out_scales`` as :func:`rms_norm_mx_cuda` writes them.  gate and up:
-    float32, float16 or bfloat16, rows at any stride (the halves of one
-    matrix, say)."""
-    rows, cols = _mx_size(gate, "gate")
-    gp, gs = _mx_matrix(gate, "gate", rows, cols, device_ordinal, _Mx.real)
-    up_, us = _mx_matrix(up, "up", rows, cols, device_ordinal, (gate.dtype,))
-    op, os_ = _mx_matrix(out, "out", rows, cols, device_ordinal, _Mx.codes)
-    cp, cs = _mx_matrix(out_scales, "out_scales", rows, cols // 32, device_ordinal, _Mx.scales)
-    if rows:
-        rc = _Mx.swiglu(_Mx.real[gate.dtype], gp, gs, up_, us, op, os_, cp, cs, rows, cols,
-                        _Mx.stream(device_ordinal), device_ordinal)
-        if rc:
-            check(rc, "swiglu_mx_cuda")
-
-
-def mxfp4_linear_cuda(x, weight, scales, out, device_ordinal: int = 0, x_scales=None, bias=None) -> None:
-    """``out = x @ W.T (+ bias)`` with MXFP4 weights (library addition):
-    ``weight`` [rows, cols / 2] holds e2m1 codes, the first of two in the low
-    nibble, and ``scales`` [rows, cols / 32] their E8M0 bytes, as a decode
-    restores them.  x [tokens, cols] is float32, float16, bfloat16, or
-    float8_e4m3fn with ``x_scales`` [tokens, cols / 32]; out [tokens, rows]
-    is float32, float16 or bfloat16, bias [rows] of out's dtype.  Sums are
-    held in 32 bits.  Rows may lie at any stride, but are contiguous."""
-    tokens, cols = _mx_size(x, "x")
-    cp = cs = bp = 0
-    if (x.dtype in _Mx.e4m3) != (x_scales is not None):
-        raise ValueError("x_scales: wanted with float8_e4m3fn activations, and only there")
-    if x_scales is not None:
-        xp, xs = _mx_matrix(x, "x", tokens, cols, device_ordinal, _Mx.e4m3)
-        cp, cs = _mx_matrix(x_scales, "x_scales", tokens, cols // 32, device_ordinal, _Mx.scales)
-        code = 29
-    else:
-        xp, xs = _mx_matrix(x, "x", tokens, cols, device_ordinal, _Mx.real)
-        code = _Mx.real[x.dtype]
-    rows = weight.shape[0] if weight.dim() else 0
-    wp, ws = _mx_matrix(weight, "weight", rows, cols // 2, device_ordinal, _Mx.weight)
-    sp, ss = _mx_matrix(scales, "scales", rows, cols // 32, device_ordinal, _Mx.scales)
-    op, os_ = _mx_matrix(out, "out", tokens, rows, device_ordinal, _Mx.real)
-    if bias is not None:
-        bp = _mx_vector(bias, "bias", rows, device_ordinal, (out.dtype,))
-    if tokens and rows:
-        rc = _Mx.linear(code, xp, xs, cp, cs, wp, ws, sp, ss, _Mx.real[out.dtype], bp, op, os_, tokens, rows, cols,
-                        _Mx.stream(device_ordinal), device_ordinal)
-        if rc:
-            check(rc, "mxfp4_linear_cuda")
+        from . import _mx
+    except ImportError as e:
+        raise RuntimeError(f"{name}: the native module of the operators is missing: build it with "
+                           "`python -m ptwm_amd.build`") from e
+    for n in _MX:
+        globals()[n] = getattr(_mx, n)
+    return globals()[name]

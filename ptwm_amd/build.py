@@ -1,4 +1,5 @@
-"""Build libptwm_mi355x.so in-tree with hipcc for gfx950.
+"""Build libptwm_mi355x.so in-tree with hipcc for gfx950, and the native
+module of the MX operators' Python entry points.
 
 Usage: ``python -m ptwm_amd.build`` (also called by ``__graft_entry__.build``).
 Always recompiles every source: the caller asked for a build.
@@ -14,6 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libptwm_mi355x.so")
+MX = os.path.join(HERE, "_mx.so")  # Python entry points of the MX operators
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["transform.hip", "decode_exact.hip", "decode_sync.hip", "zstd_device.hip", "o1sac_device.hip", "huff_ilv.hip", "rans_ilv.hip", "ilv_host.hip", "rans_host.hip", "huffman_host.cpp", "code_tables.hip", "runtime.hip", "plane_ops.hip",
@@ -45,16 +47,50 @@ def _compile(src: str) -> str:
     return obj
 
 
+def _compile_mx() -> str:
+    """The Python entry points of the MX operators, host code against torch's headers."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    obj = os.path.join(OBJ, "mx_python.o")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *(f"-I{p}" for p in cpp_extension.include_paths()), f"-I{sysconfig.get_path('include')}",
+           "-c", os.path.join(CSRC, "mx_python.cpp"), "-o", obj]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for mx_python.cpp:\n{r.stderr}")
+    if r.stderr.strip():
+        print(r.stderr, file=sys.stderr)
+    return obj
+
+
+def _link_mx(obj: str) -> None:
+    from torch.utils import cpp_extension
+
+    tmp = MX + ".tmp"
+    libs = [f"-L{p}" for p in cpp_extension.library_paths()]
+    cmd = ["g++", "-shared", "-o", tmp, obj, *libs, "-ltorch_python", "-ltorch_cpu", "-lc10", "-ldl"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"link of the MX operators' module failed:\n{r.stderr}")
+    os.replace(tmp, MX)
+
+
 def build(verbose: bool = False) -> str:
     os.makedirs(OBJ, exist_ok=True)
     with cf.ThreadPoolExecutor(max_workers=min(8, len(SOURCES))) as ex:
+        mx = ex.submit(_compile_mx)
         objs = list(ex.map(_compile, SOURCES))
+        mx_obj = mx.result()
     tmp = LIB + ".tmp"
     cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp, *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stderr}")
     os.replace(tmp, LIB)
+    _link_mx(mx_obj)
     if verbose:
         print(f"built {LIB}")
     return LIB
