@@ -11,7 +11,8 @@
 //   - x in e4m3 with scales has 4 significant bits
 //     (v_cvt_scalef32_pk_bf16_fp8);
 //   - x in f16 or f32 is split into two or three bf16 values whose sum is x,
-//     one product each.
+//     one product each; where the weights' scales allow it, f16 is multiplied
+//     as it is, by weights in f16.
 // The instruction that takes codes and scales as they lie in memory
 // (v_mfma_scale_f32_16x16x128_f8f6f4) would halve the matrix time with 8-bit
 // x, but it adds the products of eight neighbours with 13 bits below the
@@ -30,6 +31,7 @@ namespace {
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // bf16 parts that hold a value of type T exactly.
 constexpr int parts_of(uint32_t type) { return type == kTypeF32 ? 3 : type == kTypeF16 ? 2 : 1; }
@@ -78,22 +80,39 @@ __device__ __forceinline__ void parts_of_raw(const Raw8<T>& r, float scale, u32x
 }
 
 // Eight weights of one block as bf16.
-__device__ __forceinline__ bf16x8 weights8(uint32_t w, float scale) {
-  const u32x4 r = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
-  return __builtin_bit_cast(bf16x8, r);
+__device__ __forceinline__ u32x4 weights8(uint32_t w, float scale) {
+  return u32x4_make(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3)));
+}
+
+// The same as f16, where they are in its range.
+__device__ __forceinline__ u32x4 weights8_f16(uint32_t w, float scale) {
+  return u32x4_make(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3)));
+}
+
+// Whether every byte of a word of scales is in 104 .. 135: code times scale, 2^-24 to 6 * 2^8 in magnitude, is then
+// exact in f16.  (A byte that carries into the next one is itself out of range.)
+__device__ __forceinline__ bool scales_fit_f16(uint32_t s) {
+  return ((s + 0x18181818u) & 0xE0E0E0E0u) == 0x80808080u;
 }
 
 __device__ __forceinline__ float scale_f32(uint32_t byte) { return bits_f32(byte << 23); }
 
-__device__ __forceinline__ f32x4 mfma(bf16x8 a, u32x4 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-__device__ __forceinline__ f32x16 mfma32(bf16x8 a, u32x4 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+template <bool F16>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
 // Outputs n .. n+3 of token t with their bias, those that exist.
@@ -160,7 +179,7 @@ __global__ __launch_bounds__(256) void mxfp4_linear_kernel(MxLinearArgs a) {
     for (int f = 0; f < 4; ++f) {
       u32x4 p[parts_of(T)] = {};
       if (in) parts_of_raw<T>(load_raw8<T>(x + ((uint64_t)(k + q) * 32 + f * 8) * type_bytes(T)), x_scale, p);
-      const bf16x8 w8 = weights8(wv[f], scale_f32(sv));
+      const u32x4 w8 = weights8(wv[f], scale_f32(sv));
 #pragma unroll
       for (int j = parts_of(T) - 1; j >= 0; --j) acc = mfma(w8, p[j], acc);
     }
@@ -188,7 +207,7 @@ __global__ __launch_bounds__(256) void mxfp4_linear_kernel(MxLinearArgs a) {
 // load it together and each reads all of it (with RG = 1 a wavefront waits for
 // nobody until the end).  Values go there one step ahead, as they are, and are
 // widened or split as they are read (RAW), or through registers as bf16 parts,
-// where several wavefronts would split the same f16 or f32 values.  Rows are
+// where several wavefronts would split the same f32 values.  Rows are
 // held in 16-byte chunks, chunk ^ row in place (place()), so the 16 lanes that
 // read one chunk of 16 rows at a time meet every bank once.
 //
@@ -419,71 +438,83 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     const Step q = step_of(round + 1);
-    bf16x8 w8[2][RT];
-    float sf[RT], cf[CT];
-    auto widen = [&](int u) {  // the weights of product u
-      const int m = u / 4;
-      const bool in = !last || 2 * m + h < p.left;
-      const uint32_t shift = 8 * ((2 * m + h + (last ? 4 - p.in : 0)) & 3);
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        if (u % 4 == 0) sf[r] = scale_f32(in ? sn[r] >> shift & 0xFF : 127);
-        w8[u & 1][r] = weights8(in ? wv[m][r][u & 3] : 0, sf[r]);
-      }
-    };
-    widen(0);
-#pragma unroll
-    for (int v = 0; v < 8 * kParts; ++v) {
-      const int u = v / kParts, m = u / 4, rd = v / kEach;
-      // what is requested stays ahead of the products it hides behind
-      if (v % kEach == 0 && rd + 1 < kReads) read(rd + 1);
-      if constexpr (!last) {
-        // Large tiles spread the next step's requests over the first half of the products: all at once they hold the
-        // wavefront up, and its products with it, until the address unit has taken them (512x14336x4096 bf16: 71 us,
-        // 62 this way).  Where the weights' way from memory is what takes time they go out at once.
-        constexpr int kOver = (RG > 1 ? 4 : 1) * kParts;
-#pragma unroll
-        for (int k = v * kRequests / kOver; k < (v + 1) * kRequests / kOver && k < kRequests; ++k) request(k, q, next);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      if constexpr (T == kTypeE4m3) {
+    auto products = [&](auto f16) {
+      u32x4 w8[2][RT];
+      float sf[RT], cf[CT];
+      auto widen = [&](int u) {  // the weights of product u
+        const int m = u / 4;
         const bool in = !last || 2 * m + h < p.left;
         const uint32_t shift = 8 * ((2 * m + h + (last ? 4 - p.in : 0)) & 3);
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
-          if (u % 4 == 0) cf[c] = scale_f32(in ? cn[c] >> shift & 0xFF : 127);
-      }
+        for (int r = 0; r < RT; ++r) {
+          if (u % 4 == 0) sf[r] = scale_f32(in ? sn[r] >> shift & 0xFF : 127);
+          const uint32_t w = in ? wv[m][r][u & 3] : 0;
+          w8[u & 1][r] = f16 ? weights8_f16(w, sf[r]) : weights8(w, sf[r]);
+        }
+      };
+      widen(0);
 #pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        if constexpr (RAW) {
-          Raw8<T> r8;
-          if constexpr (T == kTypeE4m3) {
-            const uint32_t lo = x8[rd & 1][c][0][u % 2 * 2], hi = x8[rd & 1][c][0][u % 2 * 2 + 1];
-            r8.w = lo | (uint64_t)hi << 32;
+      for (int v = 0; v < 8 * kParts; ++v) {
+        const int u = v / kParts, m = u / 4, rd = v / kEach;
+        // what is requested stays ahead of the products it hides behind
+        if (v % kEach == 0 && rd + 1 < kReads) read(rd + 1);
+        if constexpr (!last) {
+          // Large tiles spread the next step's requests over the first half of the products: all at once they hold the
+          // wavefront up, and its products with it, until the address unit has taken them (512x14336x4096 bf16: 71 us,
+          // 62 this way).  Where the weights' way from memory is what takes time they go out at once.
+          constexpr int kOver = (RG > 1 ? 4 : 1) * kParts;
+#pragma unroll
+          for (int k = v * kRequests / kOver; k < (v + 1) * kRequests / kOver && k < kRequests; ++k) request(k, q, next);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (T == kTypeE4m3) {
+          const bool in = !last || 2 * m + h < p.left;
+          const uint32_t shift = 8 * ((2 * m + h + (last ? 4 - p.in : 0)) & 3);
+#pragma unroll
+          for (int c = 0; c < CT; ++c)
+            if (u % 4 == 0) cf[c] = scale_f32(in ? cn[c] >> shift & 0xFF : 127);
+        }
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          if constexpr (RAW && !f16) {
+            Raw8<T> r8;
+            if constexpr (T == kTypeE4m3) {
+              const uint32_t lo = x8[rd & 1][c][0][u % 2 * 2], hi = x8[rd & 1][c][0][u % 2 * 2 + 1];
+              r8.w = lo | (uint64_t)hi << 32;
+            } else {
+#pragma unroll
+              for (int g = 0; g < G; ++g) r8.w[g] = x8[rd & 1][c][g];
+            }
+            u32x4 b[P];
+            parts_of_raw<T>(r8, cf[c], b);
+#pragma unroll
+            for (int part = P - 1; part >= 0; --part)
+#pragma unroll
+              for (int r = 0; r < RT; ++r) acc[r][c] = mfma32<false>(w8[u & 1][r], b[part], acc[r][c]);
           } else {
 #pragma unroll
-            for (int g = 0; g < G; ++g) r8.w[g] = x8[rd & 1][c][g];
+            for (int r = 0; r < RT; ++r) acc[r][c] = mfma32<f16>(w8[u & 1][r], x8[rd & 1][c][0], acc[r][c]);
           }
-          u32x4 b[P];
-          parts_of_raw<T>(r8, cf[c], b);
-#pragma unroll
-          for (int part = P - 1; part >= 0; --part)
-#pragma unroll
-            for (int r = 0; r < RT; ++r) acc[r][c] = mfma32(w8[u & 1][r], b[part], acc[r][c]);
-        } else {
-#pragma unroll
-          for (int r = 0; r < RT; ++r) acc[r][c] = mfma32(w8[u & 1][r], x8[rd & 1][c][0], acc[r][c]);
         }
-      }
-      // the next product's weights are widened while the matrix unit works: an instruction of it takes the time of
-      // about six others, and the wavefront is free in between
-      if (v % kParts == kParts - 1 && u < 7) widen(u + 1);
+        // the next product's weights are widened while the matrix unit works: an instruction of it takes the time of
+        // about six others, and the wavefront is free in between
+        if (v % kParts == kParts - 1 && u < 7) widen(u + 1);
 #pragma unroll
-      for (int k = 0; k < CT * RT * (RAW ? P : 1); ++k) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
-        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // up to four others
+        for (int k = 0; k < CT * RT * (RAW && !f16 ? P : 1); ++k) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
+          __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // up to four others
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
+    };
+    // f16 needs no split where the weights are exact in f16 as well, which their scales tell
+    if constexpr (T == kTypeF16) {
+      if (__all(scales_fit_f16(sv)))
+        products(std::true_type{});
+      else
+        products(std::false_type{});
+    } else {
+      products(std::false_type{});
     }
     if constexpr (!last) store(next);
   };
@@ -688,26 +719,25 @@ hipError_t few_of(const MxLinearArgs& a, hipStream_t stream) {
                 (uint32_t)few_bytes(a.cols, NT));
 }
 
-// Whether the few tokens' kernel takes the call, and with what outcome.  Its LDS is kept to 60 KiB.  One token of f16
-// or f32: measured (us, this kernel and the tiles) 1x14336x4096 f32 9.6 and 29, f16 9.4 and 17, 1x4096x4096 f32 3.8 and
-// 15.  One of bf16 or e4m3 where there are few rows: 1x4096x14336 e4m3 9.0 and 11.2, 1x1024x4096 bf16 3.7 and 5.1,
-// 1x8192x8192 10.7 and 10.5, 1x14336x4096 9.5 and 8.0.  Two of f16 or f32, up to four of f32, whose splitting costs the
-// tiles most: 2x1024x4096 f32 4.8 and 15, 4x1024x3584 f32 6.5 and 13, bf16 6.5 and 5.5.
+// Whether the few tokens' kernel takes the call, and with what outcome.  Its LDS is kept to 60 KiB.  One token where
+// there are few rows: measured (us, this kernel and the tiles) 1x4096x14336 e4m3 9.0 and 11.2, 1x1024x4096 bf16 3.7 and
+// 5.1, 1x8192x8192 10.7 and 10.5, 1x14336x4096 9.5 and 8.0.  Up to four of f32, whose splitting costs the tiles most:
+// 1x14336x4096 9.6 and 29, 2x1024x4096 4.8 and 15, 4x1024x3584 6.5 and 13 (bf16 6.5 and 5.5).
 template <uint32_t T>
 bool few_taken(const MxLinearArgs& a, hipStream_t stream, hipError_t& e) {
-  constexpr int P = parts_of(T);
   const auto fits = [&](uint64_t nt) { return a.tokens <= nt && few_bytes(a.cols, nt) <= 60 * 1024; };
-  if (fits(1) && (P > 1 || a.rows <= 6144)) return e = few_of<T, 1>(a, stream), true;
-  if constexpr (P > 1)
+  if (fits(1) && (T == kTypeF32 || a.rows <= 6144)) return e = few_of<T, 1>(a, stream), true;
+  if constexpr (T == kTypeF32) {
     if (fits(2)) return e = few_of<T, 2>(a, stream), true;
-  if constexpr (P > 2)
     if (fits(4)) return e = few_of<T, 4>(a, stream), true;
+  }
   return false;
 }
 
 template <uint32_t T>
 hipError_t tiles_by_size(const MxLinearArgs& a, hipStream_t stream) {
-  constexpr bool kPlain = parts_of(T) == 1;
+  constexpr bool kPlain = T != kTypeF32;
+  // registers hold 128 tokens, but not with f16's two ways
   constexpr int CT = T == kTypeF32 ? 1 : T == kTypeF16 ? 2 : 4, KG = T == kTypeF32 ? 4 : 8;
   auto count = [&](uint64_t rows, uint64_t tokens) {
     return ((a.rows + rows - 1) / rows) * ((a.tokens + tokens - 1) / tokens);
@@ -718,7 +748,7 @@ hipError_t tiles_by_size(const MxLinearArgs& a, hipStream_t stream) {
   // 1024x4096x4096 bf16 (128, 256) 50, 38, 54; 128x14336x4096 bf16 (56, 112) 49, 32, 30; 200x5000x5120 e4m3 (40, 80)
   // 61, 41, 24.
   if (count(256, 32 * CT) >= 160) return tiles_of<T, 64, CT, 4, 1, kPlain>(a, stream);
-  if constexpr (kPlain)
+  if constexpr (CT == 4)
     if (count(256, 64) >= 160) return tiles_of<T, 64, 2, 4, 1, kPlain>(a, stream);
   // As many wavefronts to a tile as LDS holds where each tile has a CU of its own: 45x1354x960 bf16 (86 tiles of 32
   // rows) 4.0 and 4.8 with four, 100x4096x4096 e4m3 (256 of 64 rows) 8.9 and 9.3.

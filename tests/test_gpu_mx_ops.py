@@ -174,6 +174,26 @@ def test_linear_infinities_and_nan(kind, tokens):
         assert torch.isnan(o[0]).all() and torch.equal(o[1:], c[1:])
 
 
+@pytest.mark.parametrize("low,high", [(100, 108), (104, 136), (103, 104), (130, 137), (0, 255)])
+@pytest.mark.parametrize("tokens,rows", [(3, 100), (40, 200), (700, 4500)])
+def test_linear_f16_scales_in_and_out_of_the_types_range(tokens, rows, low, high):
+    """Weights that f16 holds, below its normal numbers too, and weights that it does not; activations among its smallest."""
+    g = gen(tokens, low)
+    codes, scales = P.random_weights(rows, 352, g, D, low, high)
+    x = torch.randn(tokens, 352, generator=g)
+    x[:, ::3] *= 2.0**-20  # below f16's normal numbers
+    x = x.to(torch.float16).to(D)
+    o = torch.empty(tokens, rows, device=D)
+    api.mxfp4_linear_cuda(x, codes, scales, o)
+    w = P.weights(codes, scales)
+    if high < 255:
+        P.check_linear(o, x, None, codes, scales)
+    else:  # sums may pass float32's largest number: those that do not are right
+        y, mag = x.double() @ w.t(), x.double().abs() @ w.abs().t()
+        small = (mag < 2.0**127) & (w.abs().amax(1) < 2.0**127)
+        assert ((o.double() - y).abs() <= (352 / 32 + 129) * 2.0**-23 * mag + 352 * 2.0**-126)[small].all()
+
+
 def test_linear_e4m3_nan_and_scale_nan():
     x, xs, codes, scales, _, o = linear_case(5, 40, 128, F8, torch.float32, False, gen(11))
     c = torch.empty_like(o)
