@@ -750,9 +750,10 @@ hipError_t tiles_by_size(const MxLinearArgs& a, hipStream_t stream) {
   if (count(256, 32 * CT) >= 160) return tiles_of<T, 64, CT, 4, 1, kPlain>(a, stream);
   if constexpr (CT == 4)
     if (count(256, 64) >= 160) return tiles_of<T, 64, 2, 4, 1, kPlain>(a, stream);
-  // As many wavefronts to a tile as LDS holds where each tile has a CU of its own: 45x1354x960 bf16 (86 tiles of 32
-  // rows) 4.0 and 4.8 with four, 100x4096x4096 e4m3 (256 of 64 rows) 8.9 and 9.3.
-  if (count(32, 32) <= 128) return tiles_of<T, 32, 1, 1, KG, true>(a, stream);
+  // As many wavefronts to a tile as LDS holds where each tile has a CU of its own, the smaller tile if it still has:
+  // 45x1354x960 bf16 (86 tiles of 32 rows) 4.0 and 4.8 with four wavefronts, 32x5120x4096 bf16 (160) 7.2 and 9.3 with
+  // 64 rows, 64x4096x4096 e4m3 (256) 6.8 and 8.9; 96x4096x4096 bf16 (384 of 32 rows, 192 of 64) 11.3 and 9.7.
+  if (count(32, 32) <= 256) return tiles_of<T, 32, 1, 1, KG, true>(a, stream);
   // Few tokens read each weight once, and more, smaller tiles keep more of them in flight: 1x14336x4096 bf16 7.7 and
   // 8.2 with 64 rows.
   if (a.tokens <= 16 && count(32, 32) <= 512) return tiles_of<T, 32, 1, 1, 4, true>(a, stream);
