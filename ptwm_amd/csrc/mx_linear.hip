@@ -145,8 +145,10 @@ __device__ __forceinline__ void store4(const MxLinearArgs& a, uint64_t t, uint32
     store4_as<kTypeF32>(a, t, n, v);
 }
 
-// A 16x16 tile of outputs by one workgroup, whose wavefronts take turns in
-// steps of 128 values (four blocks) along the rows and add up in LDS.  Lane l
+// Small products, and rows too far apart for 32-bit offsets: a 16x16 tile of
+// outputs by one workgroup, whose wavefronts take turns in steps of 128 values
+// (four blocks) along the rows and add up in LDS, operands straight from
+// memory; bound by one way to memory (16x4096x256 bf16 2.8 us).  Lane l
 // holds weight row l % 16 and block l / 16 of the step, and token l % 16.
 template <uint32_t T>
 __global__ __launch_bounds__(256) void mxfp4_linear_kernel(MxLinearArgs a) {
@@ -234,7 +236,7 @@ __device__ __forceinline__ uint32_t place(uint32_t t, uint32_t c) {
 }
 
 template <uint32_t T, int ROWS, int CT, int RG, int KG, bool RAW, bool ALIGNED>
-__global__ __launch_bounds__(64 * RG * KG, RG * KG <= 4 ? 1 + (ROWS * CT * RG > 512) : RG * KG / 4)
+__global__ __launch_bounds__(64 * RG * KG, RG * KG <= 4 ? 1 + (ROWS * CT * RG >= 512) : RG * KG / 4)
 void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
   static_assert(RAW || parts_of(T) > 1, "what needs no split goes as it is");
   constexpr int P = parts_of(T), RT = ROWS / 32, R16 = ROWS / 16;
@@ -518,8 +520,22 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
     }
     if constexpr (!last) store(next);
   };
+  // Rows of less than a step have their scales gathered, bytes past the word's start left as 2^0.
+  auto gather = [&](GlobalBytes g, uint32_t at) {
+    uint32_t word = 0x7F7F7F7Fu;
+    for (uint32_t b = 0; b < blocks; ++b) word = word >> 8 | (uint32_t)g[at + b] << 24;
+    return word;
+  };
 #pragma unroll
-  for (int k = 0; k < kRequests; ++k) request(k, step_of(0), even);
+  for (int k = 0; k < kRequests; ++k)
+    if (k >= kScales || blocks >= 4) request(k, step_of(0), even);
+  if (blocks < 4) {
+    sv = gather(s0, so);
+    if constexpr (T == kTypeE4m3) {
+#pragma unroll
+      for (int c = 0; c < XS; ++c) cv[c] = gather(c0, co[c]);
+    }
+  }
   store(even);
   uint32_t round = 0;
   for (; round + 2 < rounds; round += 2) {
@@ -545,6 +561,54 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
     return f32x4{acc[r][c][4 * j], acc[r][c][4 * j + 1], acc[r][c][4 * j + 2], acc[r][c][4 * j + 3]};
   };
   if constexpr (KG == 1) {
+    if (ROWS == 64 && n0 + ROWS <= a.rows) {
+      // Through the wavefront's own codes' LDS, so that eight lanes store 128 bytes of a token's outputs, and not a
+      // lane 8 of them: 1039x11937x96 bf16 15 us, 20 without; 512x14336x1024 bf16 19.7 and 22.1; 2048x14336x4096 e4m3
+      // 195 and 202, f16 236 and 245.
+      auto rows_first = [&](auto type) {
+        constexpr uint32_t OT = type;
+        constexpr int R = OT == kTypeF32 ? 1 : RT;  // groups of 32 rows in 128 bytes
+        f32x4 bias[RT][4] = {};
+        if (a.bias) {
+#pragma unroll
+          for (int k = 0; k < RT * 16; ++k)
+            bias[k / 16][k / 4 % 4][k % 4] =
+                load1<OT>(a.bias + (uint64_t)(n0 + k / 16 * 32 + k / 4 % 4 * 8 + h * 4 + k % 4) * type_bytes(OT));
+        }
+#pragma unroll
+        for (int pass = 0; pass < RT * CT / R; ++pass) {
+          const int c = pass * R / RT, r0 = pass * R % RT;
+#pragma unroll
+          for (int k = 0; k < R * 4; ++k) {
+            const int r = r0 + k / 4, j = k % 4;
+            const f32x4 v = quad_of((r * CT + c) * 4 + j) + bias[r][j];
+            if constexpr (OT == kTypeF32) {
+              codes[i * 8 + ((2 * j + h) ^ (i & 7))] = __builtin_bit_cast(u32x4, v);
+            } else {
+              const uint64_t two = pack2<OT>(v[0], v[1]) | (uint64_t)pack2<OT>(v[2], v[3]) << 32;
+              reinterpret_cast<uint64_t*>(codes)[2 * (i * 8 + (k ^ (i & 7))) + h] = two;
+            }
+          }
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // other lanes' values
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t t = k * 8 + lane / 8;
+            const u32x4 v = codes[t * 8 + ((lane & 7) ^ (t & 7))];
+            const uint64_t at = t0 + c * 32 + t;
+            if (at < a.tokens)
+              st16(a.out.ptr + (at * a.out.stride + n0 + r0 * 32) * type_bytes(OT) + (lane & 7) * 16, v);
+          }
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // before the next pass writes there
+        }
+      };
+      if (a.out_type == kTypeBf16)
+        rows_first(std::integral_constant<uint32_t, kTypeBf16>{});
+      else if (a.out_type == kTypeF16)
+        rows_first(std::integral_constant<uint32_t, kTypeF16>{});
+      else
+        rows_first(std::integral_constant<uint32_t, kTypeF32>{});
+      return;
+    }
 #pragma unroll
     for (int quad = 0; quad < kQuads; ++quad) write(quad, quad_of(quad));
   } else {
@@ -694,9 +758,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void mxfp4_linear_few_kernel(MxLine
   }
 }
 
-// Whether a tile's rows and tokens lie within 32-bit offsets and a row's scales fill a word.
+// Whether a tile's rows and tokens lie within 32-bit offsets.
 bool tiles_fit(const MxLinearArgs& a) {
-  return a.cols >= 128 && a.weight.stride < (1u << 23) && a.x.stride < (1u << 23) && a.scales.stride < (1u << 23) && a.x_scales.stride < (1u << 23);
+  return a.weight.stride < (1u << 23) && a.x.stride < (1u << 23) && a.scales.stride < (1u << 23) && a.x_scales.stride < (1u << 23);
 }
 
 template <uint32_t T, int ROWS, int CT, int RG, int KG, bool RAW>
@@ -748,6 +812,11 @@ hipError_t tiles_by_size(const MxLinearArgs& a, hipStream_t stream) {
   // 1024x4096x4096 bf16 (128, 256) 50, 38, 54; 128x14336x4096 bf16 (56, 112) 49, 32, 30; 200x5000x5120 e4m3 (40, 80)
   // 61, 41, 24.
   if (count(256, 32 * CT) >= 160) return tiles_of<T, 64, CT, 4, 1, kPlain>(a, stream);
+  // Rows of two steps at most leave nothing to share, and the products are soon over: a wavefront a tile.  300x5001x128
+  // bf16 4.8 and 8.7 with tiles as below, 64x4704x256 3.8 and 4.7; 700x3000x128 5.4 with 64 rows, 6.2 with 32.
+  if constexpr (T != kTypeF32)
+    if (a.cols <= 256)
+      return count(32, 32) > 1600 ? tiles_of<T, 64, 1, 1, 1, true>(a, stream) : tiles_of<T, 32, 1, 1, 1, true>(a, stream);
   if constexpr (CT == 4)
     if (count(256, 64) >= 160) return tiles_of<T, 64, 2, 4, 1, kPlain>(a, stream);
   // As many wavefronts to a tile as LDS holds where each tile has a CU of its own, the smaller tile if it still has:
@@ -768,8 +837,15 @@ hipError_t tiles_by_size(const MxLinearArgs& a, hipStream_t stream) {
 template <uint32_t T>
 hipError_t linear_of(const MxLinearArgs& a, hipStream_t stream) {
   hipError_t e = hipSuccess;
-  if (tiles_fit(a)) return few_taken<T>(a, stream, e) ? e : tiles_by_size<T>(a, stream);
   const uint64_t tiles = (uint64_t)((a.rows + 15) / 16) * ((a.tokens + 15) / 16);
+  // Small products end sooner without stages in LDS, each wavefront a step of a small tile: 16x4096x256 bf16 2.8 us and
+  // 4.0 with tiles, 2x1024x96 2.6 and 4.1, 100x1024x512 3.5 and 4.1, 16x4096x256 f32 3.4 and 5.2; 64x4704x512 bf16 (4704
+  // steps) 5.5 and 4.8.
+  const bool small = a.cols <= 512 && tiles * ((a.cols + 127) / 128) <= 2048;
+  if (tiles_fit(a)) {
+    if (few_taken<T>(a, stream, e)) return e;
+    if (!small) return tiles_by_size<T>(a, stream);
+  }
   return launch(mxfp4_linear_kernel<T>, tiles, 256, a, stream);
 }
 

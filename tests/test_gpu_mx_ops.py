@@ -83,6 +83,44 @@ def test_linear_choices(tokens, rows, cols, kind):
     P.check_linear(o, x, xs, codes, scales, b)
 
 
+# Rows of one to three blocks, less than the kernels' step, in every kernel.
+@pytest.mark.parametrize("kind", TYPES + [F8], ids=str)
+@pytest.mark.parametrize("tokens,rows", [(1, 77), (4, 7000), (19, 515), (70, 6000), (260, 5001), (1500, 3500)])
+@pytest.mark.parametrize("cols", [32, 64, 96])
+def test_linear_short_rows(tokens, rows, cols, kind):
+    x, xs, codes, scales, b, o = linear_case(tokens, rows, cols, kind, torch.float32, True, gen(tokens, rows, cols, 5))
+    api.mxfp4_linear_cuda(x, codes, scales, o, 0, x_scales=xs, bias=b)
+    P.check_linear(o, x, xs, codes, scales, b)
+    r = torch.full_like(o, float("nan"))  # the same from places that no load can take whole
+    api.mxfp4_linear_cuda(strided(x, 3, 1), strided(codes, 5, 3), strided(scales, 1, 1), r, 0,
+                          x_scales=None if xs is None else strided(xs, 1, 1), bias=b)
+    assert torch.equal(o, r)
+
+
+# Rows so far apart that offsets pass 32 bits: the weights', or the activations' and the outputs'.
+@pytest.mark.parametrize("kind", TYPES + [F8], ids=str)
+@pytest.mark.parametrize("tokens,rows,far", [(3, 530, "weights"), (530, 40, "tokens")])
+def test_linear_far_rows(tokens, rows, far, kind):
+    def apart(t, stride):
+        big = torch.empty((t.shape[0] - 1) * stride + t.shape[1], dtype=t.dtype, device=D)
+        v = big.as_strided(t.shape, (stride, 1))
+        v.copy_(t)
+        return v
+
+    x, xs, codes, scales, b, o = linear_case(tokens, rows, 352, kind, torch.float32, True, gen(tokens, rows, 6))
+    far_o = o
+    if far == "weights":
+        codes = apart(codes, (1 << 23) + 16)
+    else:
+        x, far_o = apart(x, (1 << 23) + 8), apart(o, (1 << 22) + 4)
+    api.mxfp4_linear_cuda(x, codes, scales, far_o, 0, x_scales=xs, bias=b)
+    o.copy_(far_o)
+    x, codes = x.contiguous(), codes.contiguous()
+    P.check_linear(o, x, xs, codes, scales, b)
+    del far_o
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("out", TYPES, ids=str)
 @pytest.mark.parametrize("kind", TYPES + [F8], ids=str)
 @pytest.mark.parametrize("tokens", [1, 5, 48, 160])
