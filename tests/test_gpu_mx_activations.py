@@ -39,3 +39,15 @@ def test_swiglu_rounds_like_32_bits(low, high):
         assert far.all()
         got = one_value_blocks(gate, up)[0]
         assert (got == byte).all(), f"{(got != byte).sum().item()} of {gate.numel()} values of the other scale"
+
+
+def test_swiglu_of_gates_below_the_normal_numbers():
+    """gate / 2 is a number of the type as far as gate is an even multiple of the smallest one."""
+    m = torch.arange(1, 4097, dtype=torch.float64)
+    gate = torch.cat([m, -m, m * 4096]) * 2.0**-148
+    for up in (2.0**100, -1.5 * 2.0**120, 1.0):
+        y = torch.zeros(gate.numel(), 32, dtype=torch.float64)
+        y[:, 5] = gate / 2 * up
+        assert torch.equal(gate.float().double(), gate)
+        _, codes, scales = one_value_blocks(gate.float(), torch.full_like(gate, up).float())
+        P.check_codes(codes, scales, y.to(D), UNITS * 2.0**-24)
