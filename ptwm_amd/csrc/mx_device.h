@@ -57,10 +57,6 @@ __device__ __forceinline__ uint32_t ld4(GlobalBytes p, uint32_t at) {
   return ((const __attribute__((address_space(1))) Bytes4*)(p + at))->v;
 }
 
-__host__ __device__ constexpr uint32_t type_bytes(uint32_t type) {
-  return type == kTypeF32 ? 4 : type == kTypeE4m3 ? 1 : 2;
-}
-
 __device__ __forceinline__ float bits_f32(uint32_t b) { return __builtin_bit_cast(float, b); }
 __device__ __forceinline__ uint32_t f32_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
 

@@ -23,6 +23,7 @@
 
 #include <type_traits>
 
+#include "mx_choice.h"
 #include "mx_device.h"
 
 namespace ptwm {
@@ -226,7 +227,7 @@ __global__ __launch_bounds__(256) void mxfp4_linear_kernel(MxLinearArgs a) {
 // What goes to LDS as it is goes by DMA where it lies at multiples of 16 bytes
 // (ALIGNED) and through registers otherwise, to the same places: results do
 // not depend on how operands lie.  Offsets within a tile are 32 bits on top of uniform addresses
-// (tiles_fit()), which is what leaves registers for the operands in flight.
+// (mx_tiles_fit()), which is what leaves registers for the operands in flight.
 
 // The place of 16-byte chunk c of row t among rows of S chunks.
 template <uint32_t S>
@@ -758,94 +759,53 @@ __global__ __launch_bounds__(64 * kFewWaves) void mxfp4_linear_few_kernel(MxLine
   }
 }
 
-// Whether a tile's rows and tokens lie within 32-bit offsets.
-bool tiles_fit(const MxLinearArgs& a) {
-  return a.weight.stride < (1u << 23) && a.x.stride < (1u << 23) && a.scales.stride < (1u << 23) && a.x_scales.stride < (1u << 23);
-}
-
 template <uint32_t T, int ROWS, int CT, int RG, int KG, bool RAW>
-hipError_t tiles_of(const MxLinearArgs& a, hipStream_t stream) {
+hipError_t tiles_of(const MxLinearArgs& a, bool aligned, hipStream_t stream) {
   constexpr uint32_t kRows = ROWS * RG, kTokens = 32 * CT;
   const uint64_t tiles = (uint64_t)((a.rows + kRows - 1) / kRows) * ((a.tokens + kTokens - 1) / kTokens);
-  const bool aligned = a.weight.ptr % 16 == 0 && a.weight.stride % 16 == 0 &&
-                       (!RAW || (a.x.ptr % 16 == 0 && a.x.stride * type_bytes(T) % 16 == 0));
   return launch(aligned ? mxfp4_linear_tiles_kernel<T, ROWS, CT, RG, KG, RAW, true>
                         : mxfp4_linear_tiles_kernel<T, ROWS, CT, RG, KG, RAW, false>,
                 tiles, 64 * RG * KG, a, stream);
 }
 
-// LDS that the few tokens' kernel takes: NT tokens in 32 bits, whole steps.
-constexpr uint64_t few_bytes(uint64_t cols, uint64_t nt) { return (cols + 127) / 128 * 128 * nt * 4; }
-
 template <uint32_t T, int NT>
 hipError_t few_of(const MxLinearArgs& a, hipStream_t stream) {
   return launch(mxfp4_linear_few_kernel<T, NT>, (a.rows + 15) / 16, 64 * kFewWaves, a, stream,
-                (uint32_t)few_bytes(a.cols, NT));
-}
-
-// Whether the few tokens' kernel takes the call, and with what outcome.  Its LDS is kept to 60 KiB.  One token where
-// there are few rows: measured (us, this kernel and the tiles) 1x4096x14336 e4m3 9.0 and 11.2, 1x1024x4096 bf16 3.7 and
-// 5.1, 1x8192x8192 10.7 and 10.5, 1x14336x4096 9.5 and 8.0.  Up to four of f32, whose splitting costs the tiles most:
-// 1x14336x4096 9.6 and 29, 2x1024x4096 4.8 and 15, 4x1024x3584 6.5 and 13 (bf16 6.5 and 5.5).
-template <uint32_t T>
-bool few_taken(const MxLinearArgs& a, hipStream_t stream, hipError_t& e) {
-  const auto fits = [&](uint64_t nt) { return a.tokens <= nt && few_bytes(a.cols, nt) <= 60 * 1024; };
-  if (fits(1) && (T == kTypeF32 || a.rows <= 6144)) return e = few_of<T, 1>(a, stream), true;
-  if constexpr (T == kTypeF32) {
-    if (fits(2)) return e = few_of<T, 2>(a, stream), true;
-    if (fits(4)) return e = few_of<T, 4>(a, stream), true;
-  }
-  return false;
-}
-
-template <uint32_t T>
-hipError_t tiles_by_size(const MxLinearArgs& a, hipStream_t stream) {
-  constexpr bool kPlain = T != kTypeF32;
-  // registers hold 128 tokens, but not with f16's two ways
-  constexpr int CT = T == kTypeF32 ? 1 : T == kTypeF16 ? 2 : 4, KG = T == kTypeF32 ? 4 : 8;
-  auto count = [&](uint64_t rows, uint64_t tokens) {
-    return ((a.rows + rows - 1) / rows) * ((a.tokens + tokens - 1) / tokens);
-  };
-  // Tiles of 256 rows where there are enough for the 256 CUs, with half the tokens where there are not, then smaller
-  // ones whose wavefronts share the length of the rows: measured (us; 256 rows and 128 tokens, 64 tokens, shared)
-  // 512x14336x4096 bf16 (224 tiles of 128) 62, 68, 98; 256x14336x4096 bf16 (112 of 128, 224 of 64) 52, 36, 55;
-  // 1024x4096x4096 bf16 (128, 256) 50, 38, 54; 128x14336x4096 bf16 (56, 112) 49, 32, 30; 200x5000x5120 e4m3 (40, 80)
-  // 61, 41, 24.
-  if (count(256, 32 * CT) >= 160) return tiles_of<T, 64, CT, 4, 1, kPlain>(a, stream);
-  // Rows of two steps at most leave nothing to share, and the products are soon over: a wavefront a tile.  300x5001x128
-  // bf16 4.8 and 8.7 with tiles as below, 64x4704x256 3.8 and 4.7; 700x3000x128 5.4 with 64 rows, 6.2 with 32.
-  if constexpr (T != kTypeF32)
-    if (a.cols <= 256)
-      return count(32, 32) > 1600 ? tiles_of<T, 64, 1, 1, 1, true>(a, stream) : tiles_of<T, 32, 1, 1, 1, true>(a, stream);
-  if constexpr (CT == 4)
-    if (count(256, 64) >= 160) return tiles_of<T, 64, 2, 4, 1, kPlain>(a, stream);
-  // As many wavefronts to a tile as LDS holds where each tile has a CU of its own, the smaller tile if it still has:
-  // 45x1354x960 bf16 (86 tiles of 32 rows) 4.0 and 4.8 with four wavefronts, 32x5120x4096 bf16 (160) 7.2 and 9.3 with
-  // 64 rows, 64x4096x4096 e4m3 (256) 6.8 and 8.9; 96x4096x4096 bf16 (384 of 32 rows, 192 of 64) 11.3 and 9.7.
-  if (count(32, 32) <= 256) return tiles_of<T, 32, 1, 1, KG, true>(a, stream);
-  // Few tokens read each weight once, and more, smaller tiles keep more of them in flight: 1x14336x4096 bf16 7.7 and
-  // 8.2 with 64 rows.
-  if (a.tokens <= 16 && count(32, 32) <= 512) return tiles_of<T, 32, 1, 1, 4, true>(a, stream);
-  if (count(64, 32) <= 256) return tiles_of<T, 64, 1, 1, KG, true>(a, stream);
-  // Two workgroups share a CU's LDS with 64 tokens of e4m3, with 32 of the others: 700x3000x2048 bf16 21 and 26 with
-  // 64 tokens, 256x14336x4096 e4m3 41 and 48 with 32.
-  if constexpr (T == kTypeE4m3)
-    if (a.tokens > 32) return tiles_of<T, 64, 2, 1, 4, true>(a, stream);
-  return tiles_of<T, 64, 1, 1, 4, true>(a, stream);
+                (uint32_t)mx_few_bytes(a.cols, NT));
 }
 
 template <uint32_t T>
 hipError_t linear_of(const MxLinearArgs& a, hipStream_t stream) {
-  hipError_t e = hipSuccess;
-  const uint64_t tiles = (uint64_t)((a.rows + 15) / 16) * ((a.tokens + 15) / 16);
-  // Small products end sooner without stages in LDS, each wavefront a step of a small tile: 16x4096x256 bf16 2.8 us and
-  // 4.0 with tiles, 2x1024x96 2.6 and 4.1, 100x1024x512 3.5 and 4.1, 16x4096x256 f32 3.4 and 5.2; 64x4704x512 bf16 (4704
-  // steps) 5.5 and 4.8.
-  const bool small = a.cols <= 512 && tiles * ((a.cols + 127) / 128) <= 2048;
-  if (tiles_fit(a)) {
-    if (few_taken<T>(a, stream, e)) return e;
-    if (!small) return tiles_by_size<T>(a, stream);
+  const MxLinearChoice k = choose_mxfp4_linear(T, a);
+  if (k.kind == MxLinearChoice::kFew) {
+    if (k.tokens == 1) return few_of<T, 1>(a, stream);
+    if constexpr (T == kTypeF32) {
+      if (k.tokens == 2) return few_of<T, 2>(a, stream);
+      if (k.tokens == 4) return few_of<T, 4>(a, stream);
+    }
+    return hipErrorInvalidValue;
   }
+  if (k.kind == MxLinearChoice::kTiles) {
+    constexpr int CT = mx_large_columns(T), KG = mx_sharing(T);
+    const auto is = [&](uint32_t rows, uint32_t ct, uint32_t rg, uint32_t kg) {
+      return k.rows == rows && k.ct == ct && k.rg == rg && k.kg == kg;
+    };
+    if (is(64, CT, 4, 1)) return tiles_of<T, 64, CT, 4, 1, T != kTypeF32>(a, k.aligned, stream);
+    if (is(32, 1, 1, KG)) return tiles_of<T, 32, 1, 1, KG, true>(a, k.aligned, stream);
+    if (is(64, 1, 1, KG)) return tiles_of<T, 64, 1, 1, KG, true>(a, k.aligned, stream);
+    if constexpr (T != kTypeF32) {
+      if (is(32, 1, 1, 4)) return tiles_of<T, 32, 1, 1, 4, true>(a, k.aligned, stream);
+      if (is(64, 1, 1, 4)) return tiles_of<T, 64, 1, 1, 4, true>(a, k.aligned, stream);
+      if (is(32, 1, 1, 1)) return tiles_of<T, 32, 1, 1, 1, true>(a, k.aligned, stream);
+      if (is(64, 1, 1, 1)) return tiles_of<T, 64, 1, 1, 1, true>(a, k.aligned, stream);
+    }
+    if constexpr (CT == 4)
+      if (is(64, 2, 4, 1)) return tiles_of<T, 64, 2, 4, 1, true>(a, k.aligned, stream);
+    if constexpr (T == kTypeE4m3)
+      if (is(64, 2, 1, 4)) return tiles_of<T, 64, 2, 1, 4, true>(a, k.aligned, stream);
+    return hipErrorInvalidValue;
+  }
+  const uint64_t tiles = (uint64_t)((a.rows + 15) / 16) * ((a.tokens + 15) / 16);
   return launch(mxfp4_linear_kernel<T>, tiles, 256, a, stream);
 }
 

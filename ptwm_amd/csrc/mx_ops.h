@@ -14,6 +14,9 @@ namespace ptwm {
 // Element types by their public dtype codes (dtype.rs:79-103).
 constexpr uint32_t kTypeF32 = 1, kTypeF16 = 4, kTypeBf16 = 6, kTypeE4m3 = 29;
 constexpr uint32_t kMxBlock = 32;
+__host__ __device__ constexpr uint32_t type_bytes(uint32_t type) {
+  return type == kTypeF32 ? 4 : type == kTypeE4m3 ? 1 : 2;
+}
 
 // A row-major operand: device address and row stride in elements (of scales:
 // in bytes).  Addresses need no alignment beyond the element's.
