@@ -24,9 +24,11 @@ constexpr uint32_t mx_large_columns(uint32_t type) { return type == kTypeF32 ? 1
 // Wavefronts that share the length of the rows: as many as LDS holds stages for.
 constexpr uint32_t mx_sharing(uint32_t type) { return type == kTypeF32 ? 4 : 8; }
 
-// Whether a tile's rows and tokens lie within 32-bit offsets.
-inline bool mx_tiles_fit(const MxLinearArgs& a) {
-  return a.weight.stride < (1u << 23) && a.x.stride < (1u << 23) && a.scales.stride < (1u << 23) && a.x_scales.stride < (1u << 23);
+// Whether `count` rows that lie `stride` elements apart, and `tail` bytes from the last one's start, are within 32-bit
+// offsets of the first.  A single row's stride is of no account: tensors leave anything there, as a batch of one that is
+// cut from longer ones (hidden[:, -1]) does.
+inline bool mx_within_reach(uint64_t count, uint64_t stride, uint32_t element, uint32_t tail) {
+  return count <= 1 || (stride <= 0xFFFFFFFFu && (count - 1) * stride * element + tail <= 0xFFFFFFFFu);
 }
 
 // Up to how many tokens the few tokens' kernel takes the call with, 0 if it does not.  Its LDS is kept to 60 KiB.  One
@@ -35,16 +37,28 @@ inline bool mx_tiles_fit(const MxLinearArgs& a) {
 // most: 1x14336x4096 9.6 and 29, 2x1024x4096 4.8 and 15, 4x1024x3584 6.5 and 13 (bf16 6.5 and 5.5).
 inline uint32_t mx_few_tokens(uint32_t type, const MxLinearArgs& a) {
   const auto fits = [&](uint64_t nt) { return a.tokens <= nt && mx_few_bytes(a.cols, nt) <= 60 * 1024; };
+  // 16 rows of a workgroup, whole; tokens are addressed in 64 bits
+  const uint64_t rows = a.rows < 16 ? a.rows : 16;
+  if (!fits(1) && !fits(2) && !fits(4)) return 0;
+  if (!mx_within_reach(rows, a.weight.stride, 1, a.cols / 2) || !mx_within_reach(rows, a.scales.stride, 1, a.cols / 32))
+    return 0;
   if (fits(1) && (type == kTypeF32 || a.rows <= 6144)) return 1;
   if (type == kTypeF32) return fits(2) ? 2 : fits(4) ? 4 : 0;
   return 0;
 }
 
+// A tile, or the kernel without 32-bit offsets where a wavefront's rows or a tile's tokens are too far apart for them:
+// a step of a row is 512 bytes at most.
 inline MxLinearChoice mx_tile(uint32_t type, const MxLinearArgs& a, uint32_t rows, uint32_t ct, uint32_t rg, uint32_t kg) {
+  const uint64_t n = a.rows < rows ? a.rows : rows, t = a.tokens < 32 * ct ? a.tokens : 32 * ct;
+  if (!mx_within_reach(n, a.weight.stride, 1, 512) || !mx_within_reach(n, a.scales.stride, 1, 512) ||
+      !mx_within_reach(t, a.x.stride, type_bytes(type), 512) ||
+      (type == kTypeE4m3 && !mx_within_reach(t, a.x_scales.stride, 1, 512)))
+    return {MxLinearChoice::kSmall, 0, 0, 0, 0, 0, false};
   // the large tile of f32 splits its values on their way, so they may lie anywhere
   const bool raw = type != kTypeF32 || rg == 1;
-  const bool aligned = a.weight.ptr % 16 == 0 && a.weight.stride % 16 == 0 &&
-                       (!raw || (a.x.ptr % 16 == 0 && a.x.stride * type_bytes(type) % 16 == 0));
+  const bool aligned = a.weight.ptr % 16 == 0 && (n <= 1 || a.weight.stride % 16 == 0) &&
+                       (!raw || (a.x.ptr % 16 == 0 && (t <= 1 || a.x.stride * type_bytes(type) % 16 == 0)));
   return {MxLinearChoice::kTiles, 0, rows, ct, rg, kg, aligned};
 }
 
@@ -84,11 +98,8 @@ inline MxLinearChoice choose_mxfp4_linear(uint32_t type, const MxLinearArgs& a) 
   // 4.0 with tiles, 2x1024x96 2.6 and 4.1, 100x1024x512 3.5 and 4.1, 16x4096x256 f32 3.4 and 5.2; 64x4704x512 bf16 (4704
   // steps) 5.5 and 4.8.
   const bool small = a.cols <= 512 && tiles * ((a.cols + 127) / 128) <= 2048;
-  if (mx_tiles_fit(a)) {
-    if (const uint32_t nt = mx_few_tokens(type, a)) return {MxLinearChoice::kFew, nt, 0, 0, 0, 0, false};
-    if (!small) return mx_tile_by_size(type, a);
-  }
-  return {MxLinearChoice::kSmall, 0, 0, 0, 0, 0, false};
+  if (const uint32_t nt = mx_few_tokens(type, a)) return {MxLinearChoice::kFew, nt, 0, 0, 0, 0, false};
+  return small ? MxLinearChoice{MxLinearChoice::kSmall, 0, 0, 0, 0, 0, false} : mx_tile_by_size(type, a);
 }
 
 }  // namespace ptwm

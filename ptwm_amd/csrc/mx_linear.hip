@@ -146,7 +146,7 @@ __device__ __forceinline__ void store4(const MxLinearArgs& a, uint64_t t, uint32
     store4_as<kTypeF32>(a, t, n, v);
 }
 
-// Small products, and rows too far apart for 32-bit offsets: a 16x16 tile of
+// Small products, and rows too far apart for a tile's 32-bit offsets: a 16x16 tile of
 // outputs by one workgroup, whose wavefronts take turns in steps of 128 values
 // (four blocks) along the rows and add up in LDS, operands straight from
 // memory; bound by one way to memory (16x4096x256 bf16 2.8 us).  Lane l
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(256) void mxfp4_linear_kernel(MxLinearArgs a) {
 // What goes to LDS as it is goes by DMA where it lies at multiples of 16 bytes
 // (ALIGNED) and through registers otherwise, to the same places: results do
 // not depend on how operands lie.  Offsets within a tile are 32 bits on top of uniform addresses
-// (mx_tiles_fit()), which is what leaves registers for the operands in flight.
+// (mx_tile()), which is what leaves registers for the operands in flight.
 
 // The place of 16-byte chunk c of row t among rows of S chunks.
 template <uint32_t S>

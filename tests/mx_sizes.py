@@ -44,3 +44,13 @@ SIZES = {
         (640, 4099, 416): tile(64, 1, 4, 1),
     },
 }
+
+
+# A product whose operands may lie as far apart as a tile's 32-bit offsets reach: the rows of each that one tile takes.
+FAR = (20, 40, 2208)
+FAR_COUNTS = {"x": 20, "x_scales": 20, "weight": 32, "scales": 32}
+
+
+def far_stride(operand, size):
+    """The largest stride, in elements of `size` bytes, with which a tile's rows and 512 bytes more lie within 2^32."""
+    return (2**32 - 1 - 512) // size // (FAR_COUNTS[operand] - 1)

@@ -177,3 +177,42 @@ def test_streams_and_graph_replays(kind):
         graph.replay()
         torch.cuda.synchronize()
         assert all(map(torch.equal, results(), first if k % 2 == 0 else second)), k
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("tokens,rows", [(1, 131), (1, 9001), (3, 131), (20, 131)])
+def test_last_tokens_of_sequences(kind, tokens, rows):
+    """hidden[:, -1] of [tokens, 2048, 4096], rows 2^23 elements apart: the same kernel and bits as packed rows."""
+    x, xs, codes, scales = inputs(kind, tokens, rows, 4096, gen(tokens, rows, 4))
+    hidden = torch.zeros(tokens, 2048, 4096, dtype=bytes_of(x).dtype, device=D)
+    hidden[:, -1] = bytes_of(x)
+    last = hidden.view(x.dtype)[:, -1]
+    assert last.stride(0) == 2048 * 4096
+    o, p = torch.empty(tokens, rows, device=D), torch.empty(tokens, rows, device=D)
+    api.mxfp4_linear_cuda(x, codes, scales, o, 0, x_scales=xs)
+    P.check_linear(o, x, xs, codes, scales)
+    api.mxfp4_linear_cuda(last, codes, scales, p, 0, x_scales=xs)
+    assert torch.equal(o, p)
+
+
+@pytest.mark.parametrize("kind,operand", [(k, o) for k in KINDS for o in S.FAR_COUNTS if o != "x_scales" or k == "e4m3"])
+def test_strides_about_the_reach_of_a_tile(kind, operand):
+    x, xs, codes, scales = inputs(kind, *S.FAR, gen(5))
+    o, p = (torch.empty(S.FAR[:2], device=D) for _ in range(2))
+    api.mxfp4_linear_cuda(x, codes, scales, o, 0, x_scales=xs)
+    P.check_linear(o, x, xs, codes, scales)
+    all_ = {"x": x, "weight": codes, "scales": scales, "x_scales": xs}
+    t = all_[operand]
+    stride = S.far_stride(operand, t.element_size())
+    for beyond in (0, 1):
+        big = torch.empty((t.shape[0] - 1) * (stride + beyond) + t.shape[1], dtype=bytes_of(t).dtype, device=D)
+        v = big.as_strided(t.shape, (stride + beyond, 1))
+        v.copy_(bytes_of(t))
+        call = {**all_, operand: v.view(t.dtype)}
+        api.mxfp4_linear_cuda(call["x"], call["weight"], call["scales"], p, 0, x_scales=call["x_scales"])
+        del big, v, call
+        if beyond:
+            P.check_linear(p, x, xs, codes, scales)
+        else:
+            assert torch.equal(o, p)
+    torch.cuda.empty_cache()

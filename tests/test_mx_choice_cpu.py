@@ -70,4 +70,28 @@ def test_alignment(choice, kind):
         assert choice(kind, tokens, rows, cols, w_stride=cols // 2 + 16, x_stride=cols + 16 // size) == (want, True)
         split = kind == "f32" and want[3] == 4  # such tiles take x through registers in any case
         for kw in (dict(x=size), dict(x_stride=cols + 1)):
-            assert choice(kind, tokens, rows, cols, **kw) == (want, split)
+            still = split or (tokens == 1 and "x_stride" in kw)
+            assert choice(kind, tokens, rows, cols, **kw) == (want, still)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_strides(choice, kind):
+    """The stride of a single row changes nothing; others do where a tile's rows pass 32-bit offsets."""
+    size = TYPES[kind][1]
+    huge = 1 << 40
+    for (tokens, rows, cols), want in S.SIZES[kind].items():
+        if tokens == 1:
+            one = choice(kind, tokens, rows, cols)
+            assert one[0] == want and choice(kind, tokens, rows, cols, x_stride=huge + 1, xs_stride=huge + 1) == one
+        assert choice(kind, tokens, rows, cols, x_stride=1 << 24, xs_stride=1 << 24, w_stride=1 << 24)[0] == want
+    one = choice(kind, 70, 1, 4096)
+    assert one[0][0] == S.TILES and choice(kind, 70, 1, 4096, w_stride=huge + 1, s_stride=huge + 1) == one
+    want = choice(kind, *S.FAR)[0]
+    assert want[:2] == (S.TILES, 32)
+    for operand, key, n in (("x", "x_stride", size), ("x_scales", "xs_stride", 1), ("weight", "w_stride", 1),
+                            ("scales", "s_stride", 1)):
+        if operand == "x_scales" and kind != "e4m3":
+            continue
+        last = S.far_stride(operand, n)
+        assert choice(kind, *S.FAR, **{key: last})[0] == want
+        assert choice(kind, *S.FAR, **{key: last + 1})[0] == (S.SMALL,)
