@@ -222,7 +222,7 @@ bool mx_rows(const MxRows& r, uint64_t rows, uint64_t cols) { return r.ptr && (r
 
 int64_t mx_launched(hipError_t e) { return e == hipSuccess ? kOk : kInternal; }
 
-// Rows and columns that 32-bit grids and column indexes hold.
+// Rows and columns that 32-bit indexes hold.
 constexpr uint64_t kMxMaxRows = 0x7FFFFFFF, kMxMaxCols = 1u << 30;
 
 // Host-buffer entry points stage through device memory on device 0.

@@ -143,10 +143,10 @@ __device__ __forceinline__ float exp_of_minus(float g) {
 template <uint32_t T>
 __global__ __launch_bounds__(kThreads) void swiglu_mx_kernel(MxSwigluArgs a) {
   const uint32_t per_row = a.cols / 8;
-  const uint64_t at = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
+  const uint32_t at = blockIdx.x * kThreads + threadIdx.x;
   const uint64_t row = at / per_row;
   if (row >= a.rows) return;
-  const uint64_t c = (at - row * per_row) * 8;
+  const uint32_t c = at % per_row * 8;
   float g[8], u[8];
   load8<T>(a.gate.ptr + (row * a.gate.stride + c) * type_bytes(T), g);
   load8<T>(a.up.ptr + (row * a.up.stride + c) * type_bytes(T), u);
@@ -161,8 +161,15 @@ __global__ __launch_bounds__(kThreads) void swiglu_mx_kernel(MxSwigluArgs a) {
 
 template <uint32_t T, int W, int CH>
 hipError_t norm_by(const MxNormArgs& a, hipStream_t stream) {
-  constexpr int kRows = W > 4 ? 1 : 4 / W;
-  return launch(rms_norm_mx_kernel<T, W, CH>, (a.rows + kRows - 1) / kRows, W > 4 ? 64 * W : kThreads, a, stream);
+  constexpr uint32_t kRows = W > 4 ? 1 : 4 / W, kGroup = W > 4 ? 64 * W : kThreads, kSize = type_bytes(T);
+  return in_parts(a.rows, kMaxThreads / kGroup * kRows, [&](uint64_t first, uint64_t rows) {
+    MxNormArgs p = a;
+    p.x = rows_from(a.x, first, kSize), p.residual = rows_from(a.residual, first, kSize);
+    p.sum = rows_from(a.sum, first, kSize);
+    p.codes = rows_from(a.codes, first, 1), p.scales = rows_from(a.scales, first, 1);
+    p.rows = rows;
+    return launch(rms_norm_mx_kernel<T, W, CH>, (rows + kRows - 1) / kRows, kGroup, p, stream);
+  });
 }
 
 template <uint32_t T>
@@ -178,6 +185,16 @@ hipError_t norm_of(const MxNormArgs& a, hipStream_t stream) {
   return norm_by<T, 16, 0>(a, stream);
 }
 
+template <uint32_t T>
+hipError_t swiglu_of(const MxSwigluArgs& a, hipStream_t stream) {
+  const uint32_t per_row = a.cols / 8;
+  return in_parts(a.rows, (kMaxThreads - kThreads) / per_row, [&](uint64_t first, uint64_t rows) {
+    const MxSwigluArgs p{rows_from(a.gate, first, type_bytes(T)), rows_from(a.up, first, type_bytes(T)),
+                         rows_from(a.codes, first, 1), rows_from(a.scales, first, 1), rows, a.cols};
+    return launch(swiglu_mx_kernel<T>, (rows * per_row + kThreads - 1) / kThreads, kThreads, p, stream);
+  });
+}
+
 }  // namespace
 
 hipError_t launch_rms_norm_mx(uint32_t type, const MxNormArgs& a, hipStream_t stream) {
@@ -190,11 +207,10 @@ hipError_t launch_rms_norm_mx(uint32_t type, const MxNormArgs& a, hipStream_t st
 }
 
 hipError_t launch_swiglu_mx(uint32_t type, const MxSwigluArgs& a, hipStream_t stream) {
-  const uint64_t groups = (a.rows * (a.cols / 8) + kThreads - 1) / kThreads;
   switch (type) {
-    case kTypeF32: return launch(swiglu_mx_kernel<kTypeF32>, groups, kThreads, a, stream);
-    case kTypeF16: return launch(swiglu_mx_kernel<kTypeF16>, groups, kThreads, a, stream);
-    case kTypeBf16: return launch(swiglu_mx_kernel<kTypeBf16>, groups, kThreads, a, stream);
+    case kTypeF32: return swiglu_of<kTypeF32>(a, stream);
+    case kTypeF16: return swiglu_of<kTypeF16>(a, stream);
+    case kTypeBf16: return swiglu_of<kTypeBf16>(a, stream);
     default: return hipErrorInvalidValue;
   }
 }

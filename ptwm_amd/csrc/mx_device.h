@@ -6,14 +6,32 @@
 
 namespace ptwm {
 
+// A launch holds fewer than 2^32 threads: what goes past them would not run, and no error would say so.
+constexpr uint64_t kMaxThreads = 0xFFFFFFFF;
+
 // One launch with one argument; the triple chevrons' way keeps a stack of configurations besides.
 template <typename A>
 hipError_t launch(void (*kernel)(A), uint64_t groups, uint32_t threads, const A& a, hipStream_t stream,
                   uint32_t shared = 0) {
-  if (groups > 0x7FFFFFFFu) return hipErrorInvalidValue;
+  if (groups > kMaxThreads / threads) return hipErrorInvalidValue;
   void* args[] = {const_cast<A*>(&a)};
   return hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3((uint32_t)groups), dim3(threads), args, shared,
                          stream);
+}
+
+// The rows of an operand from row `first` on.
+inline MxRows rows_from(const MxRows& r, uint64_t first, uint32_t element) {
+  return {r.ptr ? r.ptr + first * r.stride * element : 0, r.stride};
+}
+
+// Calls f(first, count) for parts of `most` rows, one after the other, until all are served or one fails.
+template <typename F>
+hipError_t in_parts(uint64_t rows, uint64_t most, F&& f) {
+  for (uint64_t first = 0; first < rows; first += most) {
+    const hipError_t e = f(first, rows - first < most ? rows - first : most);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));

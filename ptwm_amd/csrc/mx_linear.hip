@@ -759,19 +759,49 @@ __global__ __launch_bounds__(64 * kFewWaves) void mxfp4_linear_few_kernel(MxLine
   }
 }
 
+// The outputs of rows first .. first + rows - 1, and of tokens.
+MxLinearArgs some_rows(const MxLinearArgs& a, uint64_t first, uint64_t rows) {
+  MxLinearArgs p = a;
+  const uint64_t skip = first * type_bytes(a.out_type);
+  p.weight = rows_from(a.weight, first, 1), p.scales = rows_from(a.scales, first, 1);
+  p.out.ptr += skip, p.bias = a.bias ? a.bias + skip : 0;
+  p.rows = (uint32_t)rows;
+  return p;
+}
+template <uint32_t T>
+MxLinearArgs some_tokens(const MxLinearArgs& a, uint64_t first, uint64_t tokens) {
+  MxLinearArgs p = a;
+  p.x = rows_from(a.x, first, type_bytes(T)), p.x_scales = rows_from(a.x_scales, first, 1);
+  p.out = rows_from(a.out, first, type_bytes(a.out_type));
+  p.tokens = tokens;
+  return p;
+}
+
+// Workgroups of TR rows and TT tokens each, rows first, in as few launches as hold them.
+template <uint32_t T, uint32_t TR, uint32_t TT>
+hipError_t launch_tiles(void (*kernel)(MxLinearArgs), uint32_t threads, const MxLinearArgs& a, hipStream_t stream,
+                        uint32_t shared = 0) {
+  const uint64_t most = kMaxThreads / threads;
+  return in_parts(a.rows, most * TR, [&](uint64_t row, uint64_t rows) {
+    const uint64_t row_tiles = (rows + TR - 1) / TR;
+    return in_parts(a.tokens, most / row_tiles * TT, [&](uint64_t token, uint64_t tokens) {
+      return launch(kernel, row_tiles * ((tokens + TT - 1) / TT), threads,
+                    some_tokens<T>(some_rows(a, row, rows), token, tokens), stream, shared);
+    });
+  });
+}
+
 template <uint32_t T, int ROWS, int CT, int RG, int KG, bool RAW>
 hipError_t tiles_of(const MxLinearArgs& a, bool aligned, hipStream_t stream) {
-  constexpr uint32_t kRows = ROWS * RG, kTokens = 32 * CT;
-  const uint64_t tiles = (uint64_t)((a.rows + kRows - 1) / kRows) * ((a.tokens + kTokens - 1) / kTokens);
-  return launch(aligned ? mxfp4_linear_tiles_kernel<T, ROWS, CT, RG, KG, RAW, true>
-                        : mxfp4_linear_tiles_kernel<T, ROWS, CT, RG, KG, RAW, false>,
-                tiles, 64 * RG * KG, a, stream);
+  return launch_tiles<T, ROWS * RG, 32 * CT>(aligned ? mxfp4_linear_tiles_kernel<T, ROWS, CT, RG, KG, RAW, true>
+                                                     : mxfp4_linear_tiles_kernel<T, ROWS, CT, RG, KG, RAW, false>,
+                                             64 * RG * KG, a, stream);
 }
 
 template <uint32_t T, int NT>
 hipError_t few_of(const MxLinearArgs& a, hipStream_t stream) {
-  return launch(mxfp4_linear_few_kernel<T, NT>, (a.rows + 15) / 16, 64 * kFewWaves, a, stream,
-                (uint32_t)mx_few_bytes(a.cols, NT));
+  return launch_tiles<T, 16, NT>(mxfp4_linear_few_kernel<T, NT>, 64 * kFewWaves, a, stream,
+                                 (uint32_t)mx_few_bytes(a.cols, NT));
 }
 
 template <uint32_t T>
@@ -805,8 +835,7 @@ hipError_t linear_of(const MxLinearArgs& a, hipStream_t stream) {
       if (is(64, 2, 1, 4)) return tiles_of<T, 64, 2, 1, 4, true>(a, k.aligned, stream);
     return hipErrorInvalidValue;
   }
-  const uint64_t tiles = (uint64_t)((a.rows + 15) / 16) * ((a.tokens + 15) / 16);
-  return launch(mxfp4_linear_kernel<T>, tiles, 256, a, stream);
+  return launch_tiles<T, 16, 16>(mxfp4_linear_kernel<T>, 256, a, stream);
 }
 
 }  // namespace
