@@ -125,13 +125,14 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : kThreads) void rms_norm_mx_kernel(
 // y = gate / (1 + exp(-gate)) * up in 32 bits.  The exponential and the
 // reciprocal are the hardware's, each within a unit in the last place: with
 // the library's exact forms the arithmetic took longer than the memory
-// (2048x14336 bf16: 35 us, 29.6 this way).  The exponential's argument,
+// (2048x14336 bf16: 35 us, 28 to 29.5 this way).  The exponential's argument,
 // -gate * log2(e), is carried in two parts, whose low one is multiplied in
 // afterwards: rounded to 32 bits alone it puts the exponential off by half a
 // unit for every unit of |gate| (the result by 65 * 2^-24 at gate = -87).
-// From |gate| = 1 on, gate and the reciprocal's argument are taken a quarter
-// of, so that the reciprocal stays a normal number as far as the exponential
-// is finite; smaller gates, which may have no quarter, are taken as they are.
+// The reciprocal's argument is a quarter of the sum, so that it stays a normal
+// number as far as the exponential is finite, and the other quarter is taken
+// of the reciprocal: a gate below the normal numbers may have none.  (Below
+// gate = -87.3 that takes it below them itself, up to 4 * 2^-24.)
 __device__ __forceinline__ float exp_of_minus(float g) {
   constexpr float kHigh = -0x1.715476p+0f, kLow = -0x1.4ae0c0p-26f;  // -log2(e) = kHigh + kLow
   const float t = g * kHigh;
@@ -143,18 +144,17 @@ __device__ __forceinline__ float exp_of_minus(float g) {
 template <uint32_t T>
 __global__ __launch_bounds__(kThreads) void swiglu_mx_kernel(MxSwigluArgs a) {
   const uint32_t per_row = a.cols / 8;
-  const uint32_t at = blockIdx.x * kThreads + threadIdx.x;
+  const uint64_t at = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
   const uint64_t row = at / per_row;
   if (row >= a.rows) return;
-  const uint32_t c = at % per_row * 8;
+  const uint64_t c = (at - row * per_row) * 8;
   float g[8], u[8];
   load8<T>(a.gate.ptr + (row * a.gate.stride + c) * type_bytes(T), g);
   load8<T>(a.up.ptr + (row * a.up.stride + c) * type_bytes(T), u);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float e = exp_of_minus(g[i]);
-    const float k = __builtin_fabsf(g[i]) < 1.0f ? 1.0f : 0.25f;
-    g[i] = g[i] * k * __builtin_amdgcn_rcpf(__builtin_fmaf(e, k, k)) * u[i];
+    g[i] = __builtin_amdgcn_rcpf(__builtin_fmaf(e, 0.25f, 0.25f)) * 0.25f * g[i] * u[i];
   }
   store_codes(a.codes, a.scales, row, c, g);
 }
