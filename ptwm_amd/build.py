@@ -7,6 +7,7 @@ Always recompiles every source: the caller asked for a build.
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import subprocess
 import sys
@@ -79,18 +80,24 @@ def _link_mx(obj: str) -> None:
 
 
 def build(verbose: bool = False) -> str:
+    """Builds the library, and after it the module of the MX operators where torch is there to compile it against."""
     os.makedirs(OBJ, exist_ok=True)
+    with_mx = importlib.util.find_spec("torch") is not None
     with cf.ThreadPoolExecutor(max_workers=min(8, len(SOURCES))) as ex:
-        mx = ex.submit(_compile_mx)
+        mx = ex.submit(_compile_mx) if with_mx else None
         objs = list(ex.map(_compile, SOURCES))
-        mx_obj = mx.result()
     tmp = LIB + ".tmp"
     cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp, *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stderr}")
     os.replace(tmp, LIB)
-    _link_mx(mx_obj)
+    if mx is not None:
+        _link_mx(mx.result())
+    else:
+        if os.path.exists(MX):
+            os.remove(MX)
+        print("no torch: the Python entry points of the MX operators are not built", file=sys.stderr)
     if verbose:
         print(f"built {LIB}")
     return LIB
