@@ -76,6 +76,7 @@ void check_place(const at::Tensor& t, const char* name, int64_t device, const Ty
     for (at::ScalarType s : types) list += (list.empty() ? "" : ", ") + std::string(c10::toString(s));
     fail(PyExc_TypeError, "%s: dtype %s is not one of %s", name, c10::toString(t.scalar_type()), list.c_str());
   }
+  if (t.is_neg()) fail(PyExc_ValueError, "%s: a lazily negated view, resolve it first (Tensor.resolve_neg)", name);
   if (!t.is_cuda()) fail(PyExc_ValueError, "%s: tensor is not on a GPU device", name);
   if (t.get_device() != device)
     fail(PyExc_ValueError, "%s: tensor is on device %d, call names device %lld", name, (int)t.get_device(),
