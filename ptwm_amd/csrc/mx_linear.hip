@@ -465,7 +465,11 @@ void mxfp4_linear_tiles_kernel(MxLinearArgs a) {
           // Large tiles spread the next step's requests over the first half of the products: all at once they hold the
           // wavefront up, and its products with it, until the address unit has taken them (512x14336x4096 bf16: 71 us,
           // 62 this way).  Where the weights' way from memory is what takes time they go out at once.
-          constexpr int kOver = (RG > 1 ? 4 : 1) * kParts;
+          // What comes through registers is spread over all of them, which holds fewer registers at a time: over the
+          // first half 54 of bf16's, 23 of f16's and 5 of e4m3's went to scratch memory, this way 14, 15 and none
+          // (unaligned 2048x14336x4096 bf16 346 us -> 251, f16 352 -> 309, e4m3 223 -> 221; with half the wavefronts
+          // a SIMD, none at all, 280, 355, 244).
+          constexpr int kOver = (RG > 1 ? ALIGNED ? 4 : 8 : 1) * kParts;
 #pragma unroll
           for (int k = v * kRequests / kOver; k < (v + 1) * kRequests / kOver && k < kRequests; ++k) request(k, q, next);
         }
