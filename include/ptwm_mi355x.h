@@ -390,8 +390,8 @@ int64_t ptwm_mi355x_last_kernel_ms(uint32_t device_ordinal, float *out3);
  *
  * These calls differ from the codec's in one way: they queue their work on
  * `stream` (a hipStream_t of the device, 0 = the null stream) and return
- * without waiting for it.  They hold no state, lock, workspace or scratch,
- * allocate nothing, and may be captured into a graph.  Addresses need the
+ * without waiting for it.  They hold no state, lock or workspace, allocate
+ * nothing, and may be captured into a graph.  Addresses need the
  * alignment of their elements only; strides are between rows, in elements
  * (weights and scales: bytes).  dtypes are public dtype codes (dtype.rs:79-103):
  * 1 float32, 4 float16, 6 bfloat16, 29 float8_e4m3fn.  cols is a multiple of
@@ -425,7 +425,9 @@ int64_t ptwm_mi355x_swiglu_mx_cuda(uint32_t dtype, uint64_t gate, uint64_t gate_
  * float8_e4m3fn with x_scales (tokens x cols/32 bytes; 0 for the others).
  * bias (0: none) has out's dtype.  Weights and activations are taken exactly,
  * down to 2^-133; a code times its scale of 2^128 or more counts as infinite,
- * and its sums as infinite or NaN. */
+ * and its sums as infinite or NaN.  The order of a sum's additions depends on
+ * the sizes, the types and, where operands' rows lie gigabytes apart, on the
+ * strides; with float16 it depends on the scales of neighbouring rows too. */
 int64_t ptwm_mi355x_mxfp4_linear_cuda(uint32_t x_dtype, uint64_t x, uint64_t x_stride, uint64_t x_scales,
                                       uint64_t x_scales_stride, uint64_t weight, uint64_t weight_stride,
                                       uint64_t scales, uint64_t scales_stride, uint32_t out_dtype, uint64_t bias,
