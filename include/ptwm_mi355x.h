@@ -390,9 +390,7 @@ int64_t ptwm_mi355x_last_kernel_ms(uint32_t device_ordinal, float *out3);
  *
  * These calls differ from the codec's in one way: they queue their work on
  * `stream` (a hipStream_t of the device, 0 = the null stream) and return
- * without waiting for it.  They hold no state, lock or workspace, allocate
- * nothing, and may be captured into a graph.  Addresses need the
- * alignment of their elements only; strides are between rows, in elements
+X strides are between rows, in elements
  * (weights and scales: bytes).  dtypes are public dtype codes (dtype.rs:79-103):
  * 1 float32, 4 float16, 6 bfloat16, 29 float8_e4m3fn.  cols is a multiple of
  * 32.  Returns 0; -1 for arguments that do not fit together (nothing is
@@ -433,6 +431,76 @@ int64_t ptwm_mi355x_mxfp4_linear_cuda(uint32_t x_dtype, uint64_t x, uint64_t x_s
                                       uint64_t scales, uint64_t scales_stride, uint32_t out_dtype, uint64_t bias,
                                       uint64_t out, uint64_t out_stride, uint64_t tokens, uint64_t rows,
                                       uint64_t cols, uint64_t stream, uint32_t device_ordinal);
+
+/* Codes and scales of x (float32, float16 or bfloat16) in MXFP4: codes
+ * receives rows x cols/2 bytes, scales rows x cols/32.  A block whose largest
+ * magnitude is m takes the scale byte b = floor(log2 m) + 125 with saturate
+ * != 0 (m / 2^(b-127) is in [4, 8), and what is above 6, e2m1's largest value,
+ * becomes 6), or the smallest b with which nothing is above 6 (saturate 0); at
+ * least 0, a block of zeros included.  Codes are rounded to nearest, ties to
+ * even, and keep the sign of zeros.  A block that holds an infinity or NaN
+ * gets the scale 255 and zero codes. */
+int64_t ptwm_mi355x_mxfp4_quantise_cuda(uint32_t dtype, uint64_t x, uint64_t x_stride, uint64_t codes,
+                                        uint64_t codes_stride, uint64_t scales, uint64_t scales_stride, uint64_t rows,
+                                        uint64_t cols, uint32_t saturate, uint64_t stream, uint32_t device_ordinal);
+
+/* out[t, n] = sum over k of x[t, k] * weight[n, k] (+ bias[n]) with both
+ * matrices in MXFP4: x and weight rows of cols/2 bytes of codes, x_scales and
+ * scales rows of cols/32 bytes.  Products are exact, sums in 32 bits, with one
+ * rounding to out_dtype.  bias (0: none) has out's dtype.  The order of a sum's
+ * additions depends on the sizes and, where operands' rows lie gigabytes
+ * apart, on the strides. */
+int64_t ptwm_mi355x_mxfp4_matmul_cuda(uint64_t x, uint64_t x_stride, uint64_t x_scales, uint64_t x_scales_stride,
+                                      uint64_t weight, uint64_t weight_stride, uint64_t scales,
+                                      uint64_t scales_stride, uint32_t out_dtype, uint64_t bias, uint64_t out,
+                                      uint64_t out_stride, uint64_t tokens, uint64_t rows, uint64_t cols,
+                                      uint64_t stream, uint32_t device_ordinal);
+
+/* The weights of all experts for one product: rows of MXFP4 codes and their
+ * scales, with the bytes between rows and between experts, and a bias of the
+ * output's dtype (0: none) with the elements between its values (bias_stride)
+ * and between experts. */
+typedef struct ptwm_mi355x_experts {
+  uint64_t codes, codes_stride, codes_expert;
+  uint64_t scales, scales_stride, scales_expert;
+  uint64_t bias, bias_stride, bias_expert;
+} ptwm_mi355x_experts;
+
+/* A mixture-of-experts layer on MXFP4 experts.  For every token t:
+ *   logits[e] = sum over k of x[t, k] * router[e, k] (+ router_bias[e]);
+ *   the top_k largest are chosen, the lowest e of equal ones (NaN counts as
+ *   the largest), with p = softmax over them;
+ *   out[t] = sum over chosen e of p[e] * (down_e h + down_bias_e),
+ *   h = g / (1 + exp(-g)) * u, g = gate_e x[t] + gate_bias_e, u likewise.
+ * gate and up: `inner` rows of `cols` values an expert; down: `cols` rows of
+ * `inner` values.  An expert whose logit is minus infinity takes no part and
+ * has the weight 0 (a token with no other expert: zeros).  Logits are summed
+ * in 64 bits, so that the choice does not depend on an order of additions;
+ * other sums are in 32 bits, and h has 16 significant bits at least (24 where
+ * out is float32).  x, router and out are float32, float16 or bfloat16 each;
+ * router_bias has router_dtype.  out may be x itself.
+ * experts_out (int32) and weights_out (float32), tokens x top_k each and 0
+ * where not wanted, receive the choice, largest logits first, and p.
+ * Meant for a few tokens: calls of more than 64 take several passes over the
+ * weights.  1 <= top_k <= 32, top_k <= experts <= 1024; cols and inner are
+ * multiples of 32, 131072 at most.
+ * workspace: device memory of at least workspace_bytes >=
+ * ptwm_mi355x_mxfp4_moe_workspace() bytes at a multiple of 256, which the call
+ * overwrites and which nothing else may use until it is done: calls that may
+ * run at the same time (on two streams, from two graphs) take one each. */
+typedef struct ptwm_mi355x_mxfp4_moe {
+  uint64_t x, x_stride, router, router_stride, router_bias, out, out_stride;
+  ptwm_mi355x_experts gate, up, down;
+  uint64_t experts_out, weights_out;
+  uint64_t workspace, workspace_bytes;
+  uint64_t tokens, experts, top_k, cols, inner;
+  uint32_t x_dtype, router_dtype, out_dtype, reserved; /* reserved: 0 */
+} ptwm_mi355x_mxfp4_moe;
+
+/* Bytes of workspace that the call takes (its addresses are not looked at), or
+ * -1 / -5 as the call. */
+int64_t ptwm_mi355x_mxfp4_moe_workspace(const ptwm_mi355x_mxfp4_moe *call);
+int64_t ptwm_mi355x_mxfp4_moe_cuda(const ptwm_mi355x_mxfp4_moe *call, uint64_t stream, uint32_t device_ordinal);
 
 #ifdef __cplusplus
 }

@@ -26,9 +26,28 @@ _RC_NAMES = {
     -5: "Unsupported",
 }
 
-# every symbol the header declares, with its ctypes signature
 _u8p = C.c_void_p
 _u64 = C.c_uint64
+
+
+class Experts(C.Structure):
+    """ptwm_mi355x_experts (include/ptwm_mi355x.h)."""
+    _fields_ = [(n, _u64) for n in ("codes", "codes_stride", "codes_expert", "scales", "scales_stride",
+                                    "scales_expert", "bias", "bias_stride", "bias_expert")]
+
+
+class Mxfp4Moe(C.Structure):
+    """ptwm_mi355x_mxfp4_moe (include/ptwm_mi355x.h)."""
+    _fields_ = [
+        *((n, _u64) for n in ("x", "x_stride", "router", "router_stride", "router_bias", "out", "out_stride")),
+        ("gate", Experts), ("up", Experts), ("down", Experts),
+        *((n, _u64) for n in ("experts_out", "weights_out", "workspace", "workspace_bytes", "tokens", "experts",
+                              "top_k", "cols", "inner")),
+        *((n, C.c_uint32) for n in ("x_dtype", "router_dtype", "out_dtype", "reserved")),
+    ]
+
+
+# every symbol the header declares, with its ctypes signature
 _SIGS = {
     "ptwm_plane_codec_v1_encode": (C.c_int64, [_u8p, C.c_size_t, _u8p, C.c_size_t]),
     "ptwm_plane_codec_v1_decode": (C.c_int64, [_u8p, C.c_size_t, _u8p, C.c_size_t]),
@@ -95,6 +114,10 @@ _SIGS = {
     "ptwm_mi355x_swiglu_mx_cuda": (C.c_int64, [C.c_uint32] + [_u64] * 11 + [C.c_uint32]),
     "ptwm_mi355x_mxfp4_linear_cuda": (
         C.c_int64, [C.c_uint32] + [_u64] * 8 + [C.c_uint32] + [_u64] * 7 + [C.c_uint32]),
+    "ptwm_mi355x_mxfp4_quantise_cuda": (C.c_int64, [C.c_uint32] + [_u64] * 8 + [C.c_uint32, _u64, C.c_uint32]),
+    "ptwm_mi355x_mxfp4_matmul_cuda": (C.c_int64, [_u64] * 8 + [C.c_uint32] + [_u64] * 7 + [C.c_uint32]),
+    "ptwm_mi355x_mxfp4_moe_workspace": (C.c_int64, [C.POINTER(Mxfp4Moe)]),
+    "ptwm_mi355x_mxfp4_moe_cuda": (C.c_int64, [C.POINTER(Mxfp4Moe), _u64, C.c_uint32]),
 }
 
 

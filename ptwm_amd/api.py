@@ -499,12 +499,13 @@ def container_write(tensors, layout: str = "compact", payloads=None, as_array: b
 
 
 # Operators on microscaled (MX) blocks: what a program does with the MXFP4
-# tensors that a decode restored (library additions).  Unlike the codec calls
+# tensors that a decode restored, or before it codes them (library additions).  Unlike the codec calls
 # they queue their work on torch's current stream and return without waiting
 # for it, as torch's own operators do.  Their checks are native
 # (csrc/mx_python.cpp), because the smallest calls cost the host more than the
 # GPU; the module, which needs torch, is loaded at their first use.
-_MX = ("rms_norm_mx_cuda", "swiglu_mx_cuda", "mxfp4_linear_cuda")
+_MX = ("rms_norm_mx_cuda", "swiglu_mx_cuda", "mxfp4_linear_cuda", "mxfp4_quantise_cuda", "mxfp4_matmul_cuda",
+       "mxfp4_moe_cuda")
 
 
 def __getattr__(name: str):

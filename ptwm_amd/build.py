@@ -21,7 +21,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["transform.hip", "decode_exact.hip", "decode_sync.hip", "zstd_device.hip", "o1sac_device.hip", "huff_ilv.hip", "rans_ilv.hip", "ilv_host.hip", "rans_host.hip", "huffman_host.cpp", "code_tables.hip", "runtime.hip", "plane_ops.hip",
            "ref_encode.hip", "integrity.hip", "hash_host.hip", "xxh64_host.cpp", "container.cpp", "container_write.cpp", "blake3_host.cpp", "plan_parse.cpp",
-           "mx_activations.hip", "mx_linear.hip", "abi.hip"]
+           "mx_activations.hip", "mx_linear.hip", "mx_quantise.hip", "mx_matmul.hip", "mx_moe.hip", "abi.hip"]
 
 CFLAGS = [
     "--offload-arch=gfx950",

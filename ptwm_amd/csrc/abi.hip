@@ -225,6 +225,29 @@ int64_t mx_launched(hipError_t e) { return e == hipSuccess ? kOk : kInternal; }
 // Rows and columns that 32-bit indexes hold.
 constexpr uint64_t kMxMaxRows = 0x7FFFFFFF, kMxMaxCols = 1u << 30;
 
+// The experts' weights of one product; a stack of several experts lies where its strides say.
+bool mx_experts(const MxExperts& w, uint64_t rows, uint64_t cols) {
+  return mx_rows(w.codes, rows, cols / 2) && mx_rows(w.scales, rows, cols / kMxBlock);
+}
+MxExperts mx_experts_of(const ptwm_mi355x_experts& w) {
+  return {{w.codes, w.codes_stride}, {w.scales, w.scales_stride}, w.codes_expert, w.scales_expert, w.bias,
+          w.bias_expert, w.bias_stride};
+}
+// A call's sizes and dtypes, which its workspace depends on.
+int64_t mx_moe_sizes(const ptwm_mi355x_mxfp4_moe* c, MxMoeArgs& a) {
+  if (!c || c->reserved) return kInvalidInput;
+  if (!mx_float(c->x_dtype) || !mx_float(c->router_dtype) || !mx_float(c->out_dtype)) return kUnsupported;
+  const auto width = [](uint64_t n) { return n > 0 && n <= kMoeMaxWidth && n % kMxBlock == 0; };
+  if (c->tokens > kMxMaxRows || c->experts > kMoeMaxExperts || c->top_k == 0 || c->top_k > kMoeMaxTopK ||
+      c->top_k > c->experts || !width(c->cols) || !width(c->inner))
+    return kInvalidInput;
+  a = {};
+  a.tokens = c->tokens, a.experts = (uint32_t)c->experts, a.top_k = (uint32_t)c->top_k;
+  a.cols = (uint32_t)c->cols, a.inner = (uint32_t)c->inner;
+  a.x_type = c->x_dtype, a.router_type = c->router_dtype, a.out_type = c->out_dtype;
+  return kOk;
+}
+
 // Host-buffer entry points stage through device memory on device 0.
 constexpr uint32_t kHostDevice = 0;
 
@@ -1164,6 +1187,65 @@ int64_t ptwm_mi355x_mxfp4_linear_cuda(uint32_t x_dtype, uint64_t x, uint64_t x_s
   OnDevice on(device_ordinal);
   if (!on.ok) return kInvalidInput;
   return mx_launched(launch_mxfp4_linear(x_dtype, a, reinterpret_cast<hipStream_t>(stream)));
+}
+
+int64_t ptwm_mi355x_mxfp4_quantise_cuda(uint32_t dtype, uint64_t x, uint64_t x_stride, uint64_t codes,
+                                        uint64_t codes_stride, uint64_t scales, uint64_t scales_stride, uint64_t rows,
+                                        uint64_t cols, uint32_t saturate, uint64_t stream, uint32_t device_ordinal) {
+  if (!mx_float(dtype)) return kUnsupported;
+  if (rows > kMxMaxRows || cols == 0 || cols > kMxMaxCols || cols % kMxBlock) return kInvalidInput;
+  if (rows == 0) return kOk;
+  const MxQuantiseArgs a{{x, x_stride}, {codes, codes_stride}, {scales, scales_stride}, rows, (uint32_t)cols,
+                         saturate != 0};
+  if (!mx_rows(a.x, rows, cols) || !mx_rows(a.codes, rows, cols / 2) || !mx_rows(a.scales, rows, cols / kMxBlock))
+    return kInvalidInput;
+  OnDevice on(device_ordinal);
+  if (!on.ok) return kInvalidInput;
+  return mx_launched(launch_mxfp4_quantise(dtype, a, reinterpret_cast<hipStream_t>(stream)));
+}
+
+int64_t ptwm_mi355x_mxfp4_matmul_cuda(uint64_t x, uint64_t x_stride, uint64_t x_scales, uint64_t x_scales_stride,
+                                      uint64_t weight, uint64_t weight_stride, uint64_t scales,
+                                      uint64_t scales_stride, uint32_t out_dtype, uint64_t bias, uint64_t out,
+                                      uint64_t out_stride, uint64_t tokens, uint64_t rows, uint64_t cols,
+                                      uint64_t stream, uint32_t device_ordinal) {
+  if (!mx_float(out_dtype)) return kUnsupported;
+  if (tokens > kMxMaxRows || rows > kMxMaxRows || cols == 0 || cols > kMxMaxCols || cols % kMxBlock)
+    return kInvalidInput;
+  if (tokens == 0 || rows == 0) return kOk;
+  const MxLinearArgs a{{x, x_stride}, {x_scales, x_scales_stride}, {weight, weight_stride}, {scales, scales_stride},
+                       {out, out_stride}, bias, tokens, (uint32_t)rows, (uint32_t)cols, out_dtype};
+  if (!mx_rows(a.x, tokens, cols / 2) || !mx_rows(a.x_scales, tokens, cols / kMxBlock) ||
+      !mx_rows(a.weight, rows, cols / 2) || !mx_rows(a.scales, rows, cols / kMxBlock) || !mx_rows(a.out, tokens, rows))
+    return kInvalidInput;
+  OnDevice on(device_ordinal);
+  if (!on.ok) return kInvalidInput;
+  return mx_launched(launch_mxfp4_matmul(a, reinterpret_cast<hipStream_t>(stream)));
+}
+
+int64_t ptwm_mi355x_mxfp4_moe_workspace(const ptwm_mi355x_mxfp4_moe* call) {
+  MxMoeArgs a;
+  const int64_t rc = mx_moe_sizes(call, a);
+  return rc != kOk ? rc : (int64_t)mxfp4_moe_workspace(a);
+}
+
+int64_t ptwm_mi355x_mxfp4_moe_cuda(const ptwm_mi355x_mxfp4_moe* call, uint64_t stream, uint32_t device_ordinal) {
+  MxMoeArgs a;
+  const int64_t rc = mx_moe_sizes(call, a);
+  if (rc != kOk) return rc;
+  if (a.tokens == 0) return kOk;
+  a.x = {call->x, call->x_stride}, a.router = {call->router, call->router_stride};
+  a.out = {call->out, call->out_stride}, a.router_bias = call->router_bias;
+  a.gate = mx_experts_of(call->gate), a.up = mx_experts_of(call->up), a.down = mx_experts_of(call->down);
+  a.experts_out = call->experts_out, a.weights_out = call->weights_out, a.workspace = call->workspace;
+  if (!mx_rows(a.x, a.tokens, a.cols) || !mx_rows(a.router, a.experts, a.cols) ||
+      !mx_rows(a.out, a.tokens, a.cols) || !mx_experts(a.gate, a.inner, a.cols) ||
+      !mx_experts(a.up, a.inner, a.cols) || !mx_experts(a.down, a.cols, a.inner) || !a.workspace ||
+      a.workspace % 256 || call->workspace_bytes < mxfp4_moe_workspace(a))
+    return kInvalidInput;
+  OnDevice on(device_ordinal);
+  if (!on.ok) return kInvalidInput;
+  return mx_launched(launch_mxfp4_moe(a, reinterpret_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -31,64 +31,9 @@ namespace {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-// bf16 parts that hold a value of type T exactly.
-constexpr int parts_of(uint32_t type) { return type == kTypeF32 ? 3 : type == kTypeF16 ? 2 : 1; }
-
-__device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t w, float scale, bool high) {
-  return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))
-              : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
-}
-
-// Eight values as bf16 parts, each cut from what the ones before it leave
-// (truncation, so nothing rounds up to infinity).  The parts before the last
-// are finite, so an infinity or NaN is the last one, where it stays what it
-// is: NaN's highest mantissa bit is set by the subtraction.  scale: of e4m3
-// codes, read for its exponent only (byte 0 is 2^-127, 255 is NaN).
-constexpr float kBf16Max = 0x1.FEp127f;
-template <uint32_t T>
-__device__ __forceinline__ void parts_of_raw(const Raw8<T>& r, float scale, u32x4 (&p)[parts_of(T)]) {
-  if constexpr (T == kTypeBf16) {
-    p[0] = r.w[0];
-  } else if constexpr (T == kTypeE4m3) {
-    const uint32_t lo = (uint32_t)r.w, hi = (uint32_t)(r.w >> 32);
-    p[0] = u32x4_make(bf16_of_e4m3(lo, scale, false), bf16_of_e4m3(lo, scale, true), bf16_of_e4m3(hi, scale, false),
-                      bf16_of_e4m3(hi, scale, true));
-  } else {
-    float v[8];
-    values_of<T>(r, v);
-#pragma unroll
-    for (int j = 0; j < parts_of(T); ++j) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t b[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float& x = v[2 * i + e];
-          if (j + 1 < parts_of(T)) {
-            b[e] = f32_bits(__builtin_amdgcn_fmed3f(x, -kBf16Max, kBf16Max)) & 0xFFFF0000u;
-            x -= bits_f32(b[e]);
-          } else {
-            b[e] = f32_bits(x);
-          }
-        }
-        p[j][i] = __builtin_amdgcn_perm(b[1], b[0], 0x07060302u);
-      }
-    }
-  }
-}
-
-// Eight weights of one block as bf16.
-__device__ __forceinline__ u32x4 weights8(uint32_t w, float scale) {
-  return u32x4_make(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)),
-                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
-                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)),
-                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3)));
-}
-
-// The same as f16, where they are in its range.
+// Eight weights of one block as f16, where they are in its range.
 __device__ __forceinline__ u32x4 weights8_f16(uint32_t w, float scale) {
   return u32x4_make(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0)),
                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1)),
@@ -102,48 +47,12 @@ __device__ __forceinline__ bool scales_fit_f16(uint32_t s) {
   return ((s + 0x18181818u) & 0xE0E0E0E0u) == 0x80808080u;
 }
 
-__device__ __forceinline__ float scale_f32(uint32_t byte) { return bits_f32(byte << 23); }
-
-__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
 template <bool F16>
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
   if constexpr (F16)
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-// Outputs n .. n+3 of token t with their bias, those that exist.
-template <uint32_t OT>
-__device__ __forceinline__ void store4_as(const MxLinearArgs& a, uint64_t t, uint32_t n, f32x4 v) {
-  const uint64_t at = a.out.ptr + (t * a.out.stride + n) * type_bytes(OT);
-  if (n + 3 < a.rows) {
-    if (a.bias) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] += load1<OT>(a.bias + (uint64_t)(n + j) * type_bytes(OT));
-    }
-    if constexpr (OT == kTypeF32)
-      st16(at, __builtin_bit_cast(u32x4, v));
-    else
-      st8(at, pack2<OT>(v[0], v[1]) | (uint64_t)pack2<OT>(v[2], v[3]) << 32);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 3; ++j)
-      if (n + j < a.rows)
-        store1<OT>(at + j * type_bytes(OT),
-                   a.bias ? v[j] + load1<OT>(a.bias + (uint64_t)(n + j) * type_bytes(OT)) : v[j]);
-  }
-}
-__device__ __forceinline__ void store4(const MxLinearArgs& a, uint64_t t, uint32_t n, f32x4 v) {
-  if (a.out_type == kTypeBf16)
-    store4_as<kTypeBf16>(a, t, n, v);
-  else if (a.out_type == kTypeF16)
-    store4_as<kTypeF16>(a, t, n, v);
-  else
-    store4_as<kTypeF32>(a, t, n, v);
 }
 
 // Small products, and rows too far apart for a tile's 32-bit offsets: a 16x16 tile of
@@ -763,48 +672,16 @@ __global__ __launch_bounds__(64 * kFewWaves) void mxfp4_linear_few_kernel(MxLine
   }
 }
 
-// The outputs of rows first .. first + rows - 1, and of tokens.
-MxLinearArgs some_rows(const MxLinearArgs& a, uint64_t first, uint64_t rows) {
-  MxLinearArgs p = a;
-  const uint64_t skip = first * type_bytes(a.out_type);
-  p.weight = rows_from(a.weight, first, 1), p.scales = rows_from(a.scales, first, 1);
-  p.out.ptr += skip, p.bias = a.bias ? a.bias + skip : 0;
-  p.rows = (uint32_t)rows;
-  return p;
-}
-template <uint32_t T>
-MxLinearArgs some_tokens(const MxLinearArgs& a, uint64_t first, uint64_t tokens) {
-  MxLinearArgs p = a;
-  p.x = rows_from(a.x, first, type_bytes(T)), p.x_scales = rows_from(a.x_scales, first, 1);
-  p.out = rows_from(a.out, first, type_bytes(a.out_type));
-  p.tokens = tokens;
-  return p;
-}
-
-// Workgroups of TR rows and TT tokens each, rows first, in as few launches as hold them.
-template <uint32_t T, uint32_t TR, uint32_t TT>
-hipError_t launch_tiles(void (*kernel)(MxLinearArgs), uint32_t threads, const MxLinearArgs& a, hipStream_t stream,
-                        uint32_t shared = 0) {
-  const uint64_t most = kMaxThreads / threads;
-  return in_parts(a.rows, most * TR, [&](uint64_t row, uint64_t rows) {
-    const uint64_t row_tiles = (rows + TR - 1) / TR;
-    return in_parts(a.tokens, most / row_tiles * TT, [&](uint64_t token, uint64_t tokens) {
-      return launch(kernel, row_tiles * ((tokens + TT - 1) / TT), threads,
-                    some_tokens<T>(some_rows(a, row, rows), token, tokens), stream, shared);
-    });
-  });
-}
-
 template <uint32_t T, int ROWS, int CT, int RG, int KG, bool RAW>
 hipError_t tiles_of(const MxLinearArgs& a, bool aligned, hipStream_t stream) {
-  return launch_tiles<T, ROWS * RG, 32 * CT>(aligned ? mxfp4_linear_tiles_kernel<T, ROWS, CT, RG, KG, RAW, true>
+  return launch_tiles<type_bytes(T), ROWS * RG, 32 * CT>(aligned ? mxfp4_linear_tiles_kernel<T, ROWS, CT, RG, KG, RAW, true>
                                                      : mxfp4_linear_tiles_kernel<T, ROWS, CT, RG, KG, RAW, false>,
                                              64 * RG * KG, a, stream);
 }
 
 template <uint32_t T, int NT>
 hipError_t few_of(const MxLinearArgs& a, hipStream_t stream) {
-  return launch_tiles<T, 16, NT>(mxfp4_linear_few_kernel<T, NT>, 64 * kFewWaves, a, stream,
+  return launch_tiles<type_bytes(T), 16, NT>(mxfp4_linear_few_kernel<T, NT>, 64 * kFewWaves, a, stream,
                                  (uint32_t)mx_few_bytes(a.cols, NT));
 }
 
@@ -839,7 +716,7 @@ hipError_t linear_of(const MxLinearArgs& a, hipStream_t stream) {
       if (is(64, 2, 1, 4)) return tiles_of<T, 64, 2, 1, 4, true>(a, k.aligned, stream);
     return hipErrorInvalidValue;
   }
-  return launch_tiles<T, 16, 16>(mxfp4_linear_kernel<T>, 256, a, stream);
+  return launch_tiles<type_bytes(T), 16, 16>(mxfp4_linear_kernel<T>, 256, a, stream);
 }
 
 }  // namespace

@@ -8,6 +8,7 @@
 // tensor of the wanted type, ValueError for sizes, strides and devices,
 // NativeError for a refusal of the library.
 #define PY_SSIZE_T_CLEAN
+#include <ATen/ops/empty.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -129,6 +130,10 @@ int64_t device_of(PyObject* o) {
 decltype(&ptwm_mi355x_rms_norm_mx_cuda) g_norm;
 decltype(&ptwm_mi355x_swiglu_mx_cuda) g_swiglu;
 decltype(&ptwm_mi355x_mxfp4_linear_cuda) g_linear;
+decltype(&ptwm_mi355x_mxfp4_quantise_cuda) g_quantise;
+decltype(&ptwm_mi355x_mxfp4_matmul_cuda) g_matmul;
+decltype(&ptwm_mi355x_mxfp4_moe_workspace) g_moe_workspace;
+decltype(&ptwm_mi355x_mxfp4_moe_cuda) g_moe;
 
 PyObject* g_stream;  // torch's current stream of a device
 PyObject* g_error;   // NativeError
@@ -245,6 +250,143 @@ PyObject* mxfp4_linear_cuda(PyObject*, PyObject* const* args, Py_ssize_t n, PyOb
   });
 }
 
+PyObject* mxfp4_quantise_cuda(PyObject*, PyObject* const* args, Py_ssize_t n, PyObject* keywords) {
+  return guarded([&]() -> PyObject* {
+    static const char* names[] = {"x", "codes", "scales", "device_ordinal", "saturate"};
+    PyObject* a[5];
+    take_args(names, 3, args, n, keywords, a);
+    const int64_t device = device_of(a[3]);
+    const at::Tensor& x = input(a[0], "x");
+    const int64_t rows = x.size(0), cols = x.size(1);
+    const Rows xr = matrix(x, "x", rows, cols, device, kReal);
+    const Rows codes = matrix(tensor(a[1], "codes"), "codes", rows, cols / 2, device, kWeight);
+    const Rows scales = matrix(tensor(a[2], "scales"), "scales", rows, cols / 32, device, kScales);
+    const int saturate = a[4] ? PyObject_IsTrue(a[4]) : 1;
+    if (saturate < 0) throw Failed();
+    if (rows == 0) Py_RETURN_NONE;
+    return done(g_quantise(code_of(x.scalar_type()), xr.ptr, xr.stride, codes.ptr, codes.stride, scales.ptr,
+                           scales.stride, rows, cols, saturate, stream_of(device), (uint32_t)device),
+                "mxfp4_quantise_cuda");
+  });
+}
+
+PyObject* mxfp4_matmul_cuda(PyObject*, PyObject* const* args, Py_ssize_t n, PyObject* keywords) {
+  return guarded([&]() -> PyObject* {
+    static const char* names[] = {"x", "x_scales", "weight", "scales", "out", "device_ordinal", "bias"};
+    PyObject* a[7];
+    take_args(names, 5, args, n, keywords, a);
+    const int64_t device = device_of(a[5]);
+    const at::Tensor& x = tensor(a[0], "x");
+    if (x.dim() != 2) fail(PyExc_ValueError, "x: expected a matrix, a row a token");
+    const int64_t tokens = x.size(0), half = x.size(1);
+    if (half == 0 || half % 16) fail(PyExc_ValueError, "x: %lld bytes of codes are not whole blocks of 16", (long long)half);
+    const Rows xr = matrix(x, "x", tokens, half, device, kWeight);
+    const Rows xs = matrix(tensor(a[1], "x_scales"), "x_scales", tokens, half / 16, device, kScales);
+    const at::Tensor& weight = tensor(a[2], "weight");
+    const int64_t rows = weight.dim() ? weight.size(0) : 0;
+    const Rows w = matrix(weight, "weight", rows, half, device, kWeight);
+    const Rows s = matrix(tensor(a[3], "scales"), "scales", rows, half / 16, device, kScales);
+    const at::Tensor& out = tensor(a[4], "out");
+    const Rows o = matrix(out, "out", tokens, rows, device, kReal);
+    const uint64_t bias = a[6] ? vector(tensor(a[6], "bias"), "bias", rows, device, {out.scalar_type()}) : 0;
+    if (tokens == 0 || rows == 0) Py_RETURN_NONE;
+    return done(g_matmul(xr.ptr, xr.stride, xs.ptr, xs.stride, w.ptr, w.stride, s.ptr, s.stride,
+                         code_of(out.scalar_type()), bias, o.ptr, o.stride, tokens, rows, half * 2,
+                         stream_of(device), (uint32_t)device),
+                "mxfp4_matmul_cuda");
+  });
+}
+
+// A stack of matrices [experts, rows, cols] whose rows are contiguous and do not overlap: address, rows' and experts'
+// strides.
+void stack(PyObject* o, const char* name, int64_t experts, int64_t rows, int64_t cols, int64_t device,
+           const Types& types, uint64_t& ptr, uint64_t& stride, uint64_t& expert) {
+  const at::Tensor& t = tensor(o, name);
+  check_place(t, name, device, types);
+  if (t.dim() != 3 || t.size(0) != experts || t.size(1) != rows || t.size(2) != cols) {
+    std::string shape;
+    for (int64_t s : t.sizes()) shape += (shape.empty() ? "" : ", ") + std::to_string(s);
+    fail(PyExc_ValueError, "%s: shape (%s) is not (%lld, %lld, %lld)", name, shape.c_str(), (long long)experts,
+         (long long)rows, (long long)cols);
+  }
+  if ((t.stride(2) != 1 && cols > 1) || (t.stride(1) < cols && rows > 1))
+    fail(PyExc_ValueError, "%s: rows must be contiguous and must not overlap", name);
+  ptr = reinterpret_cast<uint64_t>(t.data_ptr()), stride = (uint64_t)t.stride(1), expert = (uint64_t)t.stride(0);
+}
+
+// One product's weights: codes, scales and an optional bias [experts, rows] at any strides.
+ptwm_mi355x_experts experts_of(PyObject* codes, const char* name, PyObject* scales, const char* scales_name,
+                               PyObject* bias, const char* bias_name, int64_t experts, int64_t rows, int64_t cols,
+                               int64_t device, at::ScalarType bias_type) {
+  ptwm_mi355x_experts w = {};
+  stack(codes, name, experts, rows, cols / 2, device, kWeight, w.codes, w.codes_stride, w.codes_expert);
+  stack(scales, scales_name, experts, rows, cols / 32, device, kScales, w.scales, w.scales_stride, w.scales_expert);
+  if (bias) {
+    const at::Tensor& b = tensor(bias, bias_name);
+    check_place(b, bias_name, device, {bias_type});
+    if (b.dim() != 2 || b.size(0) != experts || b.size(1) != rows)
+      fail(PyExc_ValueError, "%s: shape is not (%lld, %lld)", bias_name, (long long)experts, (long long)rows);
+    w.bias = reinterpret_cast<uint64_t>(b.data_ptr());
+    w.bias_stride = (uint64_t)b.stride(1), w.bias_expert = (uint64_t)b.stride(0);
+  }
+  return w;
+}
+
+PyObject* mxfp4_moe_cuda(PyObject*, PyObject* const* args, Py_ssize_t n, PyObject* keywords) {
+  return guarded([&]() -> PyObject* {
+    static const char* names[] = {"x",         "router",    "gate",           "gate_scales", "up",        "up_scales",
+                                  "down",      "down_scales", "out",          "top_k",       "device_ordinal",
+                                  "router_bias", "gate_bias", "up_bias",      "down_bias",   "experts",   "weights"};
+    PyObject* a[17];
+    take_args(names, 10, args, n, keywords, a);
+    ptwm_mi355x_mxfp4_moe c = {};
+    const int64_t device = device_of(a[10]);
+    const at::Tensor& x = input(a[0], "x");
+    const int64_t tokens = x.size(0), cols = x.size(1);
+    const Rows xr = matrix(x, "x", tokens, cols, device, kReal);
+    const at::Tensor& router = tensor(a[1], "router");
+    const int64_t experts = router.dim() ? router.size(0) : 0;
+    const Rows r = matrix(router, "router", experts, cols, device, kReal);
+    const at::Tensor& gate = tensor(a[2], "gate");
+    const int64_t inner = gate.dim() == 3 ? gate.size(1) : 0;
+    if (inner == 0 || inner % 32)
+      fail(PyExc_ValueError, "gate: expected [experts, inner, cols / 2] with inner in whole blocks of 32");
+    const at::Tensor& out = tensor(a[8], "out");
+    const Rows o = matrix(out, "out", tokens, cols, device, kReal);
+    const int64_t top_k = PyLong_AsLongLong(a[9]);
+    if (top_k == -1 && PyErr_Occurred()) throw Failed();
+    if (top_k < 1 || top_k > 32 || top_k > experts || experts > 1024)
+      fail(PyExc_ValueError, "top_k: %lld of %lld experts, up to 32 of up to 1024 can be chosen", (long long)top_k,
+           (long long)experts);
+    if (cols > 131072 || inner > 131072) fail(PyExc_ValueError, "x, gate: rows and inner sizes up to 131072 are taken");
+    const at::ScalarType type = out.scalar_type();
+    c.gate = experts_of(a[2], "gate", a[3], "gate_scales", a[12], "gate_bias", experts, inner, cols, device, type);
+    c.up = experts_of(a[4], "up", a[5], "up_scales", a[13], "up_bias", experts, inner, cols, device, type);
+    c.down = experts_of(a[6], "down", a[7], "down_scales", a[14], "down_bias", experts, cols, inner, device, type);
+    if (a[11]) c.router_bias = vector(tensor(a[11], "router_bias"), "router_bias", experts, device, {router.scalar_type()});
+    const auto chosen = [&](PyObject* t, const char* name, at::ScalarType kind) -> uint64_t {
+      if (!t) return 0;
+      const Rows m = matrix(tensor(t, name), name, tokens, top_k, device, {kind});
+      if (!THPVariable_Unpack(t).is_contiguous()) fail(PyExc_ValueError, "%s: must be contiguous", name);
+      return m.ptr;
+    };
+    c.experts_out = chosen(a[15], "experts", at::kInt);
+    c.weights_out = chosen(a[16], "weights", at::kFloat);
+    if (tokens == 0) Py_RETURN_NONE;
+    c.x = xr.ptr, c.x_stride = xr.stride, c.router = r.ptr, c.router_stride = r.stride;
+    c.out = o.ptr, c.out_stride = o.stride;
+    c.tokens = tokens, c.experts = experts, c.top_k = top_k, c.cols = cols, c.inner = inner;
+    c.x_dtype = code_of(x.scalar_type()), c.router_dtype = code_of(router.scalar_type()), c.out_dtype = code_of(type);
+    const int64_t bytes = g_moe_workspace(&c);
+    if (bytes < 0) return done(bytes, "mxfp4_moe_cuda");
+    // from torch's allocator: the current stream's, or a captured graph's own, so no two calls at once share it
+    const at::Tensor workspace =
+        at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, (at::DeviceIndex)device));
+    c.workspace = reinterpret_cast<uint64_t>(workspace.data_ptr()), c.workspace_bytes = bytes;
+    return done(g_moe(&c, stream_of(device), (uint32_t)device), "mxfp4_moe_cuda");
+  });
+}
+
 PyDoc_STRVAR(kNormDoc,
              "rms_norm_mx_cuda(x, weight, out, out_scales, device_ordinal=0, residual=None, sum_out=None, eps=1e-06)\n"
              "--\n\n"
@@ -275,10 +417,56 @@ PyDoc_STRVAR(kLinearDoc,
              "held in 32 bits.  Rows may lie at any stride, but are contiguous.\n"
              "Queued on torch's current stream; nothing is waited for.");
 
+PyDoc_STRVAR(kQuantiseDoc,
+             "mxfp4_quantise_cuda(x, codes, scales, device_ordinal=0, saturate=True)\n--\n\n"
+             "Values to MXFP4 (library addition): ``codes`` [rows, cols / 2] (uint8 or\n"
+             "float4_e2m1fn_x2) receives e2m1 codes, the first of two in the low nibble,\n"
+             "``scales`` [rows, cols / 32] (float8_e8m0fnu or uint8) a power of two for\n"
+             "each block of 32.  With ``saturate`` the scale leaves a block's largest\n"
+             "magnitude in [4, 8) and what is above 6 becomes 6; without it the scale is\n"
+             "the smallest with which nothing is above 6.  Codes are rounded to nearest,\n"
+             "ties to even.  A block with an infinity or NaN gets the scale NaN.\n"
+             "x [rows, cols]: float32, float16 or bfloat16, rows at any stride.\n"
+             "Queued on torch's current stream; nothing is waited for.");
+PyDoc_STRVAR(kMatmulDoc,
+             "mxfp4_matmul_cuda(x, x_scales, weight, scales, out, device_ordinal=0, bias=None)\n--\n\n"
+             "``out = x @ W.T (+ bias)`` with both matrices in MXFP4 (library addition):\n"
+             "``x`` [tokens, cols / 2] and ``weight`` [rows, cols / 2] hold e2m1 codes,\n"
+             "``x_scales`` and ``scales`` their E8M0 bytes, as mxfp4_quantise_cuda writes\n"
+             "them and a decode restores them.  out [tokens, rows] is float32, float16 or\n"
+             "bfloat16, bias [rows] of out's dtype.  Products are exact, sums are held in\n"
+             "32 bits.  Rows may lie at any stride, but are contiguous.\n"
+             "Queued on torch's current stream; nothing is waited for.");
+PyDoc_STRVAR(kMoeDoc,
+             "mxfp4_moe_cuda(x, router, gate, gate_scales, up, up_scales, down, down_scales, out, top_k,\n"
+             "               device_ordinal=0, router_bias=None, gate_bias=None, up_bias=None, down_bias=None,\n"
+             "               experts=None, weights=None)\n--\n\n"
+             "A mixture-of-experts layer on MXFP4 experts for a few tokens (library\n"
+             "addition).  A token's logits are ``x @ router.T (+ router_bias)``, summed in\n"
+             "64 bits; its top_k experts are those with the largest, the lowest index of\n"
+             "equal ones, weighted by a softmax over them.  ``out`` is the weighted sum of\n"
+             "``h @ down[e].T (+ down_bias[e])`` with ``h = silu(x @ gate[e].T\n"
+             "(+ gate_bias[e])) * (x @ up[e].T (+ up_bias[e]))``.  A logit of minus\n"
+             "infinity keeps an expert out, with the weight 0.\n\n"
+             "x, out [tokens, cols] and router [experts, cols]: float32, float16 or\n"
+             "bfloat16 each; router_bias [experts] of router's dtype.  gate and up\n"
+             "[experts, inner, cols / 2] and down [experts, cols, inner / 2] hold e2m1\n"
+             "codes, with scales [..., / 32], as a decode restores them; their rows are\n"
+             "contiguous, at any stride: views of one tensor, its halves or every second\n"
+             "row, will do.  gate_bias, up_bias [experts, inner] and down_bias [experts,\n"
+             "cols]: out's dtype, any strides.  ``experts`` (int32) and ``weights``\n"
+             "(float32) [tokens, top_k], contiguous, receive the choice, largest first.\n"
+             "out may be x.  Up to 32 of up to 1024 experts; more than 64 tokens take\n"
+             "several passes over the weights.  The workspace comes from torch's\n"
+             "allocator.  Queued on torch's current stream; nothing is waited for.");
+
 PyMethodDef kMethods[] = {
     {"rms_norm_mx_cuda", (PyCFunction)(void (*)(void))rms_norm_mx_cuda, METH_FASTCALL | METH_KEYWORDS, kNormDoc},
     {"swiglu_mx_cuda", (PyCFunction)(void (*)(void))swiglu_mx_cuda, METH_FASTCALL | METH_KEYWORDS, kSwigluDoc},
     {"mxfp4_linear_cuda", (PyCFunction)(void (*)(void))mxfp4_linear_cuda, METH_FASTCALL | METH_KEYWORDS, kLinearDoc},
+    {"mxfp4_quantise_cuda", (PyCFunction)(void (*)(void))mxfp4_quantise_cuda, METH_FASTCALL | METH_KEYWORDS, kQuantiseDoc},
+    {"mxfp4_matmul_cuda", (PyCFunction)(void (*)(void))mxfp4_matmul_cuda, METH_FASTCALL | METH_KEYWORDS, kMatmulDoc},
+    {"mxfp4_moe_cuda", (PyCFunction)(void (*)(void))mxfp4_moe_cuda, METH_FASTCALL | METH_KEYWORDS, kMoeDoc},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "ptwm_amd._mx", "Operators on MX blocks.", -1, kMethods,
@@ -304,8 +492,12 @@ PyMODINIT_FUNC PyInit__mx(void) {
     g_norm = reinterpret_cast<decltype(g_norm)>(dlsym(lib, "ptwm_mi355x_rms_norm_mx_cuda"));
     g_swiglu = reinterpret_cast<decltype(g_swiglu)>(dlsym(lib, "ptwm_mi355x_swiglu_mx_cuda"));
     g_linear = reinterpret_cast<decltype(g_linear)>(dlsym(lib, "ptwm_mi355x_mxfp4_linear_cuda"));
+    g_quantise = reinterpret_cast<decltype(g_quantise)>(dlsym(lib, "ptwm_mi355x_mxfp4_quantise_cuda"));
+    g_matmul = reinterpret_cast<decltype(g_matmul)>(dlsym(lib, "ptwm_mi355x_mxfp4_matmul_cuda"));
+    g_moe_workspace = reinterpret_cast<decltype(g_moe_workspace)>(dlsym(lib, "ptwm_mi355x_mxfp4_moe_workspace"));
+    g_moe = reinterpret_cast<decltype(g_moe)>(dlsym(lib, "ptwm_mi355x_mxfp4_moe_cuda"));
   }
-  if (!g_norm || !g_swiglu || !g_linear) {
+  if (!g_norm || !g_swiglu || !g_linear || !g_quantise || !g_matmul || !g_moe_workspace || !g_moe) {
     PyErr_SetString(PyExc_ImportError, "the library lacks the operators on MX blocks");
     return nullptr;
   }
