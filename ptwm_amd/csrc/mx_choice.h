@@ -1,5 +1,5 @@
-// mx_choice.h -- which kernel takes a product with MXFP4 weights: rules on
-// sizes, types and alignment, on the host.  The times beside them are
+// mx_choice.h -- which kernel takes a product with MXFP4 weights, and of two
+// MXFP4 matrices: rules on sizes, types and alignment, on the host.  The times beside them are
 // microseconds on an MI355X.
 #pragma once
 
@@ -100,6 +100,48 @@ inline MxLinearChoice choose_mxfp4_linear(uint32_t type, const MxLinearArgs& a) 
   const bool small = a.cols <= 512 && tiles * ((a.cols + 127) / 128) <= 2048;
   if (const uint32_t nt = mx_few_tokens(type, a)) return {MxLinearChoice::kFew, nt, 0, 0, 0, 0, false};
   return small ? MxLinearChoice{MxLinearChoice::kSmall, 0, 0, 0, 0, 0, false} : mx_tile_by_size(type, a);
+}
+
+struct MxMatmulChoice {
+  // rows and tokens of a tile; by: wavefronts that share the length of the rows
+  enum Kind : uint32_t { kSmall, k256x256, k256x128, k128x128, k128x64, k64x64, k32x32by8, k32x32by4 } kind;
+  int dma;  // what goes to LDS by DMA: nothing, the codes (1), the scales too (2)
+};
+
+// The product of two MXFP4 matrices; x.stride and weight.stride in bytes.
+inline MxMatmulChoice choose_mxfp4_matmul(const MxLinearArgs& a) {
+  const auto count = [&](uint64_t rows, uint64_t tokens) {
+    return ((a.rows + rows - 1) / rows) * ((a.tokens + tokens - 1) / tokens);
+  };
+  const auto tile = [&](MxMatmulChoice::Kind kind, uint64_t rows, uint64_t tokens) -> MxMatmulChoice {
+    const uint64_t n = a.rows < rows ? a.rows : rows, t = a.tokens < tokens ? a.tokens : tokens;
+    if (!mx_within_reach(n, a.weight.stride, 1, a.cols / 2) || !mx_within_reach(t, a.x.stride, 1, a.cols / 2))
+      return {MxMatmulChoice::kSmall, 0};
+    const auto whole = [](const MxRows& r, uint64_t count) { return r.ptr % 16 == 0 && (count <= 1 || r.stride % 16 == 0); };
+    if (!whole(a.weight, n) || !whole(a.x, t)) return {kind, 0};
+    // whole quads, so that no scales are read past a row's end
+    return {kind, a.cols % 512 == 0 && whole(a.scales, n) && whole(a.x_scales, t) ? 2 : 1};
+  };
+  // Small products of one quad of steps end sooner without stages in LDS: 16x4096x256 2.4 and 3.4, 64x4704x256 3.1 and
+  // 4.5, 100x1024x512 2.9 and 3.6.
+  if (a.cols <= 512 && count(16, 16) * ((a.cols + 127) / 128) <= 2048) return {MxMatmulChoice::kSmall, 0};
+  // The largest tile of which there are enough for the 256 CUs: measured (256x256, 256x128, 128x128, 128x64)
+  // 1024x14336x4096 (224, 448, 896, 1792 tiles) 36, 42, 50, 59; 512x14336x4096 (112, 224, 448, 896) 29, 22, 26, 35;
+  // 300x14336x4096 (112, 168, 336, 560) 27, 19, 23, 25; 200x14336x4096 (56, 112, 224, 448) 27, 19, 14, 18;
+  // 700x3000x2048 (36, 72, 144, 264) 16, 11, 8, 11; 400x4096x4096 (32, 64, 128, 224) 26, 18, 12, 10.
+  if (count(256, 256) >= 160) return tile(MxMatmulChoice::k256x256, 256, 256);
+  if (count(256, 128) >= 144) return tile(MxMatmulChoice::k256x128, 256, 128);
+  if (count(128, 128) >= 136) return tile(MxMatmulChoice::k128x128, 128, 128);
+  // Few tokens or rows: wavefronts share the length of the rows, eight where each tile has a CU of its own: measured
+  // (eight, four, 64x64 tiles) 64x4096x4096 (256 tiles of 32) 4.7, 5.0, 7.9; 1x4096x14336 (128) 8.6, 10.9, 16;
+  // 37x5001x3360 (314) 7.5, 5.9, 9.2; 1x14336x4096 (448) 8.4, 7.4, 8.0; 33x14336x4096 (896) 12.8, 9.9, 8.5.
+  if (a.cols > 512) {
+    if (count(32, 32) <= 256) return tile(MxMatmulChoice::k32x32by8, 32, 32);
+    if (count(32, 32) <= 512) return tile(MxMatmulChoice::k32x32by4, 32, 32);
+  }
+  // 64x14336x4096 (224 tiles of 64x64, 112 of 128x64) 8.7 and 10.0, 128x14336x4096 (448, 224) 11.6 and 10.7.
+  if (count(64, 64) <= 256) return tile(MxMatmulChoice::k64x64, 64, 64);
+  return tile(MxMatmulChoice::k128x64, 128, 64);
 }
 
 }  // namespace ptwm
