@@ -36,6 +36,7 @@ hipError_t in_parts(uint64_t rows, uint64_t most, F&& f) {
 }
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -75,6 +76,36 @@ __device__ __forceinline__ u32x4 ld16(GlobalBytes p, uint32_t at) {
 }
 __device__ __forceinline__ uint32_t ld4(GlobalBytes p, uint32_t at) {
   return ((const __attribute__((address_space(1))) Bytes4*)(p + at))->v;
+}
+
+// An address that is the same in all lanes, in scalar registers.
+__device__ __forceinline__ GlobalBytes uniform(uint64_t a) {
+  // the builtin's result is signed
+  const uint32_t low = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a);
+  const uint32_t high = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32));
+  return global_bytes(low | (uint64_t)high << 32);
+}
+
+// DMA of 16 bytes a lane from a uniform address and the lane's offset to consecutive places in LDS from `to` (uniform)
+// on.  Written out, because the compiler waits for all that is on its way before it reads LDS.  Nothing but a wait on vmcnt says that the bytes have come.
+__device__ __forceinline__ void dma16(GlobalBytes from, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(from)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void dma16(uint64_t from, uint32_t to) {  // from the lane's own address
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory", "m0");
+}
+
+__device__ __forceinline__ void dma4(uint64_t from, uint32_t to) {  // 4 bytes a lane, from multiples of 4
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "memory", "m0");
+}
+
+// LDS by its byte address, which takes a known offset along in the instruction.
+typedef __attribute__((address_space(3))) u32x4* LdsChunks;
+typedef __attribute__((address_space(3))) u32x2* LdsPairs;
+template <typename T>
+__device__ __forceinline__ uint32_t lds_address(T* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) T*)p;
 }
 
 __device__ __forceinline__ float bits_f32(uint32_t b) { return __builtin_bit_cast(float, b); }
