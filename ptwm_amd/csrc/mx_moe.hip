@@ -8,12 +8,10 @@
 // What it cannot do without is the chosen experts' weights from memory, each
 // once; all else is small.  The kernels:
 //   logits   a workgroup an expert and four tokens; x as bf16 parts
-//   route    (two tokens on) the choice, and the pairs of token and expert
-//            sorted by expert
+//   route    the choice, a wavefront a token (few tokens: within the next one)
 //   inner    gate and up products of an expert's tokens, h as bf16 parts
-//   outer    the down products; of one token, their weighted sum at once
-//   combine  (two tokens on) the weighted sums
-// One token takes three launches: the inner products choose for themselves.
+//   outer    the down products; of a few tokens, their weighted sums at once
+//   combine  (many tokens) the weighted sums
 //
 // The products are of bf16 on the matrix unit.  Weights are widened to bf16,
 // which is exact; x, and h, are the sum of one to three bf16 values (parts),
@@ -33,22 +31,14 @@ constexpr uint32_t kStep = 256;   // values of a row that go through LDS togethe
 // h's parts: 24 significant bits where the outputs have 24, else 16, the rounding of a 2^-8 or 2^-5 of the output's own.
 constexpr uint32_t inner_parts(uint32_t out_type) { return out_type == kTypeF32 ? 3 : 2; }
 
-struct Active {  // an expert with tokens
-  uint32_t expert, first, count, unused;
-};
-
-// Where a launch's intermediate results lie in the workspace.
+// Where a launch's intermediate results lie in the workspace.  A pair is a token's k-th expert, token * top_k + k.
 struct MoePlaces {
   uint64_t logits;   // f64 [tokens][experts]
   uint64_t x;        // bf16 [parts][tokens][x_len]
-  uint64_t h;        // bf16 [parts][tokens * top_k][h_len], rows sorted by expert
-  uint64_t y;        // f32 [tokens * top_k][cols], rows as h's
-  uint64_t chosen;   // int32 [tokens * top_k], -1 where a chosen expert is masked
-  uint64_t weights;  // f32 [tokens * top_k]
-  uint64_t place;    // int32 [tokens * top_k]: row of a pair in h and y, -1 without one
-  uint64_t order;    // int32 [tokens * top_k]: the pair of a row
-  uint64_t active;   // Active [experts with tokens]
-  uint64_t actives;  // their number
+  uint64_t h;        // bf16 [parts][pairs][h_len]
+  uint64_t y;        // f32 [pairs][cols]
+  uint64_t chosen;   // int32 [pairs], -1 where a chosen expert is masked
+  uint64_t weights;  // f32 [pairs]
   uint64_t end;
   uint32_t x_len, h_len;  // cols and inner in whole steps, zeros past their ends
 };
@@ -67,9 +57,6 @@ MoePlaces places_of(const MxMoeArgs& a) {
   p.h = take(inner_parts(a.out_type) * pairs * p.h_len * 2);
   p.y = take(pairs * a.cols * 4);
   p.chosen = take(pairs * 4), p.weights = take(pairs * 4);
-  p.place = take(pairs * 4), p.order = take(pairs * 4);
-  p.active = take((pairs < a.experts ? pairs : a.experts) * sizeof(Active));
-  p.actives = take(4);
   p.end = at;
   return p;
 }
@@ -177,239 +164,206 @@ __device__ __forceinline__ uint64_t wave_max(uint64_t v) {
   return lo | (uint64_t)hi << 32;
 }
 
-// A token's experts in the order of their logits, by one wavefront: the largest that is left, the lowest expert of equal
-// ones.
-struct Choice {
-  uint64_t key[kMoeMaxExperts / 64];
-  uint64_t best;  // the last one taken
-  __device__ __forceinline__ Choice(const MoeArgs& m, uint32_t t) {
-    const uint32_t lane = threadIdx.x & 63;
+// Chooses a token's experts: the largest that is left, the lowest expert of equal ones.  One wavefront, N logits a
+// lane; lane k returns the k-th, with its weight.  An expert at minus infinity has none, not even among its like.
+struct Chosen {
+  int32_t expert;  // -1 where masked
+  float weight;
+  int32_t reported;
+};
+template <uint32_t N>
+__device__ __forceinline__ Chosen choose_of(const MoeArgs& m, uint32_t t) {
+  const uint32_t lane = threadIdx.x & 63;
+  uint64_t key[N];
 #pragma unroll
-    for (uint32_t j = 0; j < kMoeMaxExperts / 64; ++j) {
-      const uint32_t e = j * 64 + lane;
-      key[j] = e < m.a.experts ? order_of(g_ld<double>(m.p.logits + ((uint64_t)t * m.a.experts + e) * 8)) : 0;
-    }
+  for (uint32_t j = 0; j < N; ++j) {
+    const uint32_t e = j * 64 + lane;
+    key[j] = e < m.a.experts ? order_of(g_ld<double>(m.p.logits + ((uint64_t)t * m.a.experts + e) * 8)) : 0;
   }
-  __device__ __forceinline__ uint32_t next(uint32_t experts) {
-    uint64_t most = 0;
+  Chosen mine{0, 0, 0};
+  uint64_t own = 0, top = 0;
+  for (uint32_t k = 0; k < m.a.top_k; ++k) {
+    uint64_t most = key[0];
 #pragma unroll
-    for (uint32_t j = 0; j < kMoeMaxExperts / 64; ++j)
-      if (j * 64 < experts) most = key[j] > most ? key[j] : most;
-    best = wave_max(most);
+    for (uint32_t j = 1; j < N; ++j) most = key[j] > most ? key[j] : most;
+    const uint64_t best = wave_max(most);
     uint32_t e = 0;
     bool found = false;
 #pragma unroll
-    for (uint32_t j = 0; j < kMoeMaxExperts / 64; ++j) {
-      if (j * 64 >= experts || found) continue;
+    for (uint32_t j = 0; j < N; ++j) {
       const uint64_t at = __ballot(key[j] == best);
-      if (!at) continue;
+      if (found || !at) continue;
       found = true;
-      const uint32_t lane = (uint32_t)__ffsll((long long)at) - 1;
-      e = j * 64 + lane;
-      if ((threadIdx.x & 63) == lane) key[j] = 0;
+      const uint32_t owner = (uint32_t)__ffsll((long long)at) - 1;
+      e = j * 64 + owner;
+      if (lane == owner) key[j] = 0;
     }
-    return e;
-  }
-};
-
-// Chooses a token's experts: lane k returns the k-th, with its weight.  An expert at minus infinity has none, not even
-// among its like.
-struct Chosen {
-  uint32_t expert;
-  float weight;
-  bool masked;
-};
-__device__ __forceinline__ Chosen choose(const MoeArgs& m, uint32_t t) {
-  const uint32_t lane = threadIdx.x & 63;
-  Choice c(m, t);
-  Chosen mine{0, 0, false};
-  double logit = 0, top = 0;
-  for (uint32_t k = 0; k < m.a.top_k; ++k) {
-    const uint32_t e = c.next(m.a.experts);
-    const double l = logit_of(c.best);
-    if (k == 0) top = l;
-    if (k == lane) mine.expert = e, logit = l;
+    if (k == 0) top = best;
+    if (k == lane) mine.reported = (int32_t)e, own = best;
   }
   const bool in = lane < m.a.top_k;
-  mine.masked = logit == -__builtin_inf();
-  const float w = in && !mine.masked ? expf((float)(logit - top)) : 0.0f;
+  const double logit = logit_of(own);
+  const bool masked = logit == -__builtin_inf();
+  const float w = in && !masked ? expf((float)(logit - logit_of(top))) : 0.0f;
   float sum = w;
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
-  mine.weight = mine.masked ? 0.0f : w / sum;
-  if (in) {
-    const uint64_t at = (uint64_t)t * m.a.top_k + lane;
-    g_st<int32_t>(m.p.chosen + at * 4, mine.masked ? -1 : (int32_t)mine.expert);
-    g_st<float>(m.p.weights + at * 4, mine.weight);
-    if (m.a.experts_out) g_st<int32_t>(m.a.experts_out + at * 4, (int32_t)mine.expert);
-    if (m.a.weights_out) g_st<float>(m.a.weights_out + at * 4, mine.weight);
-  }
+  mine.weight = masked ? 0.0f : w / sum;
+  mine.expert = masked ? -1 : mine.reported;
   return mine;
 }
-
-// The choice of all tokens and the pairs sorted by expert, then token, by one workgroup: a mask of tokens for each
-// expert, whose counts say where its pairs start.
-__global__ __launch_bounds__(1024) void moe_route_kernel(MoeArgs m) {
-  const MxMoeArgs& a = m.a;
-  __shared__ unsigned long long mask[kMoeMaxExperts];
-  __shared__ uint32_t first[kMoeMaxExperts], sums[16][2];
-  __shared__ int16_t chosen[kTokens * kMoeMaxTopK];
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  mask[threadIdx.x] = 0;
-  __syncthreads();
-  for (uint32_t t = wave; t < a.tokens; t += 16) {
-    const Chosen c = choose(m, t);
-    if (lane < a.top_k) {
-      chosen[t * a.top_k + lane] = c.masked ? -1 : (int16_t)c.expert;
-      if (!c.masked) atomicOr(&mask[c.expert], 1ull << t);
-    }
-  }
-  __syncthreads();
-  // running sums over the experts: of their pairs, and of those that have any
-  const uint32_t count = __popcll(mask[threadIdx.x]);
-  uint32_t pairs = count, actives = count ? 1 : 0;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t p = __shfl_up(pairs, d, 64), q = __shfl_up(actives, d, 64);
-    if (lane >= (uint32_t)d) pairs += p, actives += q;
-  }
-  if (lane == 63) sums[wave][0] = pairs, sums[wave][1] = actives;
-  __syncthreads();
-  for (uint32_t w = 0; w < wave; ++w) pairs += sums[w][0], actives += sums[w][1];
-  first[threadIdx.x] = pairs - count;
-  if (count) {
-    const uint64_t to = m.p.active + (uint64_t)(actives - 1) * sizeof(Active);
-    st16(to, u32x4_make(threadIdx.x, pairs - count, count, 0));
-  }
-  if (threadIdx.x == 1023) g_st<uint32_t>(m.p.actives, actives);
-  __syncthreads();
-  for (uint32_t p = threadIdx.x; p < a.tokens * a.top_k; p += 1024) {
-    const int e = chosen[p];
-    int32_t at = -1;
-    if (e >= 0) {
-      at = (int32_t)(first[e] + __popcll(mask[e] & ((1ull << p / a.top_k) - 1)));
-      g_st<int32_t>(m.p.order + (uint64_t)at * 4, (int32_t)p);
-    }
-    g_st<int32_t>(m.p.place + (uint64_t)p * 4, at);
-  }
+__device__ __forceinline__ Chosen choose(const MoeArgs& m, uint32_t t) {
+  if (m.a.experts <= 64) return choose_of<1>(m, t);
+  if (m.a.experts <= 256) return choose_of<4>(m, t);
+  return choose_of<kMoeMaxExperts / 64>(m, t);
+}
+__device__ __forceinline__ void store_choice(const MoeArgs& m, uint32_t t, const Chosen& c) {
+  const uint32_t lane = threadIdx.x & 63;
+  if (lane >= m.a.top_k) return;
+  const uint64_t at = (uint64_t)t * m.a.top_k + lane;
+  g_st<int32_t>(m.p.chosen + at * 4, c.expert);
+  g_st<float>(m.p.weights + at * 4, c.weight);
+  if (m.a.experts_out) g_st<int32_t>(m.a.experts_out + at * 4, c.reported);
+  if (m.a.weights_out) g_st<float>(m.a.weights_out + at * 4, c.weight);
 }
 
-// Rows of one expert's products for its tokens.  WR wavefronts hold 16 rows of
-// gate and of up each (INNER), or 32 rows of down, and share the columns; KG
-// groups of them take turns in steps of 256 values along the rows and add up in
-// LDS at the end.  ONE: the call has one token; its outer products add up over
-// all its experts at once, 16 rows a workgroup.
+__global__ __launch_bounds__(64) void moe_route_kernel(MoeArgs m) { store_choice(m, blockIdx.x, choose(m, blockIdx.x)); }
+
+// Pairs whose experts the inner products' workgroups choose for themselves, each all of them.
+constexpr uint32_t kFusedPairs = 32;
+
+// Rows of one expert's products for its tokens (or, ALL, of the outer products
+// of all experts of up to 64 pairs, weighted and added up).  WR wavefronts hold
+// 16 * RP rows each, of gate and up (INNER) or of down, and share the columns;
+// KG groups of them take turns in steps of 256 values along the rows and add up
+// in LDS at the end.
 //
 // Codes, scales and columns go through LDS by DMA, NS - 1 steps ahead: the
 // matrix instruction's order, a row a lane, would cost the address unit a cycle
 // a lane, and the requests need no registers.  A wavefront's codes and scales
-// are its own; the columns of a group are loaded by all of it.  16-byte chunks of a row of
-// codes (8) or of a column (32) lie at chunk ^ (row / 2 % 8) and chunk ^ (column
-// % 16), so that the 16 lanes that read together meet every bank once.  In a
-// product lane l takes block l / 16 of row (column) l % 16, values 8f .. 8f+7
-// with product f of four.
+// are its own; the columns of a group are loaded by all of it.  16-byte chunks
+// of a row of codes (8) or of a column (32) lie at chunk ^ (row / 2 % 8) and
+// chunk ^ (column % 16), so that the 16 lanes that read together meet every bank
+// once.  In a product lane l takes block l / 16 of row (column) l % 16, values
+// 8f .. 8f+7 with product f of four.
 //
 // kDma 2: codes lie at multiples of 16 bytes and scales of 4, whole words of
 // four blocks; 1: codes only, scales are loaded to registers a step ahead, which
 // waits for all that is on its way; 0: codes go through registers too.
-template <bool INNER, bool ONE, int WR, int KG, int XC, int NS, int kDma>
+template <bool INNER, bool ALL, int WR, int KG, int RP, int XC, int NS, int kDma>
 __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
   static_assert(WR == 1 || KG == 1, "groups of several wavefronts meet at barriers of the whole workgroup");
-  constexpr bool kAll = ONE && !INNER;                // over all experts
-  constexpr int RP = INNER || ONE ? 1 : 2;            // 16s of rows of a matrix
-  constexpr int M = INNER ? 2 : 1, RT = M * RP;       // matrices, 16s of rows
+  static_assert(!(INNER && ALL) && (!INNER || RP == 1) && (!ALL || XC <= 16), "one group of columns for all tokens");
+  constexpr int M = INNER ? 2 : 1, RT = M * RP;               // matrices, 16s of rows
   constexpr int NC = (XC + 15) / 16, CW = XC < 16 ? XC : 16;  // groups of columns, columns of one
   constexpr uint32_t G = 64 * WR, kRows = 16 * RP * WR;
   constexpr uint32_t kCodes = RT * 128, kColumns = XC * 32;  // chunks of a stage
   constexpr int JW = kCodes / 64, JX = kColumns / G, N = JX + (kDma > 0 ? JW : 0) + (kDma == 2 ? 1 : 0);
-  static_assert(kColumns % G == 0 && (NS - 2) * N < 64, "whole requests, and a wait that counts them");
+  static_assert(kColumns % G == 0 && RT <= 2 && (NS - 2) * N < 64, "whole requests, and a wait that counts them");
   __shared__ u32x4 columns[KG * NS * kColumns], codes[KG * WR * NS * kCodes];
   __shared__ uint32_t scales[KG * WR * NS * 64];
-  __shared__ int32_t list[kAll ? 2 * kMoeMaxTopK : 1];  // the experts that take part and their slots
+  __shared__ int32_t list[64], table[ALL ? 64 * CW : 1], fused[INNER ? kFusedPairs : 1];
+  __shared__ float weights[ALL ? 64 : 1];
   const MxMoeArgs& a = m.a;
   const uint32_t lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+  const uint64_t below = (1ull << lane) - 1;  // lanes
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t group = wave / WR, wr = wave % WR, gi = wr * 64 + lane;
   const uint32_t rows = INNER ? a.inner : a.cols, length = INNER ? a.cols : a.inner, blocks = length / kMxBlock;
   const uint32_t x_len = INNER ? m.p.x_len : m.p.h_len, steps = x_len / kStep;
   const uint32_t tiles = ((INNER ? m.p.h_len : rows) + kRows - 1) / kRows;
   const uint32_t slot = blockIdx.x / tiles, n0 = blockIdx.x % tiles * kRows;
-  const uint32_t parts = INNER ? parts_of(a.x_type) : inner_parts(a.out_type);
-  // the expert and its tokens
-  Active item{0, 0, 1, 0};
-  uint32_t units = steps;
-  uint32_t experts = 0;  // that take part (kAll); lane k holds the k-th and its slot
-  int32_t expert_k = 0, slot_k = 0;
-  if constexpr (kAll) {
-    const int32_t e = lane < a.top_k ? g_ld<int32_t>(m.p.chosen + lane * 4) : -1;
-    const uint64_t in = __ballot(e >= 0);
-    experts = __popcll(in);
-    const uint32_t k = __popcll(in & ((1ull << lane) - 1));
-    if (e >= 0) list[2 * k] = e, list[2 * k + 1] = (int32_t)lane;  // the same by every wavefront
-    __syncthreads();
-    if (lane < experts) expert_k = list[2 * lane], slot_k = list[2 * lane + 1];
-    units = experts * steps;
-  } else if constexpr (ONE) {
-    if (slot + 1 == a.top_k && n0 == 0) {
-      // of all wavefronts that choose, these also write the choice
-      const Chosen c = choose(m, 0);
-      item.expert = (uint32_t)__builtin_amdgcn_readlane((int)c.expert, (int)slot);
-      if (__builtin_amdgcn_readlane((int)c.masked, (int)slot)) return;
-    } else {
-      Choice c(m, 0);
-      for (uint32_t k = 0; k <= slot; ++k) item.expert = c.next(a.experts);
-      if (logit_of(c.best) == -__builtin_inf()) return;
+  const uint32_t parts = INNER ? parts_of(a.x_type) : inner_parts(a.out_type), each = CW / parts;  // tokens of CW columns
+  const uint32_t pairs = (uint32_t)a.tokens * a.top_k;
+
+  // The expert and the pairs that chose it (every wavefront writes the same to LDS); ALL: the experts that any pair
+  // chose, lane k holding the k-th, and for each the pairs of the tokens, -1 without one.
+  uint32_t e0 = 0, count = (uint32_t)a.tokens, experts = 0;
+  int32_t expert_k = 0;
+  if constexpr (ALL) {
+    const bool in = lane < pairs;
+    const int32_t e = in ? g_ld<int32_t>(m.p.chosen + lane * 4) : -1;
+    if (in) weights[lane] = g_ld<float>(m.p.weights + lane * 4);
+    uint32_t leader = lane;  // the first pair of the same expert
+    if (a.tokens > 1) {
+      for (uint32_t p = pairs; p-- > 0;)
+        if (__builtin_amdgcn_readlane(e, (int)p) == e && p < leader) leader = p;
     }
-    item.first = slot;
+    const uint64_t leaders = __ballot(e >= 0 && leader == lane);
+    experts = __popcll(leaders);
+    for (uint32_t k = lane; k < experts * CW; k += 64) table[k] = -1;
+    if (e >= 0) {
+      const uint32_t k = __popcll(leaders & ((1ull << leader) - 1));
+      table[k * CW + lane / a.top_k] = (int32_t)lane;
+      if (leader == lane) list[k] = e;
+    }
+    __syncthreads();
+    if (lane < experts) expert_k = list[lane];
   } else {
-    if (slot >= g_ld<uint32_t>(m.p.actives)) return;
-    const u32x4 v = ld16(m.p.active + (uint64_t)slot * sizeof(Active));
-    item = Active{v[0], v[1], v[2], 0};
+    const bool choosing = INNER && pairs <= kFusedPairs;
+    if (choosing) {
+      for (uint32_t t = wave; t < a.tokens; t += WR * KG) {
+        const Chosen c = choose(m, t);
+        if (lane < a.top_k) fused[INNER ? t * a.top_k + lane : 0] = c.expert;
+        if (blockIdx.x == 0) store_choice(m, t, c);
+      }
+      __syncthreads();
+    }
+    auto expert_of = [&](uint32_t p) { return choosing ? fused[INNER ? p : 0] : g_ld<int32_t>(m.p.chosen + p * 4); };
+    // a workgroup an expert, or a pair where there are fewer: the first one of an expert's serves all
+    const bool by_pair = pairs < a.experts;
+    const int32_t e = by_pair ? __builtin_amdgcn_readfirstlane(expert_of(slot)) : (int32_t)slot;
+    if (e < 0) return;
+    count = 0;
+    for (uint32_t p = 0; p < pairs; p += 64) {
+      const bool is = p + lane < pairs && expert_of(p + lane) == e;
+      const uint64_t mask = __ballot(is);
+      if (is) list[count + __popcll(mask & below)] = (int32_t)(p + lane);
+      count += __popcll(mask);
+    }
+    if (count == 0 || (by_pair && list[0] != (int32_t)slot)) return;
+    e0 = (uint32_t)e;
   }
-  const uint32_t e0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)item.expert);
-  const uint32_t first = (uint32_t)__builtin_amdgcn_readfirstlane((int)item.first);
-  const uint32_t count = (uint32_t)__builtin_amdgcn_readfirstlane((int)item.count);
+  const uint32_t units = ALL ? experts * steps : steps;
 
   // Rows past the last one take its place; their sums are not stored, or as zeros.
-  uint64_t w_at[JW], s_at;
+  uint64_t w_at[JW], s_at, byte_at[RT];  // codes, words of scales, the scales of the lane's row in a product
   auto matrix = [&](int r) -> const MxExperts& { return INNER ? (r ? a.up : a.gate) : a.down; };
   auto row_of = [&](int r, uint32_t in) { return min(n0 + (wr * RP + (INNER ? 0 : r)) * 16 + in, rows - 1); };
+  auto scales_of = [&](int r, uint32_t n) {
+    const MxExperts& w = matrix(r);
+    return w.scales.ptr + e0 * w.scales_expert + n * w.scales.stride;
+  };
 #pragma unroll
   for (int j = 0; j < JW; ++j) {
     const MxExperts& w = matrix(j / 2);
-    w_at[j] = w.codes.ptr + (kAll ? 0 : e0 * w.codes_expert) + row_of(j / 2, j % 2 * 8 + lane / 8) * w.codes.stride;
+    w_at[j] = w.codes.ptr + e0 * w.codes_expert + row_of(j / 2, j % 2 * 8 + lane / 8) * w.codes.stride;
   }
-  {
-    const int r = RT == 2 && lane >= 32;
-    const uint32_t n = row_of(r, lane / 2 % 16);
-    s_at = r == 0 ? matrix(0).scales.ptr + (kAll ? 0 : e0 * matrix(0).scales_expert) + n * matrix(0).scales.stride
-                  : matrix(1).scales.ptr + (kAll ? 0 : e0 * matrix(1).scales_expert) + n * matrix(1).scales.stride;
-  }
-  uint64_t byte_at[RT];  // of the lane's row, for scales by the byte
+  s_at = RT == 2 && lane >= 32 ? scales_of(1, row_of(1, lane / 2 % 16)) : scales_of(0, row_of(0, lane / 2 % 16));
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const MxExperts& w = matrix(r);
-    byte_at[r] = w.scales.ptr + (kAll ? 0 : e0 * w.scales_expert) + row_of(r, i) * w.scales.stride;
-  }
+  for (int r = 0; r < RT; ++r) byte_at[r] = scales_of(r, row_of(r, i));
   const uint32_t columns_at = lds_address(columns) + group * (NS * kColumns * 16);
   const uint32_t codes_at = lds_address(codes) + wave * (NS * kCodes * 16);
   const uint32_t words_at = lds_address(scales) + wave * (NS * 64 * 4);
 
-  const uint32_t each = CW / parts;  // tokens of a group of columns
   for (uint32_t t0 = 0; t0 < count; t0 += each * NC) {
     const uint32_t tokens = min(count - t0, each * NC);
     // A lane's chunks of the columns: column c holds part c % parts of a token; columns without one repeat the first.
     uint64_t x_at[JX];
+    uint32_t x_token[JX];
 #pragma unroll
     for (int j = 0; j < JX; ++j) {
       const uint32_t column = (j * G + gi) / 32, c = column % CW;
       uint32_t t = column / CW * each + c / parts, part = c % parts;
       if (c >= each * parts || t >= tokens) t = 0, part = 0;
-      uint64_t row = first + t0 + t;
-      if constexpr (INNER) row = ONE ? 0 : (uint32_t)g_ld<int32_t>(m.p.order + row * 4) / a.top_k;
       const uint32_t chunk = (gi & 31) ^ (column & 15);
-      x_at[j] = (INNER ? m.p.x + (part * a.tokens + row) * x_len * 2
-                       : m.p.h + (part * a.tokens * a.top_k + (kAll ? 0 : row)) * x_len * 2) + chunk * 16;
+      x_token[j] = t;
+      uint64_t row = part * pairs;
+      if constexpr (!ALL) {
+        const uint32_t pair = (uint32_t)list[t0 + t];
+        row = INNER ? part * (uint32_t)a.tokens + pair / a.top_k : part * pairs + pair;
+      }
+      x_at[j] = (INNER ? m.p.x : m.p.h) + row * x_len * 2 + chunk * 16;
     }
     // Where along its way a group is: a step, of the k-th expert.
     struct Unit {
@@ -417,12 +371,11 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
     };
     auto forward = [&](Unit& u) {
       u.step += KG;
-      while (kAll && u.step >= steps) u.step -= steps, ++u.k;
+      while (ALL && u.step >= steps) u.step -= steps, ++u.k;
     };
     auto expert_of = [&](const Unit& u) { return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(expert_k, (int)u.k); };
-    auto slot_of = [&](const Unit& u) { return (uint32_t)__builtin_amdgcn_readlane(slot_k, (int)u.k); };
     auto request = [&](const Unit& u, uint32_t stage) {
-      const uint64_t e = kAll ? expert_of(u) : 0;
+      const uint64_t e = ALL ? expert_of(u) : 0;
 #pragma unroll
       for (int j = 0; j < JW; ++j) {
         const uint32_t chunk = (lane & 7) ^ (j * 4 + (lane >> 4) & 7);
@@ -433,24 +386,29 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
           ((LdsChunks)(codes_at + (stage * kCodes + lane) * 16))[j * 64] = ld16(from);
       }
       if constexpr (kDma == 2)
-        dma4(s_at + e * a.down.scales_expert + min(u.step * 2 + (lane & 1), blocks / 4 - 1) * 4,
-             words_at + stage * 256);
+        dma4(s_at + e * a.down.scales_expert + min(u.step * 2 + (lane & 1), blocks / 4 - 1) * 4, words_at + stage * 256);
 #pragma unroll
-      for (int j = 0; j < JX; ++j)
-        dma16(x_at[j] + (kAll ? (uint64_t)slot_of(u) * x_len * 2 : 0) + u.step * (kStep * 2),
-              columns_at + (stage * kColumns + j * G + wr * 64) * 16);
+      for (int j = 0; j < JX; ++j) {
+        uint64_t from = x_at[j] + u.step * (kStep * 2);
+        if constexpr (ALL) {
+          // a token that did not choose the expert has another's h here, whose sums are left out
+          const int32_t pair = table[u.k * CW + x_token[j]];
+          from += (uint64_t)(uint32_t)max(pair, 0) * x_len * 2;
+        }
+        dma16(from, columns_at + (stage * kColumns + j * G + wr * 64) * 16);
+      }
     };
     uint32_t bytes[RT][2] = {}, bytes_next[RT][2] = {};
     auto load_bytes = [&](const Unit& u) {
-      const uint64_t e = kAll ? expert_of(u) : 0;
+      const uint64_t e = ALL ? expert_of(u) : 0;
 #pragma unroll
       for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int s = 0; s < 2; ++s)
-          bytes_next[r][s] = g_ld<uint8_t>(byte_at[r] + e * a.down.scales_expert +
-                                           min(u.step * 8 + s * 4 + q, blocks - 1));
+          bytes_next[r][s] =
+              g_ld<uint8_t>(byte_at[r] + e * a.down.scales_expert + min(u.step * 8 + s * 4 + q, blocks - 1));
     };
-    f32x4 acc[RT][NC] = {}, total[kAll ? RT : 1][NC] = {};
+    f32x4 acc[RT][NC] = {}, total[ALL ? RT : 1][NC] = {};
     auto compute = [&](uint32_t stage) {
       u32x2 words[RT];
       if constexpr (kDma == 2) {
@@ -484,18 +442,22 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
         }
       }
     };
-    auto add_expert = [&](uint32_t k) {  // an expert's sums, weighted
-      const float weight = g_ld<float>(m.p.weights + k * 4);
+    auto add_expert = [&](uint32_t k) {  // an expert's sums, weighted, for the tokens that chose it
+      const uint32_t c = i % CW, t = c / parts;
+      const int32_t pair = c < each * parts && t < tokens ? table[ALL ? k * CW + t : 0] : -1;
+      const float weight = weights[ALL ? max(pair, 0) : 0];
 #pragma unroll
-      for (int r = 0; r < (kAll ? RT : 1); ++r)
-#pragma unroll
-        for (int c = 0; c < NC; ++c) total[r][c] += weight * acc[r][c], acc[r][c] = f32x4{};
+      for (int r = 0; r < (ALL ? RT : 1); ++r) {
+        const f32x4 more = total[r][0] + weight * acc[r][0];
+        total[r][0] = pair >= 0 ? more : total[r][0];
+        acc[r][0] = f32x4{};
+      }
     };
     const uint32_t n = group < units ? (units - group + KG - 1) / KG : 0;  // of this group
     if (t0) __syncthreads();  // before LDS is used again
     if (n) {
       Unit now{group, 0};
-      while (kAll && now.step >= steps) now.step -= steps, ++now.k;
+      while (ALL && now.step >= steps) now.step -= steps, ++now.k;
       if constexpr (kDma < 2) load_bytes(now);
       Unit ahead = now;  // the next one to be requested
 #pragma unroll
@@ -523,11 +485,11 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
         }
         if (k + NS - 1 < n) {
           request(ahead, into);
-          forward(ahead);
+          if (k + NS < n) forward(ahead);
         }
         compute(stage);
-        if constexpr (kAll) {
-          if (k + 1 == n || next.k != now.k) add_expert(slot_of(now));
+        if constexpr (ALL) {
+          if (k + 1 == n || next.k != now.k) add_expert(now.k);
         }
         now = next;
         stage = stage + 1 == NS ? 0 : stage + 1, into = into + 1 == NS ? 0 : into + 1;
@@ -540,7 +502,7 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
-      for (int c = 0; c < NC; ++c) sums[((wave * RT + r) * NC + c) * 64 + lane] = kAll ? total[kAll ? r : 0][c] : acc[r][c];
+      for (int c = 0; c < NC; ++c) sums[((wave * RT + r) * NC + c) * 64 + lane] = ALL ? total[ALL ? r : 0][c] : acc[r][c];
     __syncthreads();
     // of 16s `r` of wavefront w of a group, row `in`, token t: over its parts and the groups
     auto sum_of = [&](uint32_t w, uint32_t r, uint32_t in, uint32_t t) {
@@ -553,14 +515,14 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
       return v;
     };
     for (uint32_t at = threadIdx.x; at < tokens * kRows; at += 64 * WR * KG) {
-      const uint32_t t = at / kRows, in = at % kRows, w = in / (16 * RP), rp = in / 16 % RP, nn = n0 + in;
-      const uint64_t row = first + t0 + t;
+      const uint32_t t = at / kRows, in = at % kRows, w = in / (16 * RP), rp = in / 16 % RP, n = n0 + in;
+      const uint64_t pair = ALL ? 0 : (uint32_t)list[t0 + t];
       if constexpr (INNER) {
-        if (nn >= m.p.h_len) continue;
+        if (n >= m.p.h_len) continue;
         float h = 0;
-        if (nn < a.inner) {
-          const float g = sum_of(w, 0, in % 16, t) + bias_of(a.gate, a.out_type, e0, nn);
-          const float u = sum_of(w, 1, in % 16, t) + bias_of(a.up, a.out_type, e0, nn);
+        if (n < a.inner) {
+          const float g = sum_of(w, 0, in % 16, t) + bias_of(a.gate, a.out_type, e0, n);
+          const float u = sum_of(w, 1, in % 16, t) + bias_of(a.up, a.out_type, e0, n);
           h = g / (1.0f + expf(-g)) * u;
         }
         // parts as x's, but for the last, which is rounded
@@ -574,16 +536,18 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
           } else {
             b = (uint16_t)pack2<kTypeBf16>(h, 0.0f);
           }
-          g_st<uint16_t>(m.p.h + ((p * a.tokens * a.top_k + row) * m.p.h_len + nn) * 2, b);
+          g_st<uint16_t>(m.p.h + (((uint64_t)p * pairs + pair) * m.p.h_len + n) * 2, b);
         }
-      } else if (nn < rows) {
+      } else if (n < rows) {
         float v = sum_of(w, rp, in % 16, t);
-        if constexpr (kAll) {
-          for (uint32_t k = 0; a.down.bias && k < experts; ++k)
-            v += g_ld<float>(m.p.weights + list[2 * k + 1] * 4) * bias_of(a.down, a.out_type, (uint32_t)list[2 * k], nn);
-          store1_as(a.out_type, a.out.ptr, nn, v);
+        if constexpr (ALL) {
+          for (uint32_t k = 0; a.down.bias && k < experts; ++k) {
+            const int32_t pair = table[k * CW + t];
+            if (pair >= 0) v += weights[pair] * bias_of(a.down, a.out_type, (uint32_t)list[k], n);
+          }
+          store1_as(a.out_type, a.out.ptr, t * a.out.stride + n, v);
         } else {
-          g_st<float>(m.p.y + (row * rows + nn) * 4, v + bias_of(a.down, a.out_type, e0, nn));
+          g_st<float>(m.p.y + (pair * rows + n) * 4, v + bias_of(a.down, a.out_type, e0, n));
         }
       }
     }
@@ -598,8 +562,8 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs m) {
   f32x4 v = {};
   for (uint32_t k = 0; k < a.top_k; ++k) {
     const uint64_t pair = (uint64_t)t * a.top_k + k;
-    const int32_t row = g_ld<int32_t>(m.p.place + pair * 4);
-    if (row >= 0) v += g_ld<float>(m.p.weights + pair * 4) * __builtin_bit_cast(f32x4, ld16(m.p.y + ((uint64_t)row * a.cols + n) * 4));
+    if (g_ld<int32_t>(m.p.chosen + pair * 4) >= 0)
+      v += g_ld<float>(m.p.weights + pair * 4) * __builtin_bit_cast(f32x4, ld16(m.p.y + (pair * a.cols + n) * 4));
   }
   const uint64_t to = t * a.out.stride + n;
   if (a.out_type == kTypeBf16)
@@ -619,14 +583,14 @@ int dma_of(const MxExperts& w, uint32_t length, uint64_t experts) {
   return length % 128 == 0 && at(w.scales, w.scales_expert, 4) ? 2 : 1;
 }
 
-template <bool INNER, bool ONE, int WR, int KG, int XC, int NS>
+template <bool INNER, bool ALL, int WR, int KG, int RP, int XC, int NS>
 hipError_t product_of(const MoeArgs& m, int dma, hipStream_t stream) {
-  constexpr uint32_t kRows = 16 * (INNER || ONE ? 1 : 2) * WR;
+  constexpr uint32_t kRows = 16 * RP * WR;
   const uint64_t tiles = ((INNER ? m.p.h_len : m.a.cols) + kRows - 1) / kRows, pairs = m.a.tokens * m.a.top_k;
-  const uint64_t items = ONE ? (INNER ? m.a.top_k : 1) : pairs < m.a.experts ? pairs : m.a.experts;
-  return launch(dma == 2   ? moe_product_kernel<INNER, ONE, WR, KG, XC, NS, 2>
-                : dma == 1 ? moe_product_kernel<INNER, ONE, WR, KG, XC, NS, 1>
-                           : moe_product_kernel<INNER, ONE, WR, KG, XC, NS, 0>,
+  const uint64_t items = ALL ? 1 : pairs < m.a.experts ? pairs : m.a.experts;
+  return launch(dma == 2   ? moe_product_kernel<INNER, ALL, WR, KG, RP, XC, NS, 2>
+                : dma == 1 ? moe_product_kernel<INNER, ALL, WR, KG, RP, XC, NS, 1>
+                           : moe_product_kernel<INNER, ALL, WR, KG, RP, XC, NS, 0>,
                 items * tiles, 64 * WR * KG, m, stream);
 }
 
@@ -654,14 +618,29 @@ hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
     if (a.experts_out) m.a.experts_out += first * a.top_k * 4;
     if (a.weights_out) m.a.weights_out += first * a.top_k * 4;
     hipError_t e = logits_of(m, stream);
-    if (tokens == 1) {
-      if (e == hipSuccess) e = product_of<true, true, 1, 4, 4, 3>(m, inner, stream);
-      if (e == hipSuccess) e = product_of<false, true, 1, 8, 4, 4>(m, outer, stream);
-      return e;
-    }
-    if (e == hipSuccess) e = launch(moe_route_kernel, 1, 1024, m, stream);
-    if (e == hipSuccess) e = product_of<true, false, 4, 1, 16, 3>(m, inner, stream);
-    if (e == hipSuccess) e = product_of<false, false, 4, 1, 16, 3>(m, outer, stream);
+    const uint64_t pairs = tokens * a.top_k;
+    const uint32_t xp = parts_of(a.x_type), hp = inner_parts(a.out_type);
+    if (e == hipSuccess && pairs > kFusedPairs) e = launch(moe_route_kernel, tokens, 64, m, stream);
+    if (e != hipSuccess) return e;
+    // columns that an expert's tokens take on average
+    const double inner_columns = (double)pairs / a.experts * xp, outer_columns = (double)pairs / a.experts * hp;
+    if (tokens * xp <= 4)
+      e = product_of<true, false, 1, 4, 1, 4, 3>(m, inner, stream);
+    else if (tokens * xp <= 16 || inner_columns <= 8)
+      e = product_of<true, false, 4, 1, 1, 16, 3>(m, inner, stream);
+    else if (inner_columns <= 20)
+      e = product_of<true, false, 4, 1, 1, 32, 2>(m, inner, stream);
+    else
+      e = product_of<true, false, 4, 1, 1, 64, 2>(m, inner, stream);
+    if (e != hipSuccess) return e;
+    if (tokens * hp <= 4 && pairs <= 64) return product_of<false, true, 1, 8, 1, 4, 4>(m, outer, stream);
+    if (tokens <= 16 / hp && pairs <= 64) return product_of<false, true, 1, 4, 1, 16, 3>(m, outer, stream);
+    if (tokens * hp <= 16 || outer_columns <= 8)
+      e = product_of<false, false, 4, 1, 2, 16, 3>(m, outer, stream);
+    else if (outer_columns <= 20)
+      e = product_of<false, false, 4, 1, 2, 32, 2>(m, outer, stream);
+    else
+      e = product_of<false, false, 4, 1, 2, 64, 2>(m, outer, stream);
     if (e == hipSuccess) e = launch(moe_combine_kernel, (tokens * (a.cols / 4) + 255) / 256, 256, m, stream);
     return e;
   });
