@@ -87,7 +87,8 @@ __device__ __forceinline__ GlobalBytes uniform(uint64_t a) {
 }
 
 // DMA of 16 bytes a lane from a uniform address and the lane's offset to consecutive places in LDS from `to` (uniform)
-// on.  Written out, because the compiler waits for all that is on its way before it reads LDS.  Nothing but a wait on vmcnt says that the bytes have come.
+// on.  Written out, because the compiler waits for all that is on its way before it reads LDS.  Nothing but a wait on
+// vmcnt says that the bytes have come.
 __device__ __forceinline__ void dma16(GlobalBytes from, uint32_t offset, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(from)
                : "memory", "m0");
@@ -99,10 +100,14 @@ __device__ __forceinline__ void dma16(uint64_t from, uint32_t to) {  // from the
 __device__ __forceinline__ void dma4(uint64_t from, uint32_t to) {  // 4 bytes a lane, from multiples of 4
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "memory", "m0");
 }
+__device__ __forceinline__ void dma1(uint64_t from, uint32_t to) {  // a byte a lane, to words
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off" ::"s"(to), "v"(from) : "memory", "m0");
+}
 
 // LDS by its byte address, which takes a known offset along in the instruction.
 typedef __attribute__((address_space(3))) u32x4* LdsChunks;
 typedef __attribute__((address_space(3))) u32x2* LdsPairs;
+typedef __attribute__((address_space(3))) uint32_t* LdsWord;
 template <typename T>
 __device__ __forceinline__ uint32_t lds_address(T* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) T*)p;

@@ -20,6 +20,8 @@
 // whatever the types, and few tokens in two parts cost no more than in one.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "mx_device.h"
 
 namespace ptwm {
@@ -91,18 +93,19 @@ __device__ __forceinline__ float bias_of(const MxExperts& w, uint32_t type, uint
   return w.bias ? load1_as(type, w.bias, e * w.bias_expert + n * w.bias_stride) : 0.0f;
 }
 
-// Logits of one expert and four tokens: 256 threads take turns along the rows.  Summed in 64 bits, in which products
+// Logits of one expert and four tokens: the threads take turns along the rows.  Summed in 64 bits, in which products
 // are exact, so that which of two near experts is chosen does not depend on the order of the additions.  The
 // workgroups after these write x's parts, a token each.
 constexpr uint32_t kLogitTokens = 4;
+constexpr uint32_t kLogitThreads = 512;
 template <uint32_t T>
-__global__ __launch_bounds__(256) void moe_logits_kernel(MoeArgs m) {
+__global__ __launch_bounds__(kLogitThreads) void moe_logits_kernel(MoeArgs m) {
   const MxMoeArgs& a = m.a;
-  __shared__ double part[kLogitTokens][256];
+  __shared__ double part[kLogitTokens][kLogitThreads];
   const uint32_t groups = ((uint32_t)a.tokens + kLogitTokens - 1) / kLogitTokens;
   if (blockIdx.x >= a.experts * groups) {
     const uint32_t t = blockIdx.x - a.experts * groups;
-    for (uint32_t k = threadIdx.x * 8; k < m.p.x_len; k += 256 * 8) {
+    for (uint32_t k = threadIdx.x * 8; k < m.p.x_len; k += kLogitThreads * 8) {
       u32x4 p[parts_of(T)] = {};
       if (k < a.cols) parts_of_raw<T>(load_raw8<T>(a.x.ptr + (t * a.x.stride + k) * type_bytes(T)), 1.0f, p);
 #pragma unroll
@@ -112,7 +115,7 @@ __global__ __launch_bounds__(256) void moe_logits_kernel(MoeArgs m) {
   }
   const uint32_t e = blockIdx.x / groups, t0 = blockIdx.x % groups * kLogitTokens;
   double sum[kLogitTokens] = {};
-  for (uint32_t k = threadIdx.x * 8; k < a.cols; k += 256 * 8) {
+  for (uint32_t k = threadIdx.x * 8; k < a.cols; k += kLogitThreads * 8) {
     float r[8], x[kLogitTokens][8];
     load8_as(a.router_type, a.router.ptr, e * a.router.stride + k, r);
 #pragma unroll
@@ -127,9 +130,11 @@ __global__ __launch_bounds__(256) void moe_logits_kernel(MoeArgs m) {
 #pragma unroll
   for (uint32_t t = 0; t < kLogitTokens; ++t) part[t][threadIdx.x] = sum[t];
   __syncthreads();
-  const uint32_t t = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  if (t0 + t >= a.tokens) return;
-  double v = (part[t][lane] + part[t][lane + 64]) + (part[t][lane + 128] + part[t][lane + 192]);
+  const uint32_t t = threadIdx.x >> 6, lane = threadIdx.x & 63;  // a wavefront a token
+  if (t >= kLogitTokens || t0 + t >= a.tokens) return;
+  double v = 0;
+#pragma unroll
+  for (uint32_t k = 0; k < kLogitThreads; k += 64) v += part[t][k + lane];
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
   if (lane == 0) {
@@ -150,18 +155,13 @@ __device__ __forceinline__ double logit_of(uint64_t order) {
 
 // The largest of a wavefront's values, in all lanes.
 template <int CTRL>
-__device__ __forceinline__ uint64_t larger_by(uint64_t v) {
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, 0xF, 0xF, false);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, 0xF, 0xF, false);
-  const uint64_t other = lo | (uint64_t)hi << 32;
-  return other > v ? other : v;
+__device__ __forceinline__ uint32_t larger_by(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false));
 }
-__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
   v = larger_by<0x111>(v), v = larger_by<0x112>(v), v = larger_by<0x114>(v), v = larger_by<0x118>(v);  // in rows of 16
   v = larger_by<0x142>(v), v = larger_by<0x143>(v);  // a row's last lane to the next rows
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), 63);
-  return lo | (uint64_t)hi << 32;
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // Chooses a token's experts: the largest that is left, the lowest expert of equal ones.  One wavefront, N logits a
@@ -186,18 +186,29 @@ __device__ __forceinline__ Chosen choose_of(const MoeArgs& m, uint32_t t) {
     uint64_t most = key[0];
 #pragma unroll
     for (uint32_t j = 1; j < N; ++j) most = key[j] > most ? key[j] : most;
-    const uint64_t best = wave_max(most);
-    uint32_t e = 0;
-    bool found = false;
-#pragma unroll
-    for (uint32_t j = 0; j < N; ++j) {
-      const uint64_t at = __ballot(key[j] == best);
-      if (found || !at) continue;
-      found = true;
-      const uint32_t owner = (uint32_t)__ffsll((long long)at) - 1;
-      e = j * 64 + owner;
-      if (lane == owner) key[j] = 0;
+    // by the upper halves, and by the lower ones where several lanes have the same
+    const uint32_t upper = (uint32_t)(most >> 32), high = wave_max(upper);
+    uint64_t at = __ballot(upper == high);
+    uint32_t owner = (uint32_t)__ffsll((long long)at) - 1, low = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)most, (int)owner);
+    if (at & (at - 1)) {
+      low = wave_max(upper == high ? (uint32_t)most : 0);
+      at = __ballot(upper == high && (uint32_t)most == low);
     }
+    const uint64_t best = low | (uint64_t)high << 32;
+    uint32_t j0 = 0;  // the lane's first with that logit
+#pragma unroll
+    for (uint32_t j = N; j-- > 0;)
+      if (key[j] == best) j0 = j;
+    if (at & (at - 1)) {  // of several lanes the one whose expert is the lowest
+#pragma unroll
+      for (uint32_t j = N; j-- > 0;)
+        if (const uint64_t with = __ballot(key[j] == best)) at = with;
+    }
+    owner = (uint32_t)__ffsll((long long)at) - 1;
+    const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)j0, (int)owner), e = first * 64 + owner;
+#pragma unroll
+    for (uint32_t j = 0; j < N; ++j)
+      if (lane == owner && j == first) key[j] = 0;
     if (k == 0) top = best;
     if (k == lane) mine.reported = (int32_t)e, own = best;
   }
@@ -214,7 +225,7 @@ __device__ __forceinline__ Chosen choose_of(const MoeArgs& m, uint32_t t) {
 }
 __device__ __forceinline__ Chosen choose(const MoeArgs& m, uint32_t t) {
   if (m.a.experts <= 64) return choose_of<1>(m, t);
-  if (m.a.experts <= 256) return choose_of<4>(m, t);
+  if (m.a.experts <= 128) return choose_of<2>(m, t);
   return choose_of<kMoeMaxExperts / 64>(m, t);
 }
 __device__ __forceinline__ void store_choice(const MoeArgs& m, uint32_t t, const Chosen& c) {
@@ -248,20 +259,22 @@ constexpr uint32_t kFusedPairs = 32;
 // 8f .. 8f+7 with product f of four.
 //
 // kDma 2: codes lie at multiples of 16 bytes and scales of 4, whole words of
-// four blocks; 1: codes only, scales are loaded to registers a step ahead, which
-// waits for all that is on its way; 0: codes go through registers too.
+// four blocks; 1: codes only, scales come byte by byte; 0: codes go through
+// registers.
 template <bool INNER, bool ALL, int WR, int KG, int RP, int XC, int NS, int kDma>
 __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
   static_assert(WR == 1 || KG == 1, "groups of several wavefronts meet at barriers of the whole workgroup");
   static_assert(!(INNER && ALL) && (!INNER || RP == 1) && (!ALL || XC <= 16), "one group of columns for all tokens");
   constexpr int M = INNER ? 2 : 1, RT = M * RP;               // matrices, 16s of rows
   constexpr int NC = (XC + 15) / 16, CW = XC < 16 ? XC : 16;  // groups of columns, columns of one
-  constexpr uint32_t G = 64 * WR, kRows = 16 * RP * WR;
+  constexpr uint32_t G = 64 * WR, kWaves = WR * KG, kRows = 16 * RP * WR;
   constexpr uint32_t kCodes = RT * 128, kColumns = XC * 32;  // chunks of a stage
-  constexpr int JW = kCodes / 64, JX = kColumns / G, N = JX + (kDma > 0 ? JW : 0) + (kDma == 2 ? 1 : 0);
+  constexpr int JW = kCodes / 64, JX = kColumns / G, JS = kDma == 2 ? 1 : 2 * RT;
+  constexpr int N = JX + (kDma > 0 ? JW : 0) + JS;  // requests of a step
+  constexpr uint32_t kScales = JS * 64;                                          // words of a stage
   static_assert(kColumns % G == 0 && RT <= 2 && (NS - 2) * N < 64, "whole requests, and a wait that counts them");
   __shared__ u32x4 columns[KG * NS * kColumns], codes[KG * WR * NS * kCodes];
-  __shared__ uint32_t scales[KG * WR * NS * 64];
+  __shared__ uint32_t scales[KG * WR * NS * kScales];
   __shared__ int32_t list[64], table[ALL ? 64 * CW : 1], fused[INNER ? kFusedPairs : 1];
   __shared__ float weights[ALL ? 64 : 1];
   const MxMoeArgs& a = m.a;
@@ -302,7 +315,7 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
   } else {
     const bool choosing = INNER && pairs <= kFusedPairs;
     if (choosing) {
-      for (uint32_t t = wave; t < a.tokens; t += WR * KG) {
+      for (uint32_t t = wave; t < a.tokens; t += kWaves) {
         const Chosen c = choose(m, t);
         if (lane < a.top_k) fused[INNER ? t * a.top_k + lane : 0] = c.expert;
         if (blockIdx.x == 0) store_choice(m, t, c);
@@ -327,7 +340,7 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
   const uint32_t units = ALL ? experts * steps : steps;
 
   // Rows past the last one take its place; their sums are not stored, or as zeros.
-  uint64_t w_at[JW], s_at, byte_at[RT];  // codes, words of scales, the scales of the lane's row in a product
+  uint64_t w_at[JW], s_at[JS];  // codes and scales
   auto matrix = [&](int r) -> const MxExperts& { return INNER ? (r ? a.up : a.gate) : a.down; };
   auto row_of = [&](int r, uint32_t in) { return min(n0 + (wr * RP + (INNER ? 0 : r)) * 16 + in, rows - 1); };
   auto scales_of = [&](int r, uint32_t n) {
@@ -339,32 +352,37 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
     const MxExperts& w = matrix(j / 2);
     w_at[j] = w.codes.ptr + e0 * w.codes_expert + row_of(j / 2, j % 2 * 8 + lane / 8) * w.codes.stride;
   }
-  s_at = RT == 2 && lane >= 32 ? scales_of(1, row_of(1, lane / 2 % 16)) : scales_of(0, row_of(0, lane / 2 % 16));
+  if constexpr (kDma == 2) {  // two words a row
+    s_at[0] = RT == 2 && lane >= 32 ? scales_of(1, row_of(1, lane / 2 % 16)) : scales_of(0, row_of(0, lane / 2 % 16));
+  } else {  // eight bytes a row
 #pragma unroll
-  for (int r = 0; r < RT; ++r) byte_at[r] = scales_of(r, row_of(r, i));
+    for (int j = 0; j < JS; ++j) s_at[j] = scales_of(j / 2, row_of(j / 2, j % 2 * 8 + lane / 8));
+  }
   const uint32_t columns_at = lds_address(columns) + group * (NS * kColumns * 16);
   const uint32_t codes_at = lds_address(codes) + wave * (NS * kCodes * 16);
-  const uint32_t words_at = lds_address(scales) + wave * (NS * 64 * 4);
+  const uint32_t scales_at = lds_address(scales) + wave * (NS * kScales * 4);
 
   for (uint32_t t0 = 0; t0 < count; t0 += each * NC) {
-    const uint32_t tokens = min(count - t0, each * NC);
-    // A lane's chunks of the columns: column c holds part c % parts of a token; columns without one repeat the first.
-    uint64_t x_at[JX];
-    uint32_t x_token[JX];
+    const uint32_t tokens = min(count - t0, each * NC), used = (tokens + each - 1) / each;  // groups of columns
+    // A lane's chunks of the columns, as offsets: column c holds part c % parts of a token; columns without one repeat
+    // the first.  (2^31 bytes hold 3 parts of 2048 pairs of the longest rows.)
+    uint32_t x_at[JX], x_token[ALL ? JX : 1];
 #pragma unroll
     for (int j = 0; j < JX; ++j) {
       const uint32_t column = (j * G + gi) / 32, c = column % CW;
       uint32_t t = column / CW * each + c / parts, part = c % parts;
       if (c >= each * parts || t >= tokens) t = 0, part = 0;
       const uint32_t chunk = (gi & 31) ^ (column & 15);
-      x_token[j] = t;
-      uint64_t row = part * pairs;
-      if constexpr (!ALL) {
+      uint32_t row = part * pairs;
+      if constexpr (ALL) {
+        x_token[j] = t;
+      } else {
         const uint32_t pair = (uint32_t)list[t0 + t];
         row = INNER ? part * (uint32_t)a.tokens + pair / a.top_k : part * pairs + pair;
       }
-      x_at[j] = (INNER ? m.p.x : m.p.h) + row * x_len * 2 + chunk * 16;
+      x_at[j] = row * x_len * 2 + chunk * 16;
     }
+    const GlobalBytes x0 = global_bytes(INNER ? m.p.x : m.p.h);
     // Where along its way a group is: a step, of the k-th expert.
     struct Unit {
       uint32_t step, k;
@@ -385,61 +403,66 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
         else
           ((LdsChunks)(codes_at + (stage * kCodes + lane) * 16))[j * 64] = ld16(from);
       }
-      if constexpr (kDma == 2)
-        dma4(s_at + e * a.down.scales_expert + min(u.step * 2 + (lane & 1), blocks / 4 - 1) * 4, words_at + stage * 256);
+#pragma unroll
+      for (int j = 0; j < JS; ++j) {
+        const uint64_t from = s_at[j] + e * a.down.scales_expert;
+        const uint32_t to = scales_at + (stage * kScales + j * 64) * 4;
+        if constexpr (kDma == 2)
+          dma4(from + min(u.step * 2 + (lane & 1), blocks / 4 - 1) * 4, to);
+        else
+          dma1(from + min(u.step * 8 + (lane & 7), blocks - 1), to);
+      }
 #pragma unroll
       for (int j = 0; j < JX; ++j) {
-        uint64_t from = x_at[j] + u.step * (kStep * 2);
+        if (NS == 2 && NC > 1 && j * G >= used * 512) break;  // a wait for all needs no count of them
+        uint32_t from = x_at[j] + u.step * (kStep * 2);
         if constexpr (ALL) {
           // a token that did not choose the expert has another's h here, whose sums are left out
           const int32_t pair = table[u.k * CW + x_token[j]];
-          from += (uint64_t)(uint32_t)max(pair, 0) * x_len * 2;
+          from += (uint32_t)max(pair, 0) * x_len * 2;
         }
-        dma16(from, columns_at + (stage * kColumns + j * G + wr * 64) * 16);
+        dma16(x0, from, columns_at + (stage * kColumns + j * G + wr * 64) * 16);
       }
     };
-    uint32_t bytes[RT][2] = {}, bytes_next[RT][2] = {};
-    auto load_bytes = [&](const Unit& u) {
-      const uint64_t e = ALL ? expert_of(u) : 0;
-#pragma unroll
-      for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-          bytes_next[r][s] =
-              g_ld<uint8_t>(byte_at[r] + e * a.down.scales_expert + min(u.step * 8 + s * 4 + q, blocks - 1));
-    };
     f32x4 acc[RT][NC] = {}, total[ALL ? RT : 1][NC] = {};
-    auto compute = [&](uint32_t stage) {
+    auto compute = [&](uint32_t stage, auto used_) {
+      constexpr int used = used_;
       u32x2 words[RT];
       if constexpr (kDma == 2) {
 #pragma unroll
-        for (int r = 0; r < RT; ++r) words[r] = *(LdsPairs)(words_at + stage * 256 + (r * 16 + i) * 8);
+        for (int r = 0; r < RT; ++r) words[r] = *(LdsPairs)(scales_at + stage * (kScales * 4) + (r * 16 + i) * 8);
       }
+      u32x4 wv[2][RT];
+      float sf[2][RT];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        u32x4 wv[RT];
-        float sf[RT];
+      for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
           const uint32_t row = r * 16 + i, c = s * 4 + q;
-          wv[r] = *(LdsChunks)(codes_at + (stage * kCodes + row * 8 + (c ^ (row / 2 & 7))) * 16);
-          sf[r] = scale_f32(kDma == 2 ? words[r][s] >> 8 * q & 0xFF : bytes[r][s]);
+          wv[s][r] = *(LdsChunks)(codes_at + (stage * kCodes + row * 8 + (c ^ (row / 2 & 7))) * 16);
+          sf[s][r] = scale_f32(kDma == 2 ? words[r][s] >> 8 * q & 0xFF
+                                         : *(LdsWord)(scales_at + (stage * kScales + row * 8 + c) * 4));
         }
+      // columns are read a product ahead, and no further: eight products' are more than the registers
+      u32x4 xv[2][used];
+      auto read = [&](int u) {
 #pragma unroll
-        for (int f = 0; f < 4; ++f) {
-          u32x4 xv[NC];
-#pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            const uint32_t column = c * 16 + i % CW, chunk = (s * 4 + q) * 4 + f;
-            xv[c] = *(LdsChunks)(columns_at + (stage * kColumns + column * 32 + (chunk ^ (column & 15))) * 16);
-          }
-#pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            const u32x4 w8 = weights8(wv[r][f], sf[r]);
-#pragma unroll
-            for (int c = 0; c < NC; ++c) acc[r][c] = mfma(w8, xv[c], acc[r][c]);
-          }
+        for (int c = 0; c < used; ++c) {
+          const uint32_t column = c * 16 + i % CW, chunk = (u / 4 * 4 + q) * 4 + u % 4;
+          xv[u & 1][c] = *(LdsChunks)(columns_at + (stage * kColumns + column * 32 + (chunk ^ (column & 15))) * 16);
         }
+      };
+      read(0);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (u < 7) read(u + 1);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const u32x4 w8 = weights8(wv[u / 4][r][u % 4], sf[u / 4][r]);
+#pragma unroll
+          for (int c = 0; c < used; ++c) acc[r][c] = mfma(w8, xv[u & 1][c], acc[r][c]);
+        }
+        if constexpr (used > 2) __builtin_amdgcn_sched_barrier(0);
       }
     };
     auto add_expert = [&](uint32_t k) {  // an expert's sums, weighted, for the tokens that chose it
@@ -458,7 +481,6 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
     if (n) {
       Unit now{group, 0};
       while (ALL && now.step >= steps) now.step -= steps, ++now.k;
-      if constexpr (kDma < 2) load_bytes(now);
       Unit ahead = now;  // the next one to be requested
 #pragma unroll
       for (uint32_t k = 0; k < NS - 1; ++k) {
@@ -478,16 +500,14 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
         asm volatile("" ::: "memory");
         Unit next = now;
         forward(next);
-        if constexpr (kDma < 2) {
-#pragma unroll
-          for (int r = 0; r < RT; ++r) bytes[r][0] = bytes_next[r][0], bytes[r][1] = bytes_next[r][1];
-          if (k + 1 < n) load_bytes(next);
-        }
         if (k + NS - 1 < n) {
           request(ahead, into);
           if (k + NS < n) forward(ahead);
         }
-        compute(stage);
+        if (NC > 1 && used > 1)
+          compute(stage, std::integral_constant<int, NC < 2 ? NC : 2>{});
+        else
+          compute(stage, std::integral_constant<int, 1>{});
         if constexpr (ALL) {
           if (k + 1 == n || next.k != now.k) add_expert(now.k);
         }
@@ -514,7 +534,7 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
           v += sums[(((g * WR + w) * RT + r) * NC + c) * 64 + in / 4 * 16 + column + p][in & 3];
       return v;
     };
-    for (uint32_t at = threadIdx.x; at < tokens * kRows; at += 64 * WR * KG) {
+    for (uint32_t at = threadIdx.x; at < tokens * kRows; at += 64 * kWaves) {
       const uint32_t t = at / kRows, in = at % kRows, w = in / (16 * RP), rp = in / 16 % RP, n = n0 + in;
       const uint64_t pair = ALL ? 0 : (uint32_t)list[t0 + t];
       if constexpr (INNER) {
@@ -560,10 +580,19 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs m) {
   const uint32_t per = a.cols / 4, at = blockIdx.x * 256 + threadIdx.x, t = at / per, n = (at - t * per) * 4;
   if (t >= a.tokens) return;
   f32x4 v = {};
-  for (uint32_t k = 0; k < a.top_k; ++k) {
-    const uint64_t pair = (uint64_t)t * a.top_k + k;
-    if (g_ld<int32_t>(m.p.chosen + pair * 4) >= 0)
-      v += g_ld<float>(m.p.weights + pair * 4) * __builtin_bit_cast(f32x4, ld16(m.p.y + (pair * a.cols + n) * 4));
+  for (uint32_t k0 = 0; k0 < a.top_k; k0 += 4) {  // four at a time on their way
+    f32x4 y[4];
+    float weight[4];
+    int32_t e[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+      const uint64_t pair = (uint64_t)t * a.top_k + min(k0 + k, a.top_k - 1);
+      e[k] = g_ld<int32_t>(m.p.chosen + pair * 4), weight[k] = g_ld<float>(m.p.weights + pair * 4);
+      y[k] = __builtin_bit_cast(f32x4, ld16(m.p.y + (pair * a.cols + n) * 4));
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k)
+      if (k0 + k < a.top_k && e[k] >= 0) v += weight[k] * y[k];
   }
   const uint64_t to = t * a.out.stride + n;
   if (a.out_type == kTypeBf16)
@@ -597,9 +626,9 @@ hipError_t product_of(const MoeArgs& m, int dma, hipStream_t stream) {
 hipError_t logits_of(const MoeArgs& m, hipStream_t stream) {
   const uint64_t groups = m.a.experts * ((m.a.tokens + kLogitTokens - 1) / kLogitTokens) + m.a.tokens;
   switch (m.a.x_type) {
-    case kTypeF32: return launch(moe_logits_kernel<kTypeF32>, groups, 256, m, stream);
-    case kTypeF16: return launch(moe_logits_kernel<kTypeF16>, groups, 256, m, stream);
-    case kTypeBf16: return launch(moe_logits_kernel<kTypeBf16>, groups, 256, m, stream);
+    case kTypeF32: return launch(moe_logits_kernel<kTypeF32>, groups, kLogitThreads, m, stream);
+    case kTypeF16: return launch(moe_logits_kernel<kTypeF16>, groups, kLogitThreads, m, stream);
+    case kTypeBf16: return launch(moe_logits_kernel<kTypeBf16>, groups, kLogitThreads, m, stream);
     default: return hipErrorInvalidValue;
   }
 }
@@ -625,22 +654,17 @@ hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
     // columns that an expert's tokens take on average
     const double inner_columns = (double)pairs / a.experts * xp, outer_columns = (double)pairs / a.experts * hp;
     if (tokens * xp <= 4)
-      e = product_of<true, false, 1, 4, 1, 4, 3>(m, inner, stream);
+      e = product_of<true, false, 1, 4, 1, 4, 2>(m, inner, stream);
     else if (tokens * xp <= 16 || inner_columns <= 8)
       e = product_of<true, false, 4, 1, 1, 16, 3>(m, inner, stream);
-    else if (inner_columns <= 20)
+    else
       e = product_of<true, false, 4, 1, 1, 32, 2>(m, inner, stream);
-    else
-      e = product_of<true, false, 4, 1, 1, 64, 2>(m, inner, stream);
     if (e != hipSuccess) return e;
-    if (tokens * hp <= 4 && pairs <= 64) return product_of<false, true, 1, 8, 1, 4, 4>(m, outer, stream);
-    if (tokens <= 16 / hp && pairs <= 64) return product_of<false, true, 1, 4, 1, 16, 3>(m, outer, stream);
+    if (tokens * hp <= 4 && pairs <= 64) return product_of<false, true, 1, 8, 1, 4, 3>(m, outer, stream);
     if (tokens * hp <= 16 || outer_columns <= 8)
-      e = product_of<false, false, 4, 1, 2, 16, 3>(m, outer, stream);
-    else if (outer_columns <= 20)
-      e = product_of<false, false, 4, 1, 2, 32, 2>(m, outer, stream);
+      e = product_of<false, false, 4, 1, 1, 16, 3>(m, outer, stream);
     else
-      e = product_of<false, false, 4, 1, 2, 64, 2>(m, outer, stream);
+      e = product_of<false, false, 4, 1, 2, 32, 2>(m, outer, stream);
     if (e == hipSuccess) e = launch(moe_combine_kernel, (tokens * (a.cols / 4) + 255) / 256, 256, m, stream);
     return e;
   });
