@@ -97,6 +97,10 @@ __device__ __forceinline__ void dma16(uint64_t from, uint32_t to) {  // from the
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory", "m0");
 }
 
+__device__ __forceinline__ void dma4(GlobalBytes from, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(from)
+               : "memory", "m0");
+}
 __device__ __forceinline__ void dma4(uint64_t from, uint32_t to) {  // 4 bytes a lane, from multiples of 4
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "memory", "m0");
 }

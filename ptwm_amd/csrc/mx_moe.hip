@@ -27,6 +27,8 @@
 namespace ptwm {
 namespace {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
 constexpr uint32_t kTokens = 64;  // of a launch; longer calls run in several
 constexpr uint32_t kStep = 256;   // values of a row that go through LDS together: a cache line of codes
 
@@ -38,12 +40,13 @@ struct MoePlaces {
   uint64_t logits;   // f64 [tokens][experts]
   uint64_t x;        // bf16 [parts][tokens][x_len]
   uint64_t h;        // bf16 [parts][pairs][h_len]
-  uint64_t y;        // f32 [pairs][cols]
+  uint64_t y;        // f32 [chunks][pairs][cols]
   uint64_t chosen;   // int32 [pairs], -1 where a chosen expert is masked
   uint64_t weights;  // f32 [pairs]
   uint64_t end;
   uint32_t x_len, h_len;  // cols and inner in whole steps, zeros past their ends
 };
+constexpr uint32_t kChunks = 8;  // that the outer products' rows are cut into at most
 MoePlaces places_of(const MxMoeArgs& a) {
   const uint64_t t = a.tokens < kTokens ? a.tokens : kTokens, pairs = t * a.top_k;
   uint64_t at = a.workspace;
@@ -57,7 +60,8 @@ MoePlaces places_of(const MxMoeArgs& a) {
   p.logits = take(t * a.experts * 8);
   p.x = take(parts_of(a.x_type) * t * p.x_len * 2);
   p.h = take(inner_parts(a.out_type) * pairs * p.h_len * 2);
-  p.y = take(pairs * a.cols * 4);
+  const uint64_t chunks = (p.h_len / kStep + 7) / 8;
+  p.y = take((chunks < kChunks ? chunks : kChunks) * pairs * a.cols * 4);
   p.chosen = take(pairs * 4), p.weights = take(pairs * 4);
   p.end = at;
   return p;
@@ -66,7 +70,14 @@ MoePlaces places_of(const MxMoeArgs& a) {
 struct MoeArgs {
   MxMoeArgs a;
   MoePlaces p;
+  uint32_t span, chunks;  // of moe_stream_kernel's rows: steps of a chunk, chunks
 };
+
+// Where a row of x or h in the workspace has 16-byte chunk `c`: of a step's, the f-th of block b (of eight) lies at
+// (b / 4 * 4 + f) * 4 + b % 4, so that what four lanes need for one product lies together.
+__device__ __forceinline__ uint32_t chunk_at(uint32_t c) {
+  return c / 16 * 16 + c % 4 * 4 + c / 4 % 4;
+}
 
 __device__ __forceinline__ void load8_as(uint32_t type, uint64_t base, uint64_t at, float (&v)[8]) {
   if (type == kTypeBf16)
@@ -93,6 +104,42 @@ __device__ __forceinline__ float bias_of(const MxExperts& w, uint32_t type, uint
   return w.bias ? load1_as(type, w.bias, e * w.bias_expert + n * w.bias_stride) : 0.0f;
 }
 
+// Outputs n .. n + 3 of token t.
+__device__ __forceinline__ void store_out(const MxMoeArgs& a, uint64_t t, uint32_t n, f32x4 v) {
+  const uint64_t to = t * a.out.stride + n;
+  if (a.out_type == kTypeBf16)
+    st8(a.out.ptr + to * 2, pack2<kTypeBf16>(v[0], v[1]) | (uint64_t)pack2<kTypeBf16>(v[2], v[3]) << 32);
+  else if (a.out_type == kTypeF16)
+    st8(a.out.ptr + to * 2, pack2<kTypeF16>(v[0], v[1]) | (uint64_t)pack2<kTypeF16>(v[2], v[3]) << 32);
+  else
+    st16(a.out.ptr + to * 4, __builtin_bit_cast(u32x4, v));
+}
+
+__device__ __forceinline__ float activated(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+
+// Two neighbours of a pair's h, the parts `apart` bytes apart: as x's, but for the last, which is rounded.
+__device__ __forceinline__ void store_h(uint32_t out_type, uint64_t to, uint64_t apart, f32x2 h) {
+  const uint32_t hp = inner_parts(out_type);
+  for (uint32_t p = 0; p < hp; ++p, to += apart) {
+    uint32_t b;
+    if (p + 1 < hp) {
+      const uint32_t low = f32_bits(__builtin_amdgcn_fmed3f(h[0], -kBf16Max, kBf16Max)) & 0xFFFF0000u;
+      const uint32_t high = f32_bits(__builtin_amdgcn_fmed3f(h[1], -kBf16Max, kBf16Max)) & 0xFFFF0000u;
+      h -= f32x2{bits_f32(low), bits_f32(high)};
+      b = low >> 16 | high;
+    } else {
+      b = pack2<kTypeBf16>(h[0], h[1]);
+    }
+    st4(to, b);
+  }
+}
+
+// The value that the lane K further on has, of 16.
+template <int K>
+__device__ __forceinline__ float right(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x100 + K, 0xF, 0xF, true));
+}
+
 // Logits of one expert and four tokens: the threads take turns along the rows.  Summed in 64 bits, in which products
 // are exact, so that which of two near experts is chosen does not depend on the order of the additions.  The
 // workgroups after these write x's parts, a token each.
@@ -109,7 +156,12 @@ __global__ __launch_bounds__(kLogitThreads) void moe_logits_kernel(MoeArgs m) {
       u32x4 p[parts_of(T)] = {};
       if (k < a.cols) parts_of_raw<T>(load_raw8<T>(a.x.ptr + (t * a.x.stride + k) * type_bytes(T)), 1.0f, p);
 #pragma unroll
-      for (int j = 0; j < parts_of(T); ++j) st16(m.p.x + ((j * a.tokens + t) * m.p.x_len + k) * 2, p[j]);
+      for (int j = 0; j < parts_of(T); ++j) st16(m.p.x + (j * a.tokens + t) * m.p.x_len * 2 + chunk_at(k / 8) * 16, p[j]);
+    }
+    const uint32_t none = (m.p.h_len - a.inner) / 8, rows = a.top_k * inner_parts(a.out_type);  // chunks of a row
+    for (uint32_t j = threadIdx.x; j < none * rows; j += kLogitThreads) {
+      const uint32_t row = j / none, part = row / a.top_k, pair = t * a.top_k + row % a.top_k;
+      st16(m.p.h + (part * a.tokens * a.top_k + pair) * m.p.h_len * 2 + chunk_at(a.inner / 8 + j % none) * 16, u32x4{});
     }
     return;
   }
@@ -284,7 +336,7 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
   const uint32_t group = wave / WR, wr = wave % WR, gi = wr * 64 + lane;
   const uint32_t rows = INNER ? a.inner : a.cols, length = INNER ? a.cols : a.inner, blocks = length / kMxBlock;
   const uint32_t x_len = INNER ? m.p.x_len : m.p.h_len, steps = x_len / kStep;
-  const uint32_t tiles = ((INNER ? m.p.h_len : rows) + kRows - 1) / kRows;
+  const uint32_t tiles = (rows + kRows - 1) / kRows;
   const uint32_t slot = blockIdx.x / tiles, n0 = blockIdx.x % tiles * kRows;
   const uint32_t parts = INNER ? parts_of(a.x_type) : inner_parts(a.out_type), each = CW / parts;  // tokens of CW columns
   const uint32_t pairs = (uint32_t)a.tokens * a.top_k;
@@ -448,7 +500,7 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
       auto read = [&](int u) {
 #pragma unroll
         for (int c = 0; c < used; ++c) {
-          const uint32_t column = c * 16 + i % CW, chunk = (u / 4 * 4 + q) * 4 + u % 4;
+          const uint32_t column = c * 16 + i % CW, chunk = u * 4 + q;
           xv[u & 1][c] = *(LdsChunks)(columns_at + (stage * kColumns + column * 32 + (chunk ^ (column & 15))) * 16);
         }
       };
@@ -504,7 +556,9 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
           request(ahead, into);
           if (k + NS < n) forward(ahead);
         }
-        if (NC > 1 && used > 1)
+        if (NC > 2 && used > 2)
+          compute(stage, std::integral_constant<int, NC>{});
+        else if (NC > 1 && used > 1)
           compute(stage, std::integral_constant<int, NC < 2 ? NC : 2>{});
         else
           compute(stage, std::integral_constant<int, 1>{});
@@ -524,53 +578,340 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
 #pragma unroll
       for (int c = 0; c < NC; ++c) sums[((wave * RT + r) * NC + c) * 64 + lane] = ALL ? total[ALL ? r : 0][c] : acc[r][c];
     __syncthreads();
-    // of 16s `r` of wavefront w of a group, row `in`, token t: over its parts and the groups
-    auto sum_of = [&](uint32_t w, uint32_t r, uint32_t in, uint32_t t) {
+    // of 16s `r` of wavefront w of a group, rows 4 `quad` .. + 3, token t: over its parts and the groups
+    auto sum_of = [&](uint32_t w, uint32_t r, uint32_t quad, uint32_t t) {
       const uint32_t c = t / each, column = t % each * parts;
-      float v = 0;
+      f32x4 v = {};
 #pragma unroll
       for (uint32_t g = 0; g < KG; ++g)
         for (uint32_t p = 0; p < parts; ++p)
-          v += sums[(((g * WR + w) * RT + r) * NC + c) * 64 + in / 4 * 16 + column + p][in & 3];
+          v += sums[(((g * WR + w) * RT + r) * NC + c) * 64 + quad * 16 + column + p];
       return v;
     };
-    for (uint32_t at = threadIdx.x; at < tokens * kRows; at += 64 * kWaves) {
-      const uint32_t t = at / kRows, in = at % kRows, w = in / (16 * RP), rp = in / 16 % RP, n = n0 + in;
+    for (uint32_t at = threadIdx.x; at < tokens * kRows / 4; at += 64 * kWaves) {
+      const uint32_t t = at / (kRows / 4), in = at % (kRows / 4), w = in / (4 * RP), rp = in / 4 % RP, n = n0 + in * 4;
       const uint64_t pair = ALL ? 0 : (uint32_t)list[t0 + t];
       if constexpr (INNER) {
-        if (n >= m.p.h_len) continue;
-        float h = 0;
-        if (n < a.inner) {
-          const float g = sum_of(w, 0, in % 16, t) + bias_of(a.gate, a.out_type, e0, n);
-          const float u = sum_of(w, 1, in % 16, t) + bias_of(a.up, a.out_type, e0, n);
-          h = g / (1.0f + expf(-g)) * u;
-        }
-        // parts as x's, but for the last, which is rounded
-        const uint32_t hp = inner_parts(a.out_type);
-        for (uint32_t p = 0; p < hp; ++p) {
-          uint16_t b;
-          if (p + 1 < hp) {
-            const uint32_t cut = f32_bits(__builtin_amdgcn_fmed3f(h, -kBf16Max, kBf16Max)) & 0xFFFF0000u;
-            h -= bits_f32(cut);
-            b = (uint16_t)(cut >> 16);
-          } else {
-            b = (uint16_t)pack2<kTypeBf16>(h, 0.0f);
-          }
-          g_st<uint16_t>(m.p.h + (((uint64_t)p * pairs + pair) * m.p.h_len + n) * 2, b);
-        }
+        if (n >= rows) continue;
+        const f32x4 g = sum_of(w, 0, in % 4, t), u = sum_of(w, 1, in % 4, t);
+        f32x4 h;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j)
+          h[j] = activated(g[j] + bias_of(a.gate, a.out_type, e0, n + j), u[j] + bias_of(a.up, a.out_type, e0, n + j));
+        const uint64_t to = m.p.h + pair * m.p.h_len * 2 + chunk_at(n / 8) * 16 + n % 8 * 2, apart = pairs * (uint64_t)m.p.h_len * 2;
+        store_h(a.out_type, to, apart, f32x2{h[0], h[1]}), store_h(a.out_type, to + 4, apart, f32x2{h[2], h[3]});
       } else if (n < rows) {
-        float v = sum_of(w, rp, in % 16, t);
+        f32x4 v = sum_of(w, rp, in % 4, t);
         if constexpr (ALL) {
           for (uint32_t k = 0; a.down.bias && k < experts; ++k) {
             const int32_t pair = table[k * CW + t];
-            if (pair >= 0) v += weights[pair] * bias_of(a.down, a.out_type, (uint32_t)list[k], n);
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j)
+              if (pair >= 0) v[j] += weights[pair] * bias_of(a.down, a.out_type, (uint32_t)list[k], n + j);
           }
-          store1_as(a.out_type, a.out.ptr, t * a.out.stride + n, v);
+          store_out(a, t, n, v);
         } else {
-          g_st<float>(m.p.y + (pair * rows + n) * 4, v + bias_of(a.down, a.out_type, e0, n));
+          st16(m.p.y + (pair * rows + n) * 4, __builtin_bit_cast(u32x4, v));
         }
       }
     }
+  }
+}
+
+// The same products where an expert has several tokens and its weights go through LDS whole (kDma 2): the columns stay
+// in registers.  A workgroup walks along consecutive tiles of 16 rows, of one expert after the other; of a tile's rows
+// wavefront w of eight has steps w, w + 8, ... of a chunk of the rows, S at most, and keeps the values of 16 * NC
+// columns there.  So LDS is for the weights, NS steps of each wavefront on their way, across the ends of tiles and of
+// experts.  A tile's sums are added up over the wavefronts through LDS, while the next tile's products run.  INNER: of
+// whole rows; else of a chunk of them, each chunk a sum of its own, which the combining kernel adds.
+constexpr uint32_t kStreamGroups = 256;  // a workgroup a compute unit
+constexpr uint32_t kStreamSlots = 16;    // experts of a workgroup, see below
+
+template <bool INNER, int S, int NC>
+__global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
+  constexpr int M = INNER ? 2 : 1, NS = 7;
+  constexpr uint32_t kCodes = 128, kWords = 32, N = 3;  // chunks and words of a step, its requests
+  constexpr uint32_t kBiasTiles = 32;                   // whose biases are held at a time
+  __shared__ u32x4 codes[8 * NS * kCodes];
+  __shared__ uint32_t scales[8 * NS * kWords];
+  __shared__ f32x4 sums[8 * M * NC * 64];
+  __shared__ int16_t chosen[kTokens * kMoeMaxTopK];
+  __shared__ uint32_t slots[kStreamSlots], share[2];
+  __shared__ int32_t list[kTokens];
+  __shared__ float biases[M][INNER ? kBiasTiles * 16 : 1];
+  const MxMoeArgs& a = m.a;
+  const uint32_t lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t rows = INNER ? a.inner : a.cols, length = INNER ? a.cols : a.inner, tiles = rows / 16;
+  const uint32_t x_len = INNER ? m.p.x_len : m.p.h_len, steps = x_len / kStep;
+  const uint32_t span = INNER ? steps : m.span, chunks = INNER ? 1 : m.chunks;
+  const uint32_t parts = INNER ? parts_of(a.x_type) : inner_parts(a.out_type), each = 16 / parts, most = each * NC;
+  const uint32_t pairs = (uint32_t)a.tokens * a.top_k;
+  auto scalar = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
+
+  // A slot is an expert's up to `most` tokens.  There are at most 2048 / 5 + 1024 (three parts, one group of columns),
+  // so of the 256 workgroups' equal shares none meets more than eight.
+  {
+    uint32_t* const counts = reinterpret_cast<uint32_t*>(sums);
+    static_assert(sizeof(sums) >= kMoeMaxExperts * 4);
+    for (uint32_t e = threadIdx.x; e < a.experts; e += 512) counts[e] = 0;
+    __syncthreads();
+    for (uint32_t p = threadIdx.x; p < pairs; p += 512) {
+      const int32_t e = g_ld<int32_t>(m.p.chosen + p * 4);
+      chosen[p] = (int16_t)e;
+      if (e >= 0) atomicAdd(&counts[e], 1u);
+    }
+    __syncthreads();
+    if (wave == 0) {
+      const uint64_t of_slot = (uint64_t)chunks * tiles;
+      auto slots_of = [&](uint32_t e) { return e < a.experts ? (counts[e] + most - 1) / most : 0; };
+      auto up_to = [&](uint32_t v) {  // the lane's and lower lanes' together
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+          const uint32_t other = __shfl_up(v, d, 64);
+          if (lane >= d) v += other;
+        }
+        return v;
+      };
+      uint32_t all = 0;
+      for (uint32_t e = 0; e < a.experts; e += 64) all += __shfl(up_to(slots_of(e + lane)), 63, 64);
+      const uint64_t first = all * of_slot * blockIdx.x / kStreamGroups;
+      const uint64_t end = all * of_slot * (blockIdx.x + 1) / kStreamGroups;
+      const uint32_t slot0 = (uint32_t)(first / of_slot);
+      uint32_t at = 0;
+      for (uint32_t e = 0; e < a.experts; e += 64) {
+        const uint32_t n = slots_of(e + lane), to = up_to(n);
+        for (uint32_t j = 0; j < n; ++j) {
+          const uint32_t slot = at + to - n + j - slot0;
+          if (slot < kStreamSlots) slots[slot] = (e + lane) | j << 16;
+        }
+        at += __shfl(to, 63, 64);
+      }
+      if (lane == 0) share[0] = (uint32_t)(end - first), share[1] = (uint32_t)(first - slot0 * of_slot);
+    }
+    __syncthreads();
+  }
+  uint32_t left = scalar(share[0]), slot = 0, chunk = scalar(share[1]) / tiles, tile = scalar(share[1]) % tiles;
+  if (left == 0) return;
+  auto steps_of = [&](uint32_t chunk) {  // of this wavefront
+    const uint32_t have = min(span, steps - chunk * span);
+    return wave < have ? (have - wave + 7) / 8 : 0;
+  };
+
+  // What is to be requested next: step `s` of `n` of matrix `r` of a tile, `run` tiles to the end of the expert's or
+  // the chunk's, `left` to the end of all.  Rows come by 32, so all of a tile's are there.
+  struct {
+    uint32_t left, run, slot, chunk, tile, n, s, r;
+    bool tail;
+    uint64_t codes[M], scales[M];  // the tile's first row, at the wavefront's first step
+    uint64_t code, scale;          // at the step
+  } next{left, 0, 0, chunk, tile, 0, 0, 0, false, {}, {}, 0, 0};
+  auto enter = [&] {
+    while (next.left && (next.n = steps_of(next.chunk)) == 0) {
+      next.left -= min(tiles - next.tile, next.left), next.tile = 0;
+      if (++next.chunk == chunks) next.chunk = 0, ++next.slot;
+    }
+    if (next.left == 0) return;
+    const uint32_t e = scalar(slots[next.slot]) & 0xFFFF, step = next.chunk * span + wave;
+    next.run = min(tiles - next.tile, next.left);
+    next.tail = length % kStep && step + (next.n - 1) * 8 == steps - 1;  // half a step at the end
+#pragma unroll
+    for (int r = 0; r < M; ++r) {
+      const MxExperts& w = INNER ? (r ? a.up : a.gate) : a.down;
+      next.codes[r] = w.codes.ptr + e * w.codes_expert + (uint64_t)next.tile * 16 * w.codes.stride + step * 128;
+      next.scales[r] = w.scales.ptr + e * w.scales_expert + (uint64_t)next.tile * 16 * w.scales.stride + step * 8;
+    }
+    next.code = next.codes[0], next.scale = next.scales[0];
+  };
+  const uint64_t code_rows = 16 * (INNER ? a.gate : a.down).codes.stride;
+  const uint64_t scale_rows = 16 * (INNER ? a.gate : a.down).scales.stride;
+  const uint32_t codes_at = lds_address(codes) + wave * (NS * kCodes * 16);
+  const uint32_t scales_at = lds_address(scales) + wave * (NS * kWords * 4);
+  // A lane's chunks and word from there: in a whole step, and in the half of one, where the last is read over again.
+  uint32_t from[2][2], word[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t c = (lane & 7) ^ (j * 4 + (lane >> 4)), row = (j * 8 + lane / 8) * (uint32_t)(code_rows / 16);
+    from[0][j] = row + c * 16, from[1][j] = row + min(c, 3u) * 16;
+  }
+  word[1] = lane / 2 * (uint32_t)(scale_rows / 16), word[0] = word[1] + lane % 2 * 4;
+  auto request = [&](uint32_t at) {
+    const uint32_t stage = scalar(at);
+    const bool half = next.tail && next.s == next.n - 1;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      dma16(uniform(next.code), half ? from[1][j] : from[0][j], codes_at + (stage * kCodes + j * 64) * 16);
+    if (lane < 32) dma4(uniform(next.scale), half ? word[1] : word[0], scales_at + stage * kWords * 4);
+    if (++next.s < next.n) {
+      next.code += 8 * 128, next.scale += 8 * 8;
+      return;
+    }
+    next.s = 0;
+    if (++next.r == M) {
+      next.r = 0, --next.left;
+      if (--next.run == 0) {
+        next.tile = 0;
+        if (++next.chunk == chunks) next.chunk = 0, ++next.slot;
+        enter();
+        return;
+      }
+#pragma unroll
+      for (int r = 0; r < M; ++r) next.codes[r] += code_rows, next.scales[r] += scale_rows;
+    }
+    next.code = next.codes[M > 1 && next.r ? M - 1 : 0], next.scale = next.scales[M > 1 && next.r ? M - 1 : 0];
+  };
+  enter();
+#pragma unroll 1
+  for (uint32_t k = 0; k < NS; ++k)
+    if (next.left) request(k);
+
+  // Sums of a tile: every 2 * NC wavefronts in turn add them up, each of 16 columns two rows of every four.
+  constexpr uint32_t kTurns = 4 / NC;
+  static_assert(4 % NC == 0);
+  const uint32_t turn = wave / (2 * NC), group = wave / 2 % NC, n_in = q * 4 + wave % 2 * 2;
+  const uint32_t summed = lds_address(sums) + (group * 64 + lane) * 16 + wave % 2 * 8;
+  const bool biased = INNER && (a.gate.bias || a.up.bias);
+  u32x4 x[S][NC][8];
+  uint32_t stage = 0, e = 0, t0 = 0, tokens = 0, used = 0;
+  bool fresh = true;
+  while (left) {
+    const uint32_t run = min(tiles - tile, left), mine = steps_of(chunk);
+    if (fresh || chunk == 0) {  // the expert's pairs, in the order of the tokens; every wavefront writes the same
+      e = scalar(slots[slot]), t0 = (e >> 16) * most, e &= 0xFFFF;
+      int32_t pair = -1;
+      if (lane < a.tokens)
+        for (uint32_t k = 0; k < a.top_k; ++k)
+          if (chosen[lane * a.top_k + k] == (int32_t)e) pair = (int32_t)(lane * a.top_k + k);
+      const uint64_t mask = __ballot(pair >= 0);
+      if (pair >= 0) list[__popcll(mask & ((1ull << lane) - 1))] = pair;
+      tokens = min((uint32_t)__popcll(mask) - t0, most), used = (tokens + each - 1) / each;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      fresh = false;
+    }
+    const GlobalBytes x0 = global_bytes(INNER ? m.p.x : m.p.h);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if (c < used) {
+        uint32_t t = c * each + i / parts, part = i % parts;  // columns without a token repeat the first
+        if (i >= each * parts || t >= tokens) t = 0, part = 0;
+        const uint32_t pair = (uint32_t)list[t0 + t];
+        const uint32_t row = INNER ? part * (uint32_t)a.tokens + pair / a.top_k : part * pairs + pair;
+        const uint32_t at = row * x_len * 2 + (chunk * span + wave) * (kStep * 2) + q * 16;
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+          if (s < mine)
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[s][c][u] = ld16(x0, at + s * 8 * (kStep * 2) + u * 64);
+      }
+    }
+    // where this lane's sums go: of the first part's column
+    const uint32_t t = group * each + i / parts;
+    const bool stores = i % parts == 0 && i / parts < each && t < tokens;
+    const uint64_t pair = stores ? (uint32_t)list[t0 + t] : 0;
+    const uint64_t out = INNER ? m.p.h + pair * m.p.h_len * 2 + chunk_at(n_in / 8) * 16 + n_in % 8 * 2
+                               : m.p.y + ((chunk * (uint64_t)pairs + pair) * rows + n_in) * 4;
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0), here rather than before each tile's first product
+
+    f32x2 v[M] = {};
+    auto add_up = [&] {
+      f32x2 terms[8][M];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int r = 0; r < M; ++r)
+          terms[k][r] = __builtin_bit_cast(f32x2, *(LdsPairs)(summed + (k * M + r) * NC * 1024));
+#pragma unroll
+      for (int r = 0; r < M; ++r) {
+        v[r] = terms[0][r];
+#pragma unroll
+        for (int k = 1; k < 8; ++k) v[r] += terms[k][r];
+      }
+    };
+    uint32_t bias0 = 0;
+    auto store = [&](uint32_t tile) {
+      // a token's parts are columns side by side
+#pragma unroll
+      for (int r = 0; r < M; ++r) {
+        const f32x2 own = v[r];
+        if (parts > 1) v[r] += f32x2{right<1>(own[0]), right<1>(own[1])};
+        if (parts > 2) v[r] += f32x2{right<2>(own[0]), right<2>(own[1])};
+      }
+      if (!stores) return;
+      if constexpr (INNER) {
+        if (biased) {
+          const uint32_t at = (tile - bias0) * 16 + n_in;
+          v[0] += f32x2{biases[0][at], biases[0][at + 1]}, v[M - 1] += f32x2{biases[M - 1][at], biases[M - 1][at + 1]};
+        }
+        store_h(m.a.out_type, out + chunk_at(tile * 2) * 16, (uint64_t)pairs * m.p.h_len * 2,
+                f32x2{activated(v[0][0], v[M - 1][0]), activated(v[0][1], v[M - 1][1])});
+      } else {
+        st8(out + tile * 64, __builtin_bit_cast(uint64_t, v[0]));
+      }
+    };
+    auto walk = [&](auto used_) {
+      constexpr int used = used_;
+      for (uint32_t k = 0; k < run; ++k) {
+        bool open = k > 0 && (k - 1) % kTurns == turn && group < used;  // the last tile's sums are this wavefront's
+        if (open) add_up();
+        if (biased && k % kBiasTiles == 0) {
+          if (open) store(tile + k - 1), open = false;  // with the biases before
+          bias0 = tile + k;
+          __syncthreads();
+          const uint32_t n = bias0 * 16 + threadIdx.x;
+          static_assert(kBiasTiles * 16 == 512, "a thread a row");
+          if (INNER && n < rows)
+            biases[0][threadIdx.x] = bias_of(a.gate, a.out_type, e, n), biases[M - 1][threadIdx.x] = bias_of(a.up, a.out_type, e, n);
+          __syncthreads();
+        }
+        f32x4 acc[M][used] = {};
+#pragma unroll
+        for (int r = 0; r < M; ++r)
+#pragma unroll
+          for (int s = 0; s < S; ++s)
+            if (s < mine) {
+              if (next.left)
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * N) : "memory");
+              else
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+              const u32x2 words = *(LdsPairs)(scales_at + stage * (kWords * 4) + i * 8);
+              u32x4 w4[2];
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                w4[h] = *(LdsChunks)(codes_at + (stage * kCodes + i * 8 + ((h * 4 + q) ^ (i / 2))) * 16);
+              asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+              if (next.left) request(stage);  // in place of what has just been read
+              stage = stage + 1 == NS ? 0 : stage + 1;
+#pragma unroll
+              for (int u = 0; u < 8; ++u) {
+                const u32x4 w8 = weights8(w4[u / 4][u % 4], scale_f32(words[u / 4] >> 8 * q & 0xFF));
+#pragma unroll
+                for (int c = 0; c < used; ++c) acc[r][c] = mfma(w8, x[s][c][u], acc[r][c]);
+              }
+            }
+        if (open) store(tile + k - 1);
+        // Sums to LDS, 16 columns at a time: lane l has rows 4 (l / 16) .. + 3 of column l % 16.
+        __builtin_amdgcn_s_barrier();  // the ones before have been read
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int r = 0; r < M; ++r)
+#pragma unroll
+          for (int c = 0; c < used; ++c) sums[((wave * M + r) * NC + c) * 64 + lane] = acc[r][c];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      }
+      if ((run - 1) % kTurns == turn && group < used) add_up(), store(tile + run - 1);
+    };
+    if (NC > 3 && used > 3)
+      walk(std::integral_constant<int, NC>{});
+    else if (NC > 2 && used > 2)
+      walk(std::integral_constant<int, NC < 3 ? NC : 3>{});
+    else if (NC > 1 && used > 1)
+      walk(std::integral_constant<int, NC < 2 ? NC : 2>{});
+    else
+      walk(std::integral_constant<int, 1>{});
+    left -= run, tile = 0;
+    if (++chunk == chunks) chunk = 0, ++slot;
   }
 }
 
@@ -579,28 +920,29 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs m) {
   const MxMoeArgs& a = m.a;
   const uint32_t per = a.cols / 4, at = blockIdx.x * 256 + threadIdx.x, t = at / per, n = (at - t * per) * 4;
   if (t >= a.tokens) return;
+  const uint64_t pairs = a.tokens * a.top_k;
+  const uint32_t terms = a.top_k * m.chunks;
   f32x4 v = {};
-  for (uint32_t k0 = 0; k0 < a.top_k; k0 += 4) {  // four at a time on their way
+  for (uint32_t j0 = 0; j0 < terms; j0 += 4) {  // four at a time on their way
     f32x4 y[4];
     float weight[4];
     int32_t e[4];
 #pragma unroll
-    for (uint32_t k = 0; k < 4; ++k) {
-      const uint64_t pair = (uint64_t)t * a.top_k + min(k0 + k, a.top_k - 1);
-      e[k] = g_ld<int32_t>(m.p.chosen + pair * 4), weight[k] = g_ld<float>(m.p.weights + pair * 4);
-      y[k] = __builtin_bit_cast(f32x4, ld16(m.p.y + (pair * a.cols + n) * 4));
+    for (uint32_t j = 0; j < 4; ++j) {
+      const uint32_t term = min(j0 + j, terms - 1), k = term / m.chunks;
+      const uint64_t pair = t * a.top_k + k;
+      e[j] = g_ld<int32_t>(m.p.chosen + pair * 4), weight[j] = g_ld<float>(m.p.weights + pair * 4);
+      y[j] = __builtin_bit_cast(f32x4, ld16(m.p.y + (((term - k * m.chunks) * pairs + pair) * a.cols + n) * 4));
+      if (a.down.bias && term == k * m.chunks && e[j] >= 0) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) y[j][i] += bias_of(a.down, a.out_type, (uint32_t)e[j], n + i);
+      }
     }
 #pragma unroll
-    for (uint32_t k = 0; k < 4; ++k)
-      if (k0 + k < a.top_k && e[k] >= 0) v += weight[k] * y[k];
+    for (uint32_t j = 0; j < 4; ++j)
+      if (j0 + j < terms && e[j] >= 0) v += weight[j] * y[j];
   }
-  const uint64_t to = t * a.out.stride + n;
-  if (a.out_type == kTypeBf16)
-    st8(a.out.ptr + to * 2, pack2<kTypeBf16>(v[0], v[1]) | (uint64_t)pack2<kTypeBf16>(v[2], v[3]) << 32);
-  else if (a.out_type == kTypeF16)
-    st8(a.out.ptr + to * 2, pack2<kTypeF16>(v[0], v[1]) | (uint64_t)pack2<kTypeF16>(v[2], v[3]) << 32);
-  else
-    st16(a.out.ptr + to * 4, __builtin_bit_cast(u32x4, v));
+  store_out(a, t, n, v);
 }
 
 // How far the weights of one product go by DMA.
@@ -615,12 +957,27 @@ int dma_of(const MxExperts& w, uint32_t length, uint64_t experts) {
 template <bool INNER, bool ALL, int WR, int KG, int RP, int XC, int NS>
 hipError_t product_of(const MoeArgs& m, int dma, hipStream_t stream) {
   constexpr uint32_t kRows = 16 * RP * WR;
-  const uint64_t tiles = ((INNER ? m.p.h_len : m.a.cols) + kRows - 1) / kRows, pairs = m.a.tokens * m.a.top_k;
+  const uint64_t tiles = ((INNER ? m.a.inner : m.a.cols) + kRows - 1) / kRows, pairs = m.a.tokens * m.a.top_k;
   const uint64_t items = ALL ? 1 : pairs < m.a.experts ? pairs : m.a.experts;
   return launch(dma == 2   ? moe_product_kernel<INNER, ALL, WR, KG, RP, XC, NS, 2>
                 : dma == 1 ? moe_product_kernel<INNER, ALL, WR, KG, RP, XC, NS, 1>
                            : moe_product_kernel<INNER, ALL, WR, KG, RP, XC, NS, 0>,
                 items * tiles, 64 * WR * KG, m, stream);
+}
+
+// 16 rows as 32-bit offsets.
+bool near_rows(const MxExperts& w) { return w.codes.stride < 1ull << 27 && w.scales.stride < 1ull << 27; }
+
+// S steps of a wavefront; false if the rows are too long for that, or too short to keep most of eight busy.
+bool chunks_of(uint32_t len, bool inner, uint32_t s, MoeArgs& m) {
+  const uint32_t steps = len / kStep, most = 8 * s, chunks = (steps + most - 1) / most;
+  if (steps < 5 || chunks > (inner ? 1 : kChunks)) return false;
+  if (!inner) m.span = (steps + chunks - 1) / chunks, m.chunks = (steps + m.span - 1) / m.span;
+  return true;
+}
+template <bool INNER, int S, int NC>
+hipError_t stream_of(const MoeArgs& m, hipStream_t stream) {
+  return launch(moe_stream_kernel<INNER, S, NC>, kStreamGroups, 512, m, stream);
 }
 
 hipError_t logits_of(const MoeArgs& m, hipStream_t stream) {
@@ -641,7 +998,7 @@ hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
   const int gate = dma_of(a.gate, a.cols, a.experts), up = dma_of(a.up, a.cols, a.experts);
   const int inner = gate < up ? gate : up, outer = dma_of(a.down, a.inner, a.experts);
   return in_parts(a.tokens, kTokens, [&](uint64_t first, uint64_t tokens) {
-    MoeArgs m{a, places_of(a)};
+    MoeArgs m{a, places_of(a), 1, 1};
     m.a.tokens = tokens;
     m.a.x = rows_from(a.x, first, type_bytes(a.x_type)), m.a.out = rows_from(a.out, first, type_bytes(a.out_type));
     if (a.experts_out) m.a.experts_out += first * a.top_k * 4;
@@ -649,22 +1006,30 @@ hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
     hipError_t e = logits_of(m, stream);
     const uint64_t pairs = tokens * a.top_k;
     const uint32_t xp = parts_of(a.x_type), hp = inner_parts(a.out_type);
+    const bool few_inner = tokens * xp <= 4, few_outer = tokens * hp <= 4 && pairs <= 64;
     if (e == hipSuccess && pairs > kFusedPairs) e = launch(moe_route_kernel, tokens, 64, m, stream);
     if (e != hipSuccess) return e;
     // columns that an expert's tokens take on average
     const double inner_columns = (double)pairs / a.experts * xp, outer_columns = (double)pairs / a.experts * hp;
-    if (tokens * xp <= 4)
+    const bool stream_inner = pairs > kFusedPairs && inner == 2 && near_rows(a.gate) &&
+                              a.gate.codes.stride == a.up.codes.stride && a.gate.scales.stride == a.up.scales.stride;
+    const bool stream_outer = pairs > kFusedPairs && outer == 2 && near_rows(a.down);
+    if (few_inner)
       e = product_of<true, false, 1, 4, 1, 4, 2>(m, inner, stream);
-    else if (tokens * xp <= 16 || inner_columns <= 8)
+    else if (stream_inner && inner_columns > 8 && chunks_of(m.p.x_len, true, 2, m))
+      e = stream_of<true, 2, 2>(m, stream);
+    else if (stream_inner && chunks_of(m.p.x_len, true, 4, m))
+      e = stream_of<true, 4, 1>(m, stream);
+    else
       e = product_of<true, false, 4, 1, 1, 16, 3>(m, inner, stream);
-    else
-      e = product_of<true, false, 4, 1, 1, 32, 2>(m, inner, stream);
     if (e != hipSuccess) return e;
-    if (tokens * hp <= 4 && pairs <= 64) return product_of<false, true, 1, 8, 1, 4, 3>(m, outer, stream);
-    if (tokens * hp <= 16 || outer_columns <= 8)
-      e = product_of<false, false, 4, 1, 1, 16, 3>(m, outer, stream);
+    if (few_outer) return product_of<false, true, 1, 8, 1, 4, 3>(m, outer, stream);
+    if (stream_outer && outer_columns > 8 && chunks_of(m.p.h_len, false, 1, m))
+      e = stream_of<false, 1, 4>(m, stream);
+    else if (stream_outer && chunks_of(m.p.h_len, false, 4, m))
+      e = stream_of<false, 4, 1>(m, stream);
     else
-      e = product_of<false, false, 4, 1, 2, 32, 2>(m, outer, stream);
+      e = product_of<false, false, 4, 1, 1, 16, 3>(m, outer, stream);
     if (e == hipSuccess) e = launch(moe_combine_kernel, (tokens * (a.cols / 4) + 255) / 256, 256, m, stream);
     return e;
   });
