@@ -96,6 +96,14 @@ __device__ __forceinline__ void dma16(GlobalBytes from, uint32_t offset, uint32_
 __device__ __forceinline__ void dma16(uint64_t from, uint32_t to) {  // from the lane's own address
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory", "m0");
 }
+// Of bytes that nobody reads again: they leave L2 first, and what is being written there stays until its lines are full.
+__device__ __forceinline__ void dma16_once(GlobalBytes from, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(to), "v"(offset), "s"(from)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void dma16_once(uint64_t from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(to), "v"(from) : "memory", "m0");
+}
 
 __device__ __forceinline__ void dma4(GlobalBytes from, uint32_t offset, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(from)

@@ -29,6 +29,7 @@ namespace {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
+constexpr uint32_t kComputeUnits = 256;
 constexpr uint32_t kTokens = 64;  // of a launch; longer calls run in several
 constexpr uint32_t kStep = 256;   // values of a row that go through LDS together: a cache line of codes
 
@@ -46,7 +47,7 @@ struct MoePlaces {
   uint64_t end;
   uint32_t x_len, h_len;  // cols and inner in whole steps, zeros past their ends
 };
-constexpr uint32_t kChunks = 8;  // that the outer products' rows are cut into at most
+constexpr uint32_t kChunks = 16;  // that the outer products' rows are cut into at most
 MoePlaces places_of(const MxMoeArgs& a) {
   const uint64_t t = a.tokens < kTokens ? a.tokens : kTokens, pairs = t * a.top_k;
   uint64_t at = a.workspace;
@@ -71,6 +72,7 @@ struct MoeArgs {
   MxMoeArgs a;
   MoePlaces p;
   uint32_t span, chunks;  // of moe_stream_kernel's rows: steps of a chunk, chunks
+  bool routed;            // moe_route_kernel has run
 };
 
 // Where a row of x or h in the workspace has 16-byte chunk `c`: of a step's, the f-th of block b (of eight) lies at
@@ -100,8 +102,24 @@ __device__ __forceinline__ void store1_as(uint32_t type, uint64_t base, uint64_t
   else
     store1<kTypeF32>(base + at * 4, v);
 }
-__device__ __forceinline__ float bias_of(const MxExperts& w, uint32_t type, uint32_t e, uint32_t n) {
-  return w.bias ? load1_as(type, w.bias, e * w.bias_expert + n * w.bias_stride) : 0.0f;
+// An expert's N biases from row n on, zeros without one.
+template <int N>
+__device__ __forceinline__ void biases_of(const MxExperts& w, uint32_t type, uint32_t e, uint32_t n, float (&b)[N]) {
+  const uint64_t at = e * w.bias_expert + n * w.bias_stride;
+  auto load = [&](auto t) {  // all on their way at once
+#pragma unroll
+    for (int j = 0; j < N; ++j) b[j] = load1<t>(w.bias + (at + j * w.bias_stride) * type_bytes(t));
+  };
+  if (!w.bias) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) b[j] = 0.0f;
+  } else if (type == kTypeBf16) {
+    load(std::integral_constant<uint32_t, kTypeBf16>{});
+  } else if (type == kTypeF16) {
+    load(std::integral_constant<uint32_t, kTypeF16>{});
+  } else {
+    load(std::integral_constant<uint32_t, kTypeF32>{});
+  }
 }
 
 // Outputs n .. n + 3 of token t.
@@ -297,9 +315,9 @@ constexpr uint32_t kFusedPairs = 32;
 
 // Rows of one expert's products for its tokens (or, ALL, of the outer products
 // of all experts of up to 64 pairs, weighted and added up).  WR wavefronts hold
-// 16 * RP rows each, of gate and up (INNER) or of down, and share the columns;
-// KG groups of them take turns in steps of 256 values along the rows and add up
-// in LDS at the end.
+// 16 rows each, of gate and up (INNER) or of down, and share the XC columns; KG
+// groups of them take turns in steps of 256 values along the rows and add up in
+// LDS at the end.
 //
 // Codes, scales and columns go through LDS by DMA, NS - 1 steps ahead: the
 // matrix instruction's order, a row a lane, would cost the address unit a cycle
@@ -313,21 +331,20 @@ constexpr uint32_t kFusedPairs = 32;
 // kDma 2: codes lie at multiples of 16 bytes and scales of 4, whole words of
 // four blocks; 1: codes only, scales come byte by byte; 0: codes go through
 // registers.
-template <bool INNER, bool ALL, int WR, int KG, int RP, int XC, int NS, int kDma>
+template <bool INNER, bool ALL, int WR, int KG, int XC, int NS, int kDma>
 __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
   static_assert(WR == 1 || KG == 1, "groups of several wavefronts meet at barriers of the whole workgroup");
-  static_assert(!(INNER && ALL) && (!INNER || RP == 1) && (!ALL || XC <= 16), "one group of columns for all tokens");
-  constexpr int M = INNER ? 2 : 1, RT = M * RP;               // matrices, 16s of rows
-  constexpr int NC = (XC + 15) / 16, CW = XC < 16 ? XC : 16;  // groups of columns, columns of one
-  constexpr uint32_t G = 64 * WR, kWaves = WR * KG, kRows = 16 * RP * WR;
-  constexpr uint32_t kCodes = RT * 128, kColumns = XC * 32;  // chunks of a stage
-  constexpr int JW = kCodes / 64, JX = kColumns / G, JS = kDma == 2 ? 1 : 2 * RT;
+  static_assert(!(INNER && ALL) && XC <= 16, "a product has 16 columns");
+  constexpr int M = INNER ? 2 : 1;  // matrices
+  constexpr uint32_t G = 64 * WR, kWaves = WR * KG, kRows = 16 * WR;
+  constexpr uint32_t kCodes = M * 128, kColumns = XC * 32;  // chunks of a stage
+  constexpr int JW = kCodes / 64, JX = kColumns / G, JS = kDma == 2 ? 1 : 2 * M;
   constexpr int N = JX + (kDma > 0 ? JW : 0) + JS;  // requests of a step
   constexpr uint32_t kScales = JS * 64;                                          // words of a stage
-  static_assert(kColumns % G == 0 && RT <= 2 && (NS - 2) * N < 64, "whole requests, and a wait that counts them");
+  static_assert(kColumns % G == 0 && (NS - 2) * N < 64, "whole requests, and a wait that counts them");
   __shared__ u32x4 columns[KG * NS * kColumns], codes[KG * WR * NS * kCodes];
   __shared__ uint32_t scales[KG * WR * NS * kScales];
-  __shared__ int32_t list[64], table[ALL ? 64 * CW : 1], fused[INNER ? kFusedPairs : 1];
+  __shared__ int32_t list[64], table[ALL ? 64 * XC : 1], fused[INNER ? kFusedPairs : 1];
   __shared__ float weights[ALL ? 64 : 1];
   const MxMoeArgs& a = m.a;
   const uint32_t lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
@@ -338,7 +355,7 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
   const uint32_t x_len = INNER ? m.p.x_len : m.p.h_len, steps = x_len / kStep;
   const uint32_t tiles = (rows + kRows - 1) / kRows;
   const uint32_t slot = blockIdx.x / tiles, n0 = blockIdx.x % tiles * kRows;
-  const uint32_t parts = INNER ? parts_of(a.x_type) : inner_parts(a.out_type), each = CW / parts;  // tokens of CW columns
+  const uint32_t parts = INNER ? parts_of(a.x_type) : inner_parts(a.out_type), each = XC / parts;  // tokens of XC columns
   const uint32_t pairs = (uint32_t)a.tokens * a.top_k;
 
   // The expert and the pairs that chose it (every wavefront writes the same to LDS); ALL: the experts that any pair
@@ -356,16 +373,16 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
     }
     const uint64_t leaders = __ballot(e >= 0 && leader == lane);
     experts = __popcll(leaders);
-    for (uint32_t k = lane; k < experts * CW; k += 64) table[k] = -1;
+    for (uint32_t k = lane; k < experts * XC; k += 64) table[k] = -1;
     if (e >= 0) {
       const uint32_t k = __popcll(leaders & ((1ull << leader) - 1));
-      table[k * CW + lane / a.top_k] = (int32_t)lane;
+      table[k * XC + lane / a.top_k] = (int32_t)lane;
       if (leader == lane) list[k] = e;
     }
     __syncthreads();
     if (lane < experts) expert_k = list[lane];
   } else {
-    const bool choosing = INNER && pairs <= kFusedPairs;
+    const bool choosing = INNER && !m.routed;
     if (choosing) {
       for (uint32_t t = wave; t < a.tokens; t += kWaves) {
         const Chosen c = choose(m, t);
@@ -394,7 +411,7 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
   // Rows past the last one take its place; their sums are not stored, or as zeros.
   uint64_t w_at[JW], s_at[JS];  // codes and scales
   auto matrix = [&](int r) -> const MxExperts& { return INNER ? (r ? a.up : a.gate) : a.down; };
-  auto row_of = [&](int r, uint32_t in) { return min(n0 + (wr * RP + (INNER ? 0 : r)) * 16 + in, rows - 1); };
+  auto row_of = [&](uint32_t in) { return min(n0 + wr * 16 + in, rows - 1); };
   auto scales_of = [&](int r, uint32_t n) {
     const MxExperts& w = matrix(r);
     return w.scales.ptr + e0 * w.scales_expert + n * w.scales.stride;
@@ -402,28 +419,28 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
 #pragma unroll
   for (int j = 0; j < JW; ++j) {
     const MxExperts& w = matrix(j / 2);
-    w_at[j] = w.codes.ptr + e0 * w.codes_expert + row_of(j / 2, j % 2 * 8 + lane / 8) * w.codes.stride;
+    w_at[j] = w.codes.ptr + e0 * w.codes_expert + row_of(j % 2 * 8 + lane / 8) * w.codes.stride;
   }
   if constexpr (kDma == 2) {  // two words a row
-    s_at[0] = RT == 2 && lane >= 32 ? scales_of(1, row_of(1, lane / 2 % 16)) : scales_of(0, row_of(0, lane / 2 % 16));
+    s_at[0] = M == 2 && lane >= 32 ? scales_of(1, row_of(lane / 2 % 16)) : scales_of(0, row_of(lane / 2 % 16));
   } else {  // eight bytes a row
 #pragma unroll
-    for (int j = 0; j < JS; ++j) s_at[j] = scales_of(j / 2, row_of(j / 2, j % 2 * 8 + lane / 8));
+    for (int j = 0; j < JS; ++j) s_at[j] = scales_of(j / 2, row_of(j % 2 * 8 + lane / 8));
   }
   const uint32_t columns_at = lds_address(columns) + group * (NS * kColumns * 16);
   const uint32_t codes_at = lds_address(codes) + wave * (NS * kCodes * 16);
   const uint32_t scales_at = lds_address(scales) + wave * (NS * kScales * 4);
 
-  for (uint32_t t0 = 0; t0 < count; t0 += each * NC) {
-    const uint32_t tokens = min(count - t0, each * NC), used = (tokens + each - 1) / each;  // groups of columns
+  for (uint32_t t0 = 0; t0 < count; t0 += each) {
+    const uint32_t tokens = min(count - t0, each);
     // A lane's chunks of the columns, as offsets: column c holds part c % parts of a token; columns without one repeat
     // the first.  (2^31 bytes hold 3 parts of 2048 pairs of the longest rows.)
     uint32_t x_at[JX], x_token[ALL ? JX : 1];
 #pragma unroll
     for (int j = 0; j < JX; ++j) {
-      const uint32_t column = (j * G + gi) / 32, c = column % CW;
-      uint32_t t = column / CW * each + c / parts, part = c % parts;
-      if (c >= each * parts || t >= tokens) t = 0, part = 0;
+      const uint32_t column = (j * G + gi) / 32;
+      uint32_t t = column / parts, part = column % parts;
+      if (t >= tokens) t = 0, part = 0;
       const uint32_t chunk = (gi & 31) ^ (column & 15);
       uint32_t row = part * pairs;
       if constexpr (ALL) {
@@ -451,7 +468,7 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
         const uint32_t chunk = (lane & 7) ^ (j * 4 + (lane >> 4) & 7);
         const uint64_t from = w_at[j] + e * a.down.codes_expert + min(u.step * 8 + chunk, blocks - 1) * 16;
         if constexpr (kDma > 0)
-          dma16(from, codes_at + (stage * kCodes + j * 64) * 16);
+          dma16_once(from, codes_at + (stage * kCodes + j * 64) * 16);
         else
           ((LdsChunks)(codes_at + (stage * kCodes + lane) * 16))[j * 64] = ld16(from);
       }
@@ -466,67 +483,47 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
       }
 #pragma unroll
       for (int j = 0; j < JX; ++j) {
-        if (NS == 2 && NC > 1 && j * G >= used * 512) break;  // a wait for all needs no count of them
         uint32_t from = x_at[j] + u.step * (kStep * 2);
         if constexpr (ALL) {
           // a token that did not choose the expert has another's h here, whose sums are left out
-          const int32_t pair = table[u.k * CW + x_token[j]];
+          const int32_t pair = table[u.k * XC + x_token[j]];
           from += (uint32_t)max(pair, 0) * x_len * 2;
         }
         dma16(x0, from, columns_at + (stage * kColumns + j * G + wr * 64) * 16);
       }
     };
-    f32x4 acc[RT][NC] = {}, total[ALL ? RT : 1][NC] = {};
-    auto compute = [&](uint32_t stage, auto used_) {
-      constexpr int used = used_;
-      u32x2 words[RT];
+    f32x4 acc[M] = {}, total = {};
+    auto compute = [&](uint32_t stage) {
+      u32x2 words[M];
       if constexpr (kDma == 2) {
 #pragma unroll
-        for (int r = 0; r < RT; ++r) words[r] = *(LdsPairs)(scales_at + stage * (kScales * 4) + (r * 16 + i) * 8);
+        for (int r = 0; r < M; ++r) words[r] = *(LdsPairs)(scales_at + stage * (kScales * 4) + (r * 16 + i) * 8);
       }
-      u32x4 wv[2][RT];
-      float sf[2][RT];
+      u32x4 wv[2][M];
+      float sf[2][M];
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
+        for (int r = 0; r < M; ++r) {
           const uint32_t row = r * 16 + i, c = s * 4 + q;
           wv[s][r] = *(LdsChunks)(codes_at + (stage * kCodes + row * 8 + (c ^ (row / 2 & 7))) * 16);
           sf[s][r] = scale_f32(kDma == 2 ? words[r][s] >> 8 * q & 0xFF
                                          : *(LdsWord)(scales_at + (stage * kScales + row * 8 + c) * 4));
         }
-      // columns are read a product ahead, and no further: eight products' are more than the registers
-      u32x4 xv[2][used];
-      auto read = [&](int u) {
-#pragma unroll
-        for (int c = 0; c < used; ++c) {
-          const uint32_t column = c * 16 + i % CW, chunk = u * 4 + q;
-          xv[u & 1][c] = *(LdsChunks)(columns_at + (stage * kColumns + column * 32 + (chunk ^ (column & 15))) * 16);
-        }
-      };
-      read(0);
+      const uint32_t column = i % XC;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        if (u < 7) read(u + 1);
+        const u32x4 xv = *(LdsChunks)(columns_at + (stage * kColumns + column * 32 + ((u * 4 + q) ^ column)) * 16);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const u32x4 w8 = weights8(wv[u / 4][r][u % 4], sf[u / 4][r]);
-#pragma unroll
-          for (int c = 0; c < used; ++c) acc[r][c] = mfma(w8, xv[u & 1][c], acc[r][c]);
-        }
-        if constexpr (used > 2) __builtin_amdgcn_sched_barrier(0);
+        for (int r = 0; r < M; ++r) acc[r] = mfma(weights8(wv[u / 4][r][u % 4], sf[u / 4][r]), xv, acc[r]);
       }
     };
     auto add_expert = [&](uint32_t k) {  // an expert's sums, weighted, for the tokens that chose it
-      const uint32_t c = i % CW, t = c / parts;
-      const int32_t pair = c < each * parts && t < tokens ? table[ALL ? k * CW + t : 0] : -1;
-      const float weight = weights[ALL ? max(pair, 0) : 0];
-#pragma unroll
-      for (int r = 0; r < (ALL ? RT : 1); ++r) {
-        const f32x4 more = total[r][0] + weight * acc[r][0];
-        total[r][0] = pair >= 0 ? more : total[r][0];
-        acc[r][0] = f32x4{};
-      }
+      const uint32_t c = i % XC, t = c / parts;
+      const int32_t pair = t < tokens ? table[ALL ? k * XC + t : 0] : -1;
+      const f32x4 more = total + weights[ALL ? max(pair, 0) : 0] * acc[0];
+      total = pair >= 0 ? more : total;
+      acc[0] = f32x4{};
     };
     const uint32_t n = group < units ? (units - group + KG - 1) / KG : 0;  // of this group
     if (t0) __syncthreads();  // before LDS is used again
@@ -556,12 +553,7 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
           request(ahead, into);
           if (k + NS < n) forward(ahead);
         }
-        if (NC > 2 && used > 2)
-          compute(stage, std::integral_constant<int, NC>{});
-        else if (NC > 1 && used > 1)
-          compute(stage, std::integral_constant<int, NC < 2 ? NC : 2>{});
-        else
-          compute(stage, std::integral_constant<int, 1>{});
+        compute(stage);
         if constexpr (ALL) {
           if (k + 1 == n || next.k != now.k) add_expert(now.k);
         }
@@ -572,42 +564,41 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
     // Sums to LDS, in place of the codes: 16 rows and 16 columns at a time, lane l rows 4 (l / 16) .. + 3 of column l % 16.
     __syncthreads();
     f32x4* const sums = reinterpret_cast<f32x4*>(codes);
-    static_assert(RT * NC * 64 <= NS * kCodes, "a wavefront's sums fit its codes");
+    static_assert(M * 64 <= NS * kCodes, "a wavefront's sums fit its codes");
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-      for (int c = 0; c < NC; ++c) sums[((wave * RT + r) * NC + c) * 64 + lane] = ALL ? total[ALL ? r : 0][c] : acc[r][c];
+    for (int r = 0; r < M; ++r) sums[(wave * M + r) * 64 + lane] = ALL ? total : acc[r];
     __syncthreads();
-    // of 16s `r` of wavefront w of a group, rows 4 `quad` .. + 3, token t: over its parts and the groups
+    // of matrix r, rows 4 `quad` .. + 3 of wavefront w of a group, token t: over its parts and the groups
     auto sum_of = [&](uint32_t w, uint32_t r, uint32_t quad, uint32_t t) {
-      const uint32_t c = t / each, column = t % each * parts;
       f32x4 v = {};
 #pragma unroll
       for (uint32_t g = 0; g < KG; ++g)
-        for (uint32_t p = 0; p < parts; ++p)
-          v += sums[(((g * WR + w) * RT + r) * NC + c) * 64 + quad * 16 + column + p];
+        for (uint32_t p = 0; p < parts; ++p) v += sums[((g * WR + w) * M + r) * 64 + quad * 16 + t * parts + p];
       return v;
     };
     for (uint32_t at = threadIdx.x; at < tokens * kRows / 4; at += 64 * kWaves) {
-      const uint32_t t = at / (kRows / 4), in = at % (kRows / 4), w = in / (4 * RP), rp = in / 4 % RP, n = n0 + in * 4;
+      const uint32_t t = at / (kRows / 4), in = at % (kRows / 4), w = in / 4, n = n0 + in * 4;
       const uint64_t pair = ALL ? 0 : (uint32_t)list[t0 + t];
       if constexpr (INNER) {
         if (n >= rows) continue;
+        float gb[4], ub[4];
+        biases_of(a.gate, a.out_type, e0, n, gb), biases_of(a.up, a.out_type, e0, n, ub);
         const f32x4 g = sum_of(w, 0, in % 4, t), u = sum_of(w, 1, in % 4, t);
         f32x4 h;
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j)
-          h[j] = activated(g[j] + bias_of(a.gate, a.out_type, e0, n + j), u[j] + bias_of(a.up, a.out_type, e0, n + j));
+        for (uint32_t j = 0; j < 4; ++j) h[j] = activated(g[j] + gb[j], u[j] + ub[j]);
         const uint64_t to = m.p.h + pair * m.p.h_len * 2 + chunk_at(n / 8) * 16 + n % 8 * 2, apart = pairs * (uint64_t)m.p.h_len * 2;
         store_h(a.out_type, to, apart, f32x2{h[0], h[1]}), store_h(a.out_type, to + 4, apart, f32x2{h[2], h[3]});
       } else if (n < rows) {
-        f32x4 v = sum_of(w, rp, in % 4, t);
+        f32x4 v = sum_of(w, 0, in % 4, t);
         if constexpr (ALL) {
           for (uint32_t k = 0; a.down.bias && k < experts; ++k) {
-            const int32_t pair = table[k * CW + t];
+            const int32_t pair = table[k * XC + t];
+            float bias[4];
+            biases_of(a.down, a.out_type, (uint32_t)list[k], n, bias);
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j)
-              if (pair >= 0) v[j] += weights[pair] * bias_of(a.down, a.out_type, (uint32_t)list[k], n + j);
+              if (pair >= 0) v[j] += weights[pair] * bias[j];
           }
           store_out(a, t, n, v);
         } else {
@@ -624,27 +615,28 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
 // columns there.  So LDS is for the weights, NS steps of each wavefront on their way, across the ends of tiles and of
 // experts.  A tile's sums are added up over the wavefronts through LDS, while the next tile's products run.  INNER: of
 // whole rows; else of a chunk of them, each chunk a sum of its own, which the combining kernel adds.
-constexpr uint32_t kStreamGroups = 256;  // a workgroup a compute unit
+constexpr uint32_t kStreamGroups = kComputeUnits;
 constexpr uint32_t kStreamSlots = 16;    // experts of a workgroup, see below
 
 template <bool INNER, int S, int NC>
 __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
-  constexpr int M = INNER ? 2 : 1, NS = 7;
+  constexpr int M = 2, U = M * S, NS = S == 4 ? 8 : S == 2 ? 7 : 5, D = NS % U;  // steps of a tile, on their way
   constexpr uint32_t kCodes = 128, kWords = 32, N = 3;  // chunks and words of a step, its requests
-  constexpr uint32_t kBiasTiles = 32;                   // whose biases are held at a time
+  constexpr uint32_t kBiasTiles = 16;                   // whose biases are held at a time
   __shared__ u32x4 codes[8 * NS * kCodes];
   __shared__ uint32_t scales[8 * NS * kWords];
-  __shared__ f32x4 sums[8 * M * NC * 64];
+  __shared__ f32x2 sums[8 * M * NC * 128];
   __shared__ int16_t chosen[kTokens * kMoeMaxTopK];
+  __shared__ u32x4 none[8];
   __shared__ uint32_t slots[kStreamSlots], share[2];
   __shared__ int32_t list[kTokens];
   __shared__ float biases[M][INNER ? kBiasTiles * 16 : 1];
   const MxMoeArgs& a = m.a;
   const uint32_t lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t rows = INNER ? a.inner : a.cols, length = INNER ? a.cols : a.inner, tiles = rows / 16;
+  const uint32_t rows = INNER ? a.inner : a.cols, length = INNER ? a.cols : a.inner, tiles = rows / (INNER ? 16 : 32);
   const uint32_t x_len = INNER ? m.p.x_len : m.p.h_len, steps = x_len / kStep;
-  const uint32_t span = INNER ? steps : m.span, chunks = INNER ? 1 : m.chunks;
+  const uint32_t span = m.span, chunks = m.chunks;
   const uint32_t parts = INNER ? parts_of(a.x_type) : inner_parts(a.out_type), each = 16 / parts, most = each * NC;
   const uint32_t pairs = (uint32_t)a.tokens * a.top_k;
   auto scalar = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
@@ -698,81 +690,81 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
     return wave < have ? (have - wave + 7) / 8 : 0;
   };
 
-  // What is to be requested next: step `s` of `n` of matrix `r` of a tile, `run` tiles to the end of the expert's or
-  // the chunk's, `left` to the end of all.  Rows come by 32, so all of a tile's are there.
+  // The tile to be requested next, T ahead: of it `n` steps, `run` tiles to the end of the expert's or the chunk's,
+  // `left` to the end of all.  Rows come by 32, so all of a tile's are there.
   struct {
-    uint32_t left, run, slot, chunk, tile, n, s, r;
-    bool tail;
-    uint64_t codes[M], scales[M];  // the tile's first row, at the wavefront's first step
-    uint64_t code, scale;          // at the step
-  } next{left, 0, 0, chunk, tile, 0, 0, 0, false, {}, {}, 0, 0};
+    uint32_t left, run, slot, chunk, tile, n, half;
+    uint64_t codes[M], scales[M];  // the first row, at the wavefront's first step
+  } next{left, 0, 0, chunk, tile, 0, 0, {}, {}};
   auto enter = [&] {
-    while (next.left && (next.n = steps_of(next.chunk)) == 0) {
-      next.left -= min(tiles - next.tile, next.left), next.tile = 0;
-      if (++next.chunk == chunks) next.chunk = 0, ++next.slot;
-    }
-    if (next.left == 0) return;
     const uint32_t e = scalar(slots[next.slot]) & 0xFFFF, step = next.chunk * span + wave;
-    next.run = min(tiles - next.tile, next.left);
-    next.tail = length % kStep && step + (next.n - 1) * 8 == steps - 1;  // half a step at the end
+    next.run = min(tiles - next.tile, next.left), next.n = steps_of(next.chunk);
+    next.half = length % kStep && step + (next.n - 1) * 8 == steps - 1 ? next.n - 1 : ~0u;  // a step that is half one
 #pragma unroll
     for (int r = 0; r < M; ++r) {
       const MxExperts& w = INNER ? (r ? a.up : a.gate) : a.down;
-      next.codes[r] = w.codes.ptr + e * w.codes_expert + (uint64_t)next.tile * 16 * w.codes.stride + step * 128;
-      next.scales[r] = w.scales.ptr + e * w.scales_expert + (uint64_t)next.tile * 16 * w.scales.stride + step * 8;
+      const uint64_t n = INNER ? next.tile * 16 : next.tile * 32 + r * 16;
+      next.codes[r] = w.codes.ptr + e * w.codes_expert + n * w.codes.stride + step * 128;
+      next.scales[r] = w.scales.ptr + e * w.scales_expert + n * w.scales.stride + step * 8;
     }
-    next.code = next.codes[0], next.scale = next.scales[0];
   };
-  const uint64_t code_rows = 16 * (INNER ? a.gate : a.down).codes.stride;
-  const uint64_t scale_rows = 16 * (INNER ? a.gate : a.down).scales.stride;
+  const uint64_t codes_stride = (INNER ? a.gate : a.down).codes.stride, code_rows = codes_stride * (INNER ? 16 : 32);
+  const uint64_t scales_stride = (INNER ? a.gate : a.down).scales.stride, scale_rows = scales_stride * (INNER ? 16 : 32);
+  auto forward = [&] {
+    --next.left;
+    if (--next.run) {
+#pragma unroll
+      for (int r = 0; r < M; ++r) next.codes[r] += code_rows, next.scales[r] += scale_rows;
+    } else if (next.left) {
+      next.tile = 0;
+      if (++next.chunk == chunks) next.chunk = 0, ++next.slot;
+      enter();
+    }
+  };
   const uint32_t codes_at = lds_address(codes) + wave * (NS * kCodes * 16);
   const uint32_t scales_at = lds_address(scales) + wave * (NS * kWords * 4);
+  const uint32_t none_at = scalar(lds_address(none) + wave * 16);
   // A lane's chunks and word from there: in a whole step, and in the half of one, where the last is read over again.
   uint32_t from[2][2], word[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const uint32_t c = (lane & 7) ^ (j * 4 + (lane >> 4)), row = (j * 8 + lane / 8) * (uint32_t)(code_rows / 16);
+    const uint32_t c = (lane & 7) ^ (j * 4 + (lane >> 4)), row = (j * 8 + lane / 8) * (uint32_t)codes_stride;
     from[0][j] = row + c * 16, from[1][j] = row + min(c, 3u) * 16;
   }
-  word[1] = lane / 2 * (uint32_t)(scale_rows / 16), word[0] = word[1] + lane % 2 * 4;
-  auto request = [&](uint32_t at) {
-    const uint32_t stage = scalar(at);
-    const bool half = next.tail && next.s == next.n - 1;
+  word[1] = lane / 2 * (uint32_t)scales_stride, word[0] = word[1] + lane % 2 * 4;
+  // Step u of the tile to the ring's place `at`.  Steps that the tile does not have are requests too, of one lane and to
+  // nowhere, so that a wait can count on them.
+  auto request = [&](uint32_t at, int u) {
+    const int r = u / S, s = u % S;
+    const GlobalBytes code = uniform(next.codes[r] + s * 8 * 128), scale = uniform(next.scales[r] + s * 8 * 8);
+    const uint32_t to = scalar(codes_at + at * (kCodes * 16)), scales_to = scalar(scales_at + at * (kWords * 4));
+    if (s < next.n) {
+      const bool half = s == next.half;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-      dma16(uniform(next.code), half ? from[1][j] : from[0][j], codes_at + (stage * kCodes + j * 64) * 16);
-    if (lane < 32) dma4(uniform(next.scale), half ? word[1] : word[0], scales_at + stage * kWords * 4);
-    if (++next.s < next.n) {
-      next.code += 8 * 128, next.scale += 8 * 8;
-      return;
-    }
-    next.s = 0;
-    if (++next.r == M) {
-      next.r = 0, --next.left;
-      if (--next.run == 0) {
-        next.tile = 0;
-        if (++next.chunk == chunks) next.chunk = 0, ++next.slot;
-        enter();
-        return;
-      }
+      for (int j = 0; j < 2; ++j) dma16_once(code, half ? from[1][j] : from[0][j], to + j * 1024);
+      if (lane < 32) dma4(scale, half ? word[1] : word[0], scales_to);
+    } else if (lane == 0) {
 #pragma unroll
-      for (int r = 0; r < M; ++r) next.codes[r] += code_rows, next.scales[r] += scale_rows;
+      for (uint32_t j = 0; j < N; ++j) dma4(uniform(next.scales[r] - wave * 8), 0, none_at);
     }
-    next.code = next.codes[M > 1 && next.r ? M - 1 : 0], next.scale = next.scales[M > 1 && next.r ? M - 1 : 0];
   };
   enter();
-#pragma unroll 1
+#pragma unroll
   for (uint32_t k = 0; k < NS; ++k)
-    if (next.left) request(k);
+    if (next.left) {
+      request(k, k % U);
+      if (k % U == U - 1) forward();
+    }
+  uint32_t ring = 0;  // where the tile's first step is
 
   // Sums of a tile: every 2 * NC wavefronts in turn add them up, each of 16 columns two rows of every four.
   constexpr uint32_t kTurns = 4 / NC;
   static_assert(4 % NC == 0);
   const uint32_t turn = wave / (2 * NC), group = wave / 2 % NC, n_in = q * 4 + wave % 2 * 2;
-  const uint32_t summed = lds_address(sums) + (group * 64 + lane) * 16 + wave % 2 * 8;
+  const uint32_t summed = lds_address(sums) + (group * 128 + wave % 2 * 64 + lane) * 8;
   const bool biased = INNER && (a.gate.bias || a.up.bias);
   u32x4 x[S][NC][8];
-  uint32_t stage = 0, e = 0, t0 = 0, tokens = 0, used = 0;
+  uint32_t e = 0, t0 = 0, tokens = 0, used = 0;
   bool fresh = true;
   while (left) {
     const uint32_t run = min(tiles - tile, left), mine = steps_of(chunk);
@@ -840,12 +832,13 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
       if constexpr (INNER) {
         if (biased) {
           const uint32_t at = (tile - bias0) * 16 + n_in;
-          v[0] += f32x2{biases[0][at], biases[0][at + 1]}, v[M - 1] += f32x2{biases[M - 1][at], biases[M - 1][at + 1]};
+          v[0] += f32x2{biases[0][at], biases[0][at + 1]}, v[1] += f32x2{biases[1][at], biases[1][at + 1]};
         }
         store_h(m.a.out_type, out + chunk_at(tile * 2) * 16, (uint64_t)pairs * m.p.h_len * 2,
-                f32x2{activated(v[0][0], v[M - 1][0]), activated(v[0][1], v[M - 1][1])});
+                f32x2{activated(v[0][0], v[1][0]), activated(v[0][1], v[1][1])});
       } else {
-        st8(out + tile * 64, __builtin_bit_cast(uint64_t, v[0]));
+#pragma unroll
+        for (int r = 0; r < M; ++r) st8(out + tile * 128 + r * 64, __builtin_bit_cast(uint64_t, v[r]));
       }
     };
     auto walk = [&](auto used_) {
@@ -858,36 +851,47 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
           bias0 = tile + k;
           __syncthreads();
           const uint32_t n = bias0 * 16 + threadIdx.x;
-          static_assert(kBiasTiles * 16 == 512, "a thread a row");
-          if (INNER && n < rows)
-            biases[0][threadIdx.x] = bias_of(a.gate, a.out_type, e, n), biases[M - 1][threadIdx.x] = bias_of(a.up, a.out_type, e, n);
+          static_assert(kBiasTiles * 16 <= 512, "a thread a row");
+          if (INNER && threadIdx.x < kBiasTiles * 16 && n < rows) {
+#pragma unroll
+            for (int r = 0; r < M; ++r) {
+              float bias[1];
+              biases_of(r ? a.up : a.gate, a.out_type, e, n, bias);
+              biases[r][INNER ? threadIdx.x : 0] = bias[0];
+            }
+          }
           __syncthreads();
         }
         f32x4 acc[M][used] = {};
 #pragma unroll
         for (int r = 0; r < M; ++r)
 #pragma unroll
-          for (int s = 0; s < S; ++s)
+          for (int s = 0; s < S; ++s) {
+            const uint32_t at = ring + r * S + s - (ring + r * S + s >= NS ? NS : 0);
             if (s < mine) {
               if (next.left)
                 asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * N) : "memory");
               else
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-              const u32x2 words = *(LdsPairs)(scales_at + stage * (kWords * 4) + i * 8);
+              const u32x2 words = *(LdsPairs)(scales_at + i * 8 + at * (kWords * 4));
               u32x4 w4[2];
 #pragma unroll
               for (int h = 0; h < 2; ++h)
-                w4[h] = *(LdsChunks)(codes_at + (stage * kCodes + i * 8 + ((h * 4 + q) ^ (i / 2))) * 16);
+                w4[h] = *(LdsChunks)(codes_at + (i * 8 + ((h * 4 + q) ^ (i / 2))) * 16 + at * (kCodes * 16));
               asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-              if (next.left) request(stage);  // in place of what has just been read
-              stage = stage + 1 == NS ? 0 : stage + 1;
+              if (next.left) request(at, (r * S + s + D) % U);  // in place of what has just been read
 #pragma unroll
               for (int u = 0; u < 8; ++u) {
-                const u32x4 w8 = weights8(w4[u / 4][u % 4], scale_f32(words[u / 4] >> 8 * q & 0xFF));
+                const u32x4 w8 = weights8(w4[u / 4][u % 4], scale_f32(__builtin_amdgcn_ubfe(words[u / 4], 8 * q, 8)));
 #pragma unroll
                 for (int c = 0; c < used; ++c) acc[r][c] = mfma(w8, x[s][c][u], acc[r][c]);
               }
+            } else if (next.left) {
+              request(at, (r * S + s + D) % U);
             }
+            if ((r * S + s + D) % U == U - 1 && next.left) forward();
+          }
+        ring = ring + U >= NS ? ring + U - NS : ring + U;
         if (open) store(tile + k - 1);
         // Sums to LDS, 16 columns at a time: lane l has rows 4 (l / 16) .. + 3 of column l % 16.
         __builtin_amdgcn_s_barrier();  // the ones before have been read
@@ -895,7 +899,10 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
 #pragma unroll
         for (int r = 0; r < M; ++r)
 #pragma unroll
-          for (int c = 0; c < used; ++c) sums[((wave * M + r) * NC + c) * 64 + lane] = acc[r][c];
+          for (int c = 0; c < used; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              sums[((wave * M + r) * NC + c) * 128 + h * 64 + lane] = f32x2{acc[r][c][2 * h], acc[r][c][2 * h + 1]};
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
@@ -925,18 +932,24 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs m) {
   f32x4 v = {};
   for (uint32_t j0 = 0; j0 < terms; j0 += 4) {  // four at a time on their way
     f32x4 y[4];
-    float weight[4];
+    float weight[4], bias[4][4];
     int32_t e[4];
+    bool first[4];
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
       const uint32_t term = min(j0 + j, terms - 1), k = term / m.chunks;
       const uint64_t pair = t * a.top_k + k;
+      first[j] = term == k * m.chunks;
       e[j] = g_ld<int32_t>(m.p.chosen + pair * 4), weight[j] = g_ld<float>(m.p.weights + pair * 4);
       y[j] = __builtin_bit_cast(f32x4, ld16(m.p.y + (((term - k * m.chunks) * pairs + pair) * a.cols + n) * 4));
-      if (a.down.bias && term == k * m.chunks && e[j] >= 0) {
+    }
+    if (a.down.bias) {
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) y[j][i] += bias_of(a.down, a.out_type, (uint32_t)e[j], n + i);
-      }
+      for (uint32_t j = 0; j < 4; ++j) biases_of(a.down, a.out_type, (uint32_t)max(e[j], 0), n, bias[j]);
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) y[j][i] += first[j] ? bias[j][i] : 0.0f;
     }
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j)
@@ -954,25 +967,25 @@ int dma_of(const MxExperts& w, uint32_t length, uint64_t experts) {
   return length % 128 == 0 && at(w.scales, w.scales_expert, 4) ? 2 : 1;
 }
 
-template <bool INNER, bool ALL, int WR, int KG, int RP, int XC, int NS>
+template <bool INNER, bool ALL, int WR, int KG, int XC, int NS>
 hipError_t product_of(const MoeArgs& m, int dma, hipStream_t stream) {
-  constexpr uint32_t kRows = 16 * RP * WR;
+  constexpr uint32_t kRows = 16 * WR;
   const uint64_t tiles = ((INNER ? m.a.inner : m.a.cols) + kRows - 1) / kRows, pairs = m.a.tokens * m.a.top_k;
   const uint64_t items = ALL ? 1 : pairs < m.a.experts ? pairs : m.a.experts;
-  return launch(dma == 2   ? moe_product_kernel<INNER, ALL, WR, KG, RP, XC, NS, 2>
-                : dma == 1 ? moe_product_kernel<INNER, ALL, WR, KG, RP, XC, NS, 1>
-                           : moe_product_kernel<INNER, ALL, WR, KG, RP, XC, NS, 0>,
+  return launch(dma == 2   ? moe_product_kernel<INNER, ALL, WR, KG, XC, NS, 2>
+                : dma == 1 ? moe_product_kernel<INNER, ALL, WR, KG, XC, NS, 1>
+                           : moe_product_kernel<INNER, ALL, WR, KG, XC, NS, 0>,
                 items * tiles, 64 * WR * KG, m, stream);
 }
 
 // 16 rows as 32-bit offsets.
 bool near_rows(const MxExperts& w) { return w.codes.stride < 1ull << 27 && w.scales.stride < 1ull << 27; }
 
-// S steps of a wavefront; false if the rows are too long for that, or too short to keep most of eight busy.
-bool chunks_of(uint32_t len, bool inner, uint32_t s, MoeArgs& m) {
-  const uint32_t steps = len / kStep, most = 8 * s, chunks = (steps + most - 1) / most;
-  if (steps < 5 || chunks > (inner ? 1 : kChunks)) return false;
-  if (!inner) m.span = (steps + chunks - 1) / chunks, m.chunks = (steps + m.span - 1) / m.span;
+// Cuts rows into chunks, at most `most` of them, of which a wavefront has s steps at most.
+bool chunks_of(uint32_t len, uint32_t most, uint32_t s, MoeArgs& m) {
+  const uint32_t steps = len / kStep, chunks = (steps + 8 * s - 1) / (8 * s);
+  if (chunks > most) return false;
+  m.span = (steps + chunks - 1) / chunks, m.chunks = (steps + m.span - 1) / m.span;
   return true;
 }
 template <bool INNER, int S, int NC>
@@ -998,7 +1011,7 @@ hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
   const int gate = dma_of(a.gate, a.cols, a.experts), up = dma_of(a.up, a.cols, a.experts);
   const int inner = gate < up ? gate : up, outer = dma_of(a.down, a.inner, a.experts);
   return in_parts(a.tokens, kTokens, [&](uint64_t first, uint64_t tokens) {
-    MoeArgs m{a, places_of(a), 1, 1};
+    MoeArgs m{a, places_of(a), 1, 1, false};
     m.a.tokens = tokens;
     m.a.x = rows_from(a.x, first, type_bytes(a.x_type)), m.a.out = rows_from(a.out, first, type_bytes(a.out_type));
     if (a.experts_out) m.a.experts_out += first * a.top_k * 4;
@@ -1006,30 +1019,27 @@ hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
     hipError_t e = logits_of(m, stream);
     const uint64_t pairs = tokens * a.top_k;
     const uint32_t xp = parts_of(a.x_type), hp = inner_parts(a.out_type);
-    const bool few_inner = tokens * xp <= 4, few_outer = tokens * hp <= 4 && pairs <= 64;
-    if (e == hipSuccess && pairs > kFusedPairs) e = launch(moe_route_kernel, tokens, 64, m, stream);
+    const bool stream_inner = tokens > 1 && inner == 2 && a.cols > 2048 && near_rows(a.gate) && near_rows(a.up) &&
+                              a.gate.codes.stride == a.up.codes.stride && a.gate.scales.stride == a.up.scales.stride &&
+                              chunks_of(m.p.x_len, 1, 4, m);
+    if (e == hipSuccess && (pairs > kFusedPairs || stream_inner)) e = launch(moe_route_kernel, tokens, 64, m, stream);
+    m.routed = pairs > kFusedPairs || stream_inner;
     if (e != hipSuccess) return e;
-    // columns that an expert's tokens take on average
-    const double inner_columns = (double)pairs / a.experts * xp, outer_columns = (double)pairs / a.experts * hp;
-    const bool stream_inner = pairs > kFusedPairs && inner == 2 && near_rows(a.gate) &&
-                              a.gate.codes.stride == a.up.codes.stride && a.gate.scales.stride == a.up.scales.stride;
-    const bool stream_outer = pairs > kFusedPairs && outer == 2 && near_rows(a.down);
-    if (few_inner)
-      e = product_of<true, false, 1, 4, 1, 4, 2>(m, inner, stream);
-    else if (stream_inner && inner_columns > 8 && chunks_of(m.p.x_len, true, 2, m))
+    const uint64_t groups = (pairs < a.experts ? pairs : a.experts) * ((a.inner + 63) / 64);
+    if (tokens * xp <= 4 && groups < kComputeUnits && !stream_inner)
+      e = product_of<true, false, 1, 4, 4, 2>(m, inner, stream);
+    else if (stream_inner && m.p.x_len <= 16 * kStep)
       e = stream_of<true, 2, 2>(m, stream);
-    else if (stream_inner && chunks_of(m.p.x_len, true, 4, m))
+    else if (stream_inner)
       e = stream_of<true, 4, 1>(m, stream);
     else
-      e = product_of<true, false, 4, 1, 1, 16, 3>(m, inner, stream);
+      e = product_of<true, false, 4, 1, 16, 3>(m, inner, stream);
     if (e != hipSuccess) return e;
-    if (few_outer) return product_of<false, true, 1, 8, 1, 4, 3>(m, outer, stream);
-    if (stream_outer && outer_columns > 8 && chunks_of(m.p.h_len, false, 1, m))
+    if (tokens * hp <= 4 && pairs <= 64) return product_of<false, true, 1, 8, 4, 3>(m, outer, stream);
+    if (outer == 2 && a.inner > 1024 && near_rows(a.down) && chunks_of(m.p.h_len, kChunks, 1, m))
       e = stream_of<false, 1, 4>(m, stream);
-    else if (stream_outer && chunks_of(m.p.h_len, false, 4, m))
-      e = stream_of<false, 4, 1>(m, stream);
     else
-      e = product_of<false, false, 4, 1, 1, 16, 3>(m, outer, stream);
+      e = product_of<false, false, 4, 1, 16, 3>(m, outer, stream);
     if (e == hipSuccess) e = launch(moe_combine_kernel, (tokens * (a.cols / 4) + 255) / 256, 256, m, stream);
     return e;
   });
