@@ -609,7 +609,7 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
   }
 }
 
-// The same products where an expert has several tokens and its weights go through LDS whole (kDma 2): the columns stay
+// The same products where an expert has several tokens and its codes lie at multiples of 16 bytes: the columns stay
 // in registers.  A workgroup walks along consecutive tiles of 16 rows, of one expert after the other; of a tile's rows
 // wavefront w of eight has steps w, w + 8, ... of a chunk of the rows, S at most, and keeps the values of 16 * NC
 // columns there.  So LDS is for the weights, NS steps of each wavefront on their way, across the ends of tiles and of
@@ -620,8 +620,8 @@ constexpr uint32_t kStreamSlots = 16;    // experts of a workgroup, see below
 
 template <bool INNER, int S, int NC>
 __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
-  constexpr int M = 2, U = M * S, NS = S == 4 ? 8 : S == 2 ? 7 : 5, D = NS % U;  // steps of a tile, on their way
-  constexpr uint32_t kCodes = 128, kWords = 32, N = 3;  // chunks and words of a step, its requests
+  constexpr int M = 2, U = M * S, NS = S == 4 ? 7 : S == 2 ? 6 : 5, D = NS % U;  // steps of a tile, on their way
+  constexpr uint32_t kCodes = 128, kWords = 64, N = 3;  // chunks and words of a step, its requests
   constexpr uint32_t kBiasTiles = 16;                   // whose biases are held at a time
   __shared__ u32x4 codes[8 * NS * kCodes];
   __shared__ uint32_t scales[8 * NS * kWords];
@@ -692,20 +692,32 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
 
   // The tile to be requested next, T ahead: of it `n` steps, `run` tiles to the end of the expert's or the chunk's,
   // `left` to the end of all.  Rows come by 32, so all of a tile's are there.
+  auto part_of = [&](uint32_t chunk, uint32_t n) {  // which of n steps is only part of one
+    return length % kStep && chunk * span + wave + (n - 1) * 8 == steps - 1 ? n - 1 : ~0u;
+  };
   struct {
-    uint32_t left, run, slot, chunk, tile, n, half;
-    uint64_t codes[M], scales[M];  // the first row, at the wavefront's first step
+    uint32_t left, run, slot, chunk, tile, n, part;
+    uint64_t codes[M], scales[M];  // the first row, at the wavefront's first step; scales at words
   } next{left, 0, 0, chunk, tile, 0, 0, {}, {}};
+  // A lane's chunks and word from there, in a whole step and in the part of one that a row may end with, where the last
+  // chunk is read over again.  A step's eight scales are at any byte, within three words, of which only those are read
+  // that hold one of the row's own.
+  uint32_t from[2][2], word[M][2];
+  const uint32_t last = (length - 1) / kMxBlock % 8;  // block of the last step
   auto enter = [&] {
     const uint32_t e = scalar(slots[next.slot]) & 0xFFFF, step = next.chunk * span + wave;
     next.run = min(tiles - next.tile, next.left), next.n = steps_of(next.chunk);
-    next.half = length % kStep && step + (next.n - 1) * 8 == steps - 1 ? next.n - 1 : ~0u;  // a step that is half one
+    next.part = part_of(next.chunk, next.n);
 #pragma unroll
     for (int r = 0; r < M; ++r) {
       const MxExperts& w = INNER ? (r ? a.up : a.gate) : a.down;
       const uint64_t n = INNER ? next.tile * 16 : next.tile * 32 + r * 16;
       next.codes[r] = w.codes.ptr + e * w.codes_expert + n * w.codes.stride + step * 128;
-      next.scales[r] = w.scales.ptr + e * w.scales_expert + n * w.scales.stride + step * 8;
+      const uint64_t at = w.scales.ptr + e * w.scales_expert + n * w.scales.stride + step * 8;
+      const uint32_t row = (uint32_t)at % 4 + lane / 4 * (uint32_t)w.scales.stride;  // bytes from at's word
+      next.scales[r] = at / 4 * 4;
+      word[r][0] = (row / 4 + min(lane % 4, (row % 4 + 7) / 4)) * 4;
+      word[r][1] = (row / 4 + min(lane % 4, (row % 4 + last) / 4)) * 4;
     }
   };
   const uint64_t codes_stride = (INNER ? a.gate : a.down).codes.stride, code_rows = codes_stride * (INNER ? 16 : 32);
@@ -724,14 +736,11 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
   const uint32_t codes_at = lds_address(codes) + wave * (NS * kCodes * 16);
   const uint32_t scales_at = lds_address(scales) + wave * (NS * kWords * 4);
   const uint32_t none_at = scalar(lds_address(none) + wave * 16);
-  // A lane's chunks and word from there: in a whole step, and in the half of one, where the last is read over again.
-  uint32_t from[2][2], word[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const uint32_t c = (lane & 7) ^ (j * 4 + (lane >> 4)), row = (j * 8 + lane / 8) * (uint32_t)codes_stride;
-    from[0][j] = row + c * 16, from[1][j] = row + min(c, 3u) * 16;
+    from[0][j] = row + c * 16, from[1][j] = row + min(c, last) * 16;
   }
-  word[1] = lane / 2 * (uint32_t)scales_stride, word[0] = word[1] + lane % 2 * 4;
   // Step u of the tile to the ring's place `at`.  Steps that the tile does not have are requests too, of one lane and to
   // nowhere, so that a wait can count on them.
   auto request = [&](uint32_t at, int u) {
@@ -739,13 +748,13 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
     const GlobalBytes code = uniform(next.codes[r] + s * 8 * 128), scale = uniform(next.scales[r] + s * 8 * 8);
     const uint32_t to = scalar(codes_at + at * (kCodes * 16)), scales_to = scalar(scales_at + at * (kWords * 4));
     if (s < next.n) {
-      const bool half = s == next.half;
+      const bool part = s == next.part;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) dma16_once(code, half ? from[1][j] : from[0][j], to + j * 1024);
-      if (lane < 32) dma4(scale, half ? word[1] : word[0], scales_to);
+      for (int j = 0; j < 2; ++j) dma16_once(code, part ? from[1][j] : from[0][j], to + j * 1024);
+      dma4(scale, part ? word[r][1] : word[r][0], scales_to);
     } else if (lane == 0) {
 #pragma unroll
-      for (uint32_t j = 0; j < N; ++j) dma4(uniform(next.scales[r] - wave * 8), 0, none_at);
+      for (uint32_t j = 0; j < N; ++j) dma4(uniform(next.scales[r] - wave * 8), word[r][1], none_at);
     }
   };
   enter();
@@ -756,6 +765,7 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
       if (k % U == U - 1) forward();
     }
   uint32_t ring = 0;  // where the tile's first step is
+  auto wrapped = [](uint32_t at) { return at >= NS ? at - NS : at; };
 
   // Sums of a tile: every 2 * NC wavefronts in turn add them up, each of 16 columns two rows of every four.
   constexpr uint32_t kTurns = 4 / NC;
@@ -764,6 +774,10 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
   const uint32_t summed = lds_address(sums) + (group * 128 + wave % 2 * 64 + lane) * 8;
   const bool biased = INNER && (a.gate.bias || a.up.bias);
   u32x4 x[S][NC][8];
+  // A block's scale among a step's eight, blocks past the row's end having the last one's.
+  uint32_t pick[2][2], shift[M] = {};
+#pragma unroll
+  for (uint32_t h = 0; h < 2; ++h) pick[0][h] = (h * 4 + q) | 0x0C0C0C00, pick[1][h] = min(h * 4 + q, last) | 0x0C0C0C00;
   uint32_t e = 0, t0 = 0, tokens = 0, used = 0;
   bool fresh = true;
   while (left) {
@@ -778,16 +792,22 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
       if (pair >= 0) list[__popcll(mask & ((1ull << lane) - 1))] = pair;
       tokens = min((uint32_t)__popcll(mask) - t0, most), used = (tokens + each - 1) / each;
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int r = 0; r < M; ++r) {  // bytes from a word to the row's first scale
+        const MxExperts& w = INNER ? (r ? a.up : a.gate) : a.down;
+        shift[r] = (uint32_t)(w.scales.ptr + e * w.scales_expert + i * w.scales.stride) % 4;
+      }
       fresh = false;
     }
+    const uint32_t part = part_of(chunk, mine);
     const GlobalBytes x0 = global_bytes(INNER ? m.p.x : m.p.h);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       if (c < used) {
-        uint32_t t = c * each + i / parts, part = i % parts;  // columns without a token repeat the first
-        if (i >= each * parts || t >= tokens) t = 0, part = 0;
+        uint32_t t = c * each + i / parts, p = i % parts;  // columns without a token repeat the first
+        if (i >= each * parts || t >= tokens) t = 0, p = 0;
         const uint32_t pair = (uint32_t)list[t0 + t];
-        const uint32_t row = INNER ? part * (uint32_t)a.tokens + pair / a.top_k : part * pairs + pair;
+        const uint32_t row = INNER ? p * (uint32_t)a.tokens + pair / a.top_k : p * pairs + pair;
         const uint32_t at = row * x_len * 2 + (chunk * span + wave) * (kStep * 2) + q * 16;
 #pragma unroll
         for (int s = 0; s < S; ++s)
@@ -867,22 +887,28 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
         for (int r = 0; r < M; ++r)
 #pragma unroll
           for (int s = 0; s < S; ++s) {
-            const uint32_t at = ring + r * S + s - (ring + r * S + s >= NS ? NS : 0);
+            const uint32_t at = wrapped(ring + (r * S + s) % NS);
             if (s < mine) {
               if (next.left)
                 asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * N) : "memory");
               else
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-              const u32x2 words = *(LdsPairs)(scales_at + i * 8 + at * (kWords * 4));
+              const u32x4 words = *(LdsChunks)(scales_at + i * 16 + at * (kWords * 4));
               u32x4 w4[2];
 #pragma unroll
               for (int h = 0; h < 2; ++h)
                 w4[h] = *(LdsChunks)(codes_at + (i * 8 + ((h * 4 + q) ^ (i / 2))) * 16 + at * (kCodes * 16));
               asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
               if (next.left) request(at, (r * S + s + D) % U);  // in place of what has just been read
+              const uint32_t low = __builtin_amdgcn_alignbyte(words[1], words[0], shift[r]);
+              const uint32_t high = __builtin_amdgcn_alignbyte(words[2], words[1], shift[r]);
+              float scale[2];
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                scale[h] = scale_f32(__builtin_amdgcn_perm(high, low, s == part ? pick[1][h] : pick[0][h]));
 #pragma unroll
               for (int u = 0; u < 8; ++u) {
-                const u32x4 w8 = weights8(w4[u / 4][u % 4], scale_f32(__builtin_amdgcn_ubfe(words[u / 4], 8 * q, 8)));
+                const u32x4 w8 = weights8(w4[u / 4][u % 4], scale[u / 4]);
 #pragma unroll
                 for (int c = 0; c < used; ++c) acc[r][c] = mfma(w8, x[s][c][u], acc[r][c]);
               }
@@ -891,7 +917,7 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
             }
             if ((r * S + s + D) % U == U - 1 && next.left) forward();
           }
-        ring = ring + U >= NS ? ring + U - NS : ring + U;
+        ring = wrapped(ring + U % NS);
         if (open) store(tile + k - 1);
         // Sums to LDS, 16 columns at a time: lane l has rows 4 (l / 16) .. + 3 of column l % 16.
         __builtin_amdgcn_s_barrier();  // the ones before have been read
@@ -1019,7 +1045,7 @@ hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
     hipError_t e = logits_of(m, stream);
     const uint64_t pairs = tokens * a.top_k;
     const uint32_t xp = parts_of(a.x_type), hp = inner_parts(a.out_type);
-    const bool stream_inner = tokens > 1 && inner == 2 && a.cols > 2048 && near_rows(a.gate) && near_rows(a.up) &&
+    const bool stream_inner = tokens > 1 && inner > 0 && a.cols > 2048 && near_rows(a.gate) && near_rows(a.up) &&
                               a.gate.codes.stride == a.up.codes.stride && a.gate.scales.stride == a.up.scales.stride &&
                               chunks_of(m.p.x_len, 1, 4, m);
     if (e == hipSuccess && (pairs > kFusedPairs || stream_inner)) e = launch(moe_route_kernel, tokens, 64, m, stream);
@@ -1036,7 +1062,7 @@ hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
       e = product_of<true, false, 4, 1, 16, 3>(m, inner, stream);
     if (e != hipSuccess) return e;
     if (tokens * hp <= 4 && pairs <= 64) return product_of<false, true, 1, 8, 4, 3>(m, outer, stream);
-    if (outer == 2 && a.inner > 1024 && near_rows(a.down) && chunks_of(m.p.h_len, kChunks, 1, m))
+    if (outer > 0 && a.inner > 1024 && near_rows(a.down) && chunks_of(m.p.h_len, kChunks, 1, m))
       e = stream_of<false, 1, 4>(m, stream);
     else
       e = product_of<false, false, 4, 1, 16, 3>(m, outer, stream);

@@ -14,6 +14,9 @@ SIZES = [  # tokens, experts, top_k, cols, inner: steps of 256 values, whole and
     (64, 1, 1, 2176, 8192), (17, 300, 2, 2560, 1152), (40, 6, 6, 8064, 1408), (65, 3, 2, 8192, 2304), (8, 2, 1, 8320, 1280),
     (5, 3, 2, 64, 32768), (4, 2, 2, 96, 32896), (64, 4, 4, 2304, 1024), (64, 40, 32, 2304, 1152), (63, 1024, 2, 64, 1152),
     (16, 8, 2, 5120, 32), (50, 7, 1, 32, 14336),
+    # rows of blocks that are no multiple of four: scales at any byte, one to seven blocks in the last step
+    (7, 3, 2, 2080, 1056), (30, 4, 2, 2112, 1184), (64, 5, 2, 2144, 1248), (21, 6, 3, 4128, 1504), (40, 2, 1, 5056, 2400),
+    (12, 4, 2, 8160, 4320), (10, 2, 1, 3360, 14304), (64, 33, 4, 2272, 1312),
 ]
 
 
