@@ -328,22 +328,22 @@ constexpr uint32_t kFusedPairs = 32;
 // once.  In a product lane l takes block l / 16 of row (column) l % 16, values
 // 8f .. 8f+7 with product f of four.
 //
-// kDma 2: codes lie at multiples of 16 bytes and scales of 4, whole words of
-// four blocks; 1: codes only, scales come byte by byte; 0: codes go through
-// registers.
-template <bool INNER, bool ALL, int WR, int KG, int XC, int NS, int kDma>
+// A step's eight scales of a row lie at any byte, within three words, of which
+// those come that hold one of the row's own; four lanes a row.  kDma: codes lie
+// at multiples of 16 bytes; else they go through registers.
+template <bool INNER, bool ALL, int WR, int KG, int XC, int NS, bool kDma>
 __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
   static_assert(WR == 1 || KG == 1, "groups of several wavefronts meet at barriers of the whole workgroup");
   static_assert(!(INNER && ALL) && XC <= 16, "a product has 16 columns");
   constexpr int M = INNER ? 2 : 1;  // matrices
   constexpr uint32_t G = 64 * WR, kWaves = WR * KG, kRows = 16 * WR;
   constexpr uint32_t kCodes = M * 128, kColumns = XC * 32;  // chunks of a stage
-  constexpr int JW = kCodes / 64, JX = kColumns / G, JS = kDma == 2 ? 1 : 2 * M;
-  constexpr int N = JX + (kDma > 0 ? JW : 0) + JS;  // requests of a step
+  constexpr int JW = kCodes / 64, JX = kColumns / G, JS = M;
+  constexpr int N = JX + (kDma ? JW : 0) + JS;  // requests of a step
   constexpr uint32_t kScales = JS * 64;                                          // words of a stage
   static_assert(kColumns % G == 0 && (NS - 2) * N < 64, "whole requests, and a wait that counts them");
   __shared__ u32x4 columns[KG * NS * kColumns], codes[KG * WR * NS * kCodes];
-  __shared__ uint32_t scales[KG * WR * NS * kScales];
+  __shared__ u32x4 scales[KG * WR * NS * kScales / 4];
   __shared__ int32_t list[64], table[ALL ? 64 * XC : 1], fused[INNER ? kFusedPairs : 1];
   __shared__ float weights[ALL ? 64 : 1];
   const MxMoeArgs& a = m.a;
@@ -421,12 +421,9 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
     const MxExperts& w = matrix(j / 2);
     w_at[j] = w.codes.ptr + e0 * w.codes_expert + row_of(j % 2 * 8 + lane / 8) * w.codes.stride;
   }
-  if constexpr (kDma == 2) {  // two words a row
-    s_at[0] = M == 2 && lane >= 32 ? scales_of(1, row_of(lane / 2 % 16)) : scales_of(0, row_of(lane / 2 % 16));
-  } else {  // eight bytes a row
+  uint32_t shift[M];  // bytes from a word to the scales of row i, the expert's aside
 #pragma unroll
-    for (int j = 0; j < JS; ++j) s_at[j] = scales_of(j / 2, row_of(j % 2 * 8 + lane / 8));
-  }
+  for (int j = 0; j < JS; ++j) s_at[j] = scales_of(j, row_of(lane / 4)), shift[j] = (uint32_t)scales_of(j, row_of(i));
   const uint32_t columns_at = lds_address(columns) + group * (NS * kColumns * 16);
   const uint32_t codes_at = lds_address(codes) + wave * (NS * kCodes * 16);
   const uint32_t scales_at = lds_address(scales) + wave * (NS * kScales * 4);
@@ -467,19 +464,16 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
       for (int j = 0; j < JW; ++j) {
         const uint32_t chunk = (lane & 7) ^ (j * 4 + (lane >> 4) & 7);
         const uint64_t from = w_at[j] + e * a.down.codes_expert + min(u.step * 8 + chunk, blocks - 1) * 16;
-        if constexpr (kDma > 0)
+        if constexpr (kDma)
           dma16_once(from, codes_at + (stage * kCodes + j * 64) * 16);
         else
           ((LdsChunks)(codes_at + (stage * kCodes + lane) * 16))[j * 64] = ld16(from);
       }
+      const uint32_t last = min(blocks - 1 - u.step * 8, 7u);  // block of the step
 #pragma unroll
       for (int j = 0; j < JS; ++j) {
-        const uint64_t from = s_at[j] + e * a.down.scales_expert;
-        const uint32_t to = scales_at + (stage * kScales + j * 64) * 4;
-        if constexpr (kDma == 2)
-          dma4(from + min(u.step * 2 + (lane & 1), blocks / 4 - 1) * 4, to);
-        else
-          dma1(from + min(u.step * 8 + (lane & 7), blocks - 1), to);
+        const uint64_t from = s_at[j] + e * a.down.scales_expert + u.step * 8;
+        dma4(from / 4 * 4 + min(lane % 4, ((uint32_t)from % 4 + last) / 4) * 4, scales_at + (stage * kScales + j * 64) * 4);
       }
 #pragma unroll
       for (int j = 0; j < JX; ++j) {
@@ -493,23 +487,24 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
       }
     };
     f32x4 acc[M] = {}, total = {};
-    auto compute = [&](uint32_t stage) {
-      u32x2 words[M];
-      if constexpr (kDma == 2) {
-#pragma unroll
-        for (int r = 0; r < M; ++r) words[r] = *(LdsPairs)(scales_at + stage * (kScales * 4) + (r * 16 + i) * 8);
-      }
+    auto compute = [&](const Unit& now, uint32_t stage) {
+      const uint32_t last = min(blocks - 1 - now.step * 8, 7u);
+      const uint32_t expert = ALL ? (uint32_t)(expert_of(now) * a.down.scales_expert) : 0;
       u32x4 wv[2][M];
       float sf[2][M];
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int r = 0; r < M; ++r) {
+        const u32x4 words = *(LdsChunks)(scales_at + (stage * kScales + (r * 16 + i) * 4) * 4);
+        const uint32_t low = __builtin_amdgcn_alignbyte(words[1], words[0], (shift[r] + expert) % 4);
+        const uint32_t high = __builtin_amdgcn_alignbyte(words[2], words[1], (shift[r] + expert) % 4);
 #pragma unroll
-        for (int r = 0; r < M; ++r) {
+        for (int s = 0; s < 2; ++s) {
           const uint32_t row = r * 16 + i, c = s * 4 + q;
           wv[s][r] = *(LdsChunks)(codes_at + (stage * kCodes + row * 8 + (c ^ (row / 2 & 7))) * 16);
-          sf[s][r] = scale_f32(kDma == 2 ? words[r][s] >> 8 * q & 0xFF
-                                         : *(LdsWord)(scales_at + (stage * kScales + row * 8 + c) * 4));
+          // blocks past the row's end have the last one's
+          sf[s][r] = scale_f32(__builtin_amdgcn_perm(high, low, min(c, last) | 0x0C0C0C00));
         }
+      }
       const uint32_t column = i % XC;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
@@ -553,7 +548,7 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
           request(ahead, into);
           if (k + NS < n) forward(ahead);
         }
-        compute(stage);
+        compute(now, stage);
         if constexpr (ALL) {
           if (k + 1 == n || next.k != now.k) add_expert(now.k);
         }
@@ -955,52 +950,53 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs m) {
   if (t >= a.tokens) return;
   const uint64_t pairs = a.tokens * a.top_k;
   const uint32_t terms = a.top_k * m.chunks;
+  constexpr uint32_t kAhead = 8;  // terms on their way at a time
   f32x4 v = {};
-  for (uint32_t j0 = 0; j0 < terms; j0 += 4) {  // four at a time on their way
-    f32x4 y[4];
-    float weight[4], bias[4][4];
-    int32_t e[4];
-    bool first[4];
+  for (uint32_t j0 = 0; j0 < terms; j0 += kAhead) {
+    f32x4 y[kAhead];
+    float weight[kAhead];
+    int32_t e[kAhead];
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) {
+    for (uint32_t j = 0; j < kAhead; ++j) {
       const uint32_t term = min(j0 + j, terms - 1), k = term / m.chunks;
       const uint64_t pair = t * a.top_k + k;
-      first[j] = term == k * m.chunks;
       e[j] = g_ld<int32_t>(m.p.chosen + pair * 4), weight[j] = g_ld<float>(m.p.weights + pair * 4);
       y[j] = __builtin_bit_cast(f32x4, ld16(m.p.y + (((term - k * m.chunks) * pairs + pair) * a.cols + n) * 4));
     }
-    if (a.down.bias) {
 #pragma unroll
-      for (uint32_t j = 0; j < 4; ++j) biases_of(a.down, a.out_type, (uint32_t)max(e[j], 0), n, bias[j]);
+    for (uint32_t j = 0; j < kAhead; ++j)
+      if (j0 + j < terms && e[j] >= 0) v += weight[j] * y[j];
+  }
+  for (uint32_t k0 = 0; a.down.bias && k0 < a.top_k; k0 += 4) {
+    float weight[4], bias[4][4];
+    int32_t e[4];
 #pragma unroll
-      for (uint32_t j = 0; j < 4; ++j)
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) y[j][i] += first[j] ? bias[j][i] : 0.0f;
+    for (uint32_t k = 0; k < 4; ++k) {
+      const uint64_t pair = t * a.top_k + min(k0 + k, a.top_k - 1);
+      e[k] = g_ld<int32_t>(m.p.chosen + pair * 4), weight[k] = g_ld<float>(m.p.weights + pair * 4);
+      biases_of(a.down, a.out_type, (uint32_t)max(e[k], 0), n, bias[k]);
     }
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j)
-      if (j0 + j < terms && e[j] >= 0) v += weight[j] * y[j];
+    for (uint32_t k = 0; k < 4; ++k)
+      if (k0 + k < a.top_k && e[k] >= 0)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += weight[k] * bias[k][i];
   }
   store_out(a, t, n, v);
 }
 
-// How far the weights of one product go by DMA.
-int dma_of(const MxExperts& w, uint32_t length, uint64_t experts) {
-  const auto at = [&](const MxRows& r, uint64_t expert, uint64_t n) {
-    return r.ptr % n == 0 && r.stride % n == 0 && (experts == 1 || expert % n == 0);
-  };
-  if (!at(w.codes, w.codes_expert, 16)) return 0;
-  return length % 128 == 0 && at(w.scales, w.scales_expert, 4) ? 2 : 1;
+// Codes at multiples of 16 bytes.
+bool dma_of(const MxExperts& w, uint64_t experts) {
+  return w.codes.ptr % 16 == 0 && w.codes.stride % 16 == 0 && (experts == 1 || w.codes_expert % 16 == 0);
 }
 
 template <bool INNER, bool ALL, int WR, int KG, int XC, int NS>
-hipError_t product_of(const MoeArgs& m, int dma, hipStream_t stream) {
+hipError_t product_of(const MoeArgs& m, bool dma, hipStream_t stream) {
   constexpr uint32_t kRows = 16 * WR;
   const uint64_t tiles = ((INNER ? m.a.inner : m.a.cols) + kRows - 1) / kRows, pairs = m.a.tokens * m.a.top_k;
   const uint64_t items = ALL ? 1 : pairs < m.a.experts ? pairs : m.a.experts;
-  return launch(dma == 2   ? moe_product_kernel<INNER, ALL, WR, KG, XC, NS, 2>
-                : dma == 1 ? moe_product_kernel<INNER, ALL, WR, KG, XC, NS, 1>
-                           : moe_product_kernel<INNER, ALL, WR, KG, XC, NS, 0>,
+  return launch(dma ? moe_product_kernel<INNER, ALL, WR, KG, XC, NS, true>
+                    : moe_product_kernel<INNER, ALL, WR, KG, XC, NS, false>,
                 items * tiles, 64 * WR * KG, m, stream);
 }
 
@@ -1034,8 +1030,7 @@ hipError_t logits_of(const MoeArgs& m, hipStream_t stream) {
 uint64_t mxfp4_moe_workspace(const MxMoeArgs& a) { return places_of(a).end - a.workspace; }
 
 hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
-  const int gate = dma_of(a.gate, a.cols, a.experts), up = dma_of(a.up, a.cols, a.experts);
-  const int inner = gate < up ? gate : up, outer = dma_of(a.down, a.inner, a.experts);
+  const bool inner = dma_of(a.gate, a.experts) && dma_of(a.up, a.experts), outer = dma_of(a.down, a.experts);
   return in_parts(a.tokens, kTokens, [&](uint64_t first, uint64_t tokens) {
     MoeArgs m{a, places_of(a), 1, 1, false};
     m.a.tokens = tokens;
@@ -1045,7 +1040,7 @@ hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
     hipError_t e = logits_of(m, stream);
     const uint64_t pairs = tokens * a.top_k;
     const uint32_t xp = parts_of(a.x_type), hp = inner_parts(a.out_type);
-    const bool stream_inner = tokens > 1 && inner > 0 && a.cols > 2048 && near_rows(a.gate) && near_rows(a.up) &&
+    const bool stream_inner = tokens > 1 && inner && a.cols > 2048 && near_rows(a.gate) && near_rows(a.up) &&
                               a.gate.codes.stride == a.up.codes.stride && a.gate.scales.stride == a.up.scales.stride &&
                               chunks_of(m.p.x_len, 1, 4, m);
     if (e == hipSuccess && (pairs > kFusedPairs || stream_inner)) e = launch(moe_route_kernel, tokens, 64, m, stream);
@@ -1059,10 +1054,11 @@ hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
     else if (stream_inner)
       e = stream_of<true, 4, 1>(m, stream);
     else
-      e = product_of<true, false, 4, 1, 16, 3>(m, inner, stream);
+      e = product_of<true, false, 4, 1, 16, 2>(m, inner, stream);
     if (e != hipSuccess) return e;
-    if (tokens * hp <= 4 && pairs <= 64) return product_of<false, true, 1, 8, 4, 3>(m, outer, stream);
-    if (outer > 0 && a.inner > 1024 && near_rows(a.down) && chunks_of(m.p.h_len, kChunks, 1, m))
+    if (tokens * hp <= 4 && pairs <= 64 && (a.cols >= 2048 || pairs * (m.p.h_len / kStep) <= 64))
+      return product_of<false, true, 1, 8, 4, 3>(m, outer, stream);
+    if (outer && a.inner > 1024 && near_rows(a.down) && chunks_of(m.p.h_len, kChunks, 1, m))
       e = stream_of<false, 1, 4>(m, stream);
     else
       e = product_of<false, false, 4, 1, 16, 3>(m, outer, stream);
