@@ -12,6 +12,10 @@
 //   inner    gate and up products of an expert's tokens, h as bf16 parts
 //   outer    the down products; of a few tokens, their weighted sums at once
 //   combine  (many tokens) the weighted sums
+// Inner and outer products are each one of two kernels: moe_product_kernel, a
+// workgroup a few rows of an expert, whose columns go through LDS beside the
+// weights, and moe_stream_kernel, a workgroup a compute unit for all of a
+// launch, whose columns stay in registers.
 //
 // The products are of bf16 on the matrix unit.  Weights are widened to bf16,
 // which is exact; x, and h, are the sum of one to three bf16 values (parts),
@@ -33,7 +37,7 @@ constexpr uint32_t kComputeUnits = 256;
 constexpr uint32_t kTokens = 64;  // of a launch; longer calls run in several
 constexpr uint32_t kStep = 256;   // values of a row that go through LDS together: a cache line of codes
 
-// h's parts: 24 significant bits where the outputs have 24, else 16, the rounding of a 2^-8 or 2^-5 of the output's own.
+// h's parts: 24 significant bits where the outputs have 24, else 16, whose rounding is 2^-8 or 2^-5 of the output's own.
 constexpr uint32_t inner_parts(uint32_t out_type) { return out_type == kTypeF32 ? 3 : 2; }
 
 // Where a launch's intermediate results lie in the workspace.  A pair is a token's k-th expert, token * top_k + k.
@@ -223,7 +227,7 @@ __device__ __forceinline__ double logit_of(uint64_t order) {
   return __builtin_bit_cast(double, order >> 63 ? order ^ 1ull << 63 : ~order);
 }
 
-// The largest of a wavefront's values, in all lanes.
+// The largest of a wavefront's values, in all lanes.  By DPP: eight choices of 128 experts through LDS took 2 us more.
 template <int CTRL>
 __device__ __forceinline__ uint32_t larger_by(uint32_t v) {
   return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false));
@@ -259,7 +263,8 @@ __device__ __forceinline__ Chosen choose_of(const MoeArgs& m, uint32_t t) {
     // by the upper halves, and by the lower ones where several lanes have the same
     const uint32_t upper = (uint32_t)(most >> 32), high = wave_max(upper);
     uint64_t at = __ballot(upper == high);
-    uint32_t owner = (uint32_t)__ffsll((long long)at) - 1, low = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)most, (int)owner);
+    uint32_t owner = (uint32_t)__ffsll((long long)at) - 1;
+    uint32_t low = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)most, (int)owner);
     if (at & (at - 1)) {
       low = wave_max(upper == high ? (uint32_t)most : 0);
       at = __ballot(upper == high && (uint32_t)most == low);
@@ -310,7 +315,9 @@ __device__ __forceinline__ void store_choice(const MoeArgs& m, uint32_t t, const
 
 __global__ __launch_bounds__(64) void moe_route_kernel(MoeArgs m) { store_choice(m, blockIdx.x, choose(m, blockIdx.x)); }
 
-// Pairs whose experts the inner products' workgroups choose for themselves, each all of them.
+// Up to so many, the inner products' workgroups choose the experts for themselves, each all of them: a wavefront two
+// tokens.  (16 experts of 1024x2048, 4 tokens: 22 us, 26 with a launch for the choice; 64 experts, 32 tokens: 49 and 37.)
+constexpr uint32_t kFusedTokens = 8;
 constexpr uint32_t kFusedPairs = 32;
 
 // Rows of one expert's products for its tokens (or, ALL, of the outer products
@@ -331,6 +338,12 @@ constexpr uint32_t kFusedPairs = 32;
 // A step's eight scales of a row lie at any byte, within three words, of which
 // those come that hold one of the row's own; four lanes a row.  kDma: codes lie
 // at multiples of 16 bytes; else they go through registers.
+//
+// Memory's latency bounds it: a workgroup ends after 1 to 56 steps, of which
+// NS - 1 are on their way, and the chip's bytes on their way are what its
+// workgroups have.  8 experts of 4096x14336, 1 token: inner 27 us (125 MB, 4.6
+// TB/s), outer 14.6 us (62 MB, 4.3 TB/s).  Three stages of the inner products,
+// two workgroups a compute unit instead of three, 30.6 us.
 template <bool INNER, bool ALL, int WR, int KG, int XC, int NS, bool kDma>
 __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
   static_assert(WR == 1 || KG == 1, "groups of several wavefronts meet at barriers of the whole workgroup");
@@ -473,7 +486,8 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
 #pragma unroll
       for (int j = 0; j < JS; ++j) {
         const uint64_t from = s_at[j] + e * a.down.scales_expert + u.step * 8;
-        dma4(from / 4 * 4 + min(lane % 4, ((uint32_t)from % 4 + last) / 4) * 4, scales_at + (stage * kScales + j * 64) * 4);
+        dma4(from / 4 * 4 + min(lane % 4, ((uint32_t)from % 4 + last) / 4) * 4,
+             scales_at + (stage * kScales + j * 64) * 4);
       }
 #pragma unroll
       for (int j = 0; j < JX; ++j) {
@@ -582,7 +596,8 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
         f32x4 h;
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) h[j] = activated(g[j] + gb[j], u[j] + ub[j]);
-        const uint64_t to = m.p.h + pair * m.p.h_len * 2 + chunk_at(n / 8) * 16 + n % 8 * 2, apart = pairs * (uint64_t)m.p.h_len * 2;
+        const uint64_t to = m.p.h + pair * m.p.h_len * 2 + chunk_at(n / 8) * 16 + n % 8 * 2;
+        const uint64_t apart = pairs * (uint64_t)m.p.h_len * 2;
         store_h(a.out_type, to, apart, f32x2{h[0], h[1]}), store_h(a.out_type, to + 4, apart, f32x2{h[2], h[3]});
       } else if (n < rows) {
         f32x4 v = sum_of(w, 0, in % 4, t);
@@ -610,6 +625,11 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
 // columns there.  So LDS is for the weights, NS steps of each wavefront on their way, across the ends of tiles and of
 // experts.  A tile's sums are added up over the wavefronts through LDS, while the next tile's products run.  INNER: of
 // whole rows; else of a chunk of them, each chunk a sum of its own, which the combining kernel adds.
+//
+// 8 experts of 4096x14336, 64 tokens: inner 97 us (499 MB, 5.1 TB/s: memory), outer 72 us (250 MB, 3.5 TB/s; 49 without
+// the products and 63 without the loads: a tile's 16 products a wavefront and 16 columns, its two barriers and the sums'
+// way through LDS take as long as its bytes).  With columns through LDS they took 120 and 101.  Weights that stayed in L2
+// as others do (no "once") took 114 and 75: lines of h and y, of which a tile writes 32 or 64 bytes, left L2 in pieces.
 constexpr uint32_t kStreamGroups = kComputeUnits;
 constexpr uint32_t kStreamSlots = 16;    // experts of a workgroup, see below
 
@@ -943,7 +963,8 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
   }
 }
 
-// The weighted sums of each token's experts, the largest weight first.
+// The weighted sums of each token's experts, the largest weight first.  64 tokens of 4096, two experts in seven chunks:
+// 5.7 us for 15 MB that lie in the last-level cache, the launch and one trip to memory.
 __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs m) {
   const MxMoeArgs& a = m.a;
   const uint32_t per = a.cols / 4, at = blockIdx.x * 256 + threadIdx.x, t = at / per, n = (at - t * per) * 4;
@@ -1040,12 +1061,16 @@ hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
     hipError_t e = logits_of(m, stream);
     const uint64_t pairs = tokens * a.top_k;
     const uint32_t xp = parts_of(a.x_type), hp = inner_parts(a.out_type);
+    // Rows that keep most of eight wavefronts busy (2 of 8 experts of 4096x14336, 8 tokens: 79 us, 88 by the other
+    // kernel; 64 tokens 97 and 134; 8192 columns, 64 tokens 78 and 99; 128 experts of 2048x768, 16 tokens 36 and 30).
     const bool stream_inner = tokens > 1 && inner && a.cols > 2048 && near_rows(a.gate) && near_rows(a.up) &&
                               a.gate.codes.stride == a.up.codes.stride && a.gate.scales.stride == a.up.scales.stride &&
                               chunks_of(m.p.x_len, 1, 4, m);
-    if (e == hipSuccess && (pairs > kFusedPairs || stream_inner)) e = launch(moe_route_kernel, tokens, 64, m, stream);
-    m.routed = pairs > kFusedPairs || stream_inner;
+    m.routed = tokens > kFusedTokens || pairs > kFusedPairs || stream_inner;
+    if (e == hipSuccess && m.routed) e = launch(moe_route_kernel, tokens, 64, m, stream);
     if (e != hipSuccess) return e;
+    // 16 rows a workgroup, four wavefronts along them, where 64 would leave compute units idle (8 of 128 experts of
+    // 2048x768, 1 token: 9.2 us and 12.7; 2 of 8 of 4096x14336: 31 and 27)
     const uint64_t groups = (pairs < a.experts ? pairs : a.experts) * ((a.inner + 63) / 64);
     if (tokens * xp <= 4 && groups < kComputeUnits && !stream_inner)
       e = product_of<true, false, 1, 4, 4, 2>(m, inner, stream);
@@ -1056,9 +1081,16 @@ hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
     else
       e = product_of<true, false, 4, 1, 16, 2>(m, inner, stream);
     if (e != hipSuccess) return e;
+    // The weighted sums at once, without a launch of their own of 4 us, unless few workgroups have much to do (2 of 8
+    // experts of 4096x14336, 1 token: 15.0 us, 17.4 before the sums; 6 of 53 of 512x6080: 17.9 and 9.6).
     if (tokens * hp <= 4 && pairs <= 64 && (a.cols >= 2048 || pairs * (m.p.h_len / kStep) <= 64))
       return product_of<false, true, 1, 8, 4, 3>(m, outer, stream);
-    if (outer && a.inner > 1024 && near_rows(a.down) && chunks_of(m.p.h_len, kChunks, 1, m))
+    // As above, and shorter rows too where there are more of them than the other kernel's workgroups do in one round
+    // (8 experts of 4096x14336, 64 tokens: 72 us and 131; 32 of 4096x2048, 16 tokens 27 and 30; 11 of 1120x1504, 7
+    // tokens 8.0 and 6.0).
+    const uint64_t outer_groups = (pairs < a.experts ? pairs : a.experts) * ((a.cols + 63) / 64);
+    if (outer && a.inner > (outer_groups > 2 * kComputeUnits ? 1024 : 2048) && near_rows(a.down) &&
+        chunks_of(m.p.h_len, kChunks, 1, m))
       e = stream_of<false, 1, 4>(m, stream);
     else
       e = product_of<false, false, 4, 1, 16, 3>(m, outer, stream);

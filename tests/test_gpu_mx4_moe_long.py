@@ -17,6 +17,8 @@ SIZES = [  # tokens, experts, top_k, cols, inner: steps of 256 values, whole and
     # rows of blocks that are no multiple of four: scales at any byte, one to seven blocks in the last step
     (7, 3, 2, 2080, 1056), (30, 4, 2, 2112, 1184), (64, 5, 2, 2144, 1248), (21, 6, 3, 4128, 1504), (40, 2, 1, 5056, 2400),
     (12, 4, 2, 8160, 4320), (10, 2, 1, 3360, 14304), (64, 33, 4, 2272, 1312),
+    # many experts
+    (63, 1024, 2, 64, 2176), (20, 600, 4, 2080, 64),
 ]
 
 
