@@ -1062,10 +1062,13 @@ hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
     const uint64_t pairs = tokens * a.top_k;
     const uint32_t xp = parts_of(a.x_type), hp = inner_parts(a.out_type);
     // Rows that keep most of eight wavefronts busy (2 of 8 experts of 4096x14336, 8 tokens: 79 us, 88 by the other
-    // kernel; 64 tokens 97 and 134; 8192 columns, 64 tokens 78 and 99; 128 experts of 2048x768, 16 tokens 36 and 30).
-    const bool stream_inner = tokens > 1 && inner && a.cols > 2048 && near_rows(a.gate) && near_rows(a.up) &&
-                              a.gate.codes.stride == a.up.codes.stride && a.gate.scales.stride == a.up.scales.stride &&
-                              chunks_of(m.p.x_len, 1, 4, m);
+    // kernel; 64 tokens 97 and 134; 8192 columns, 64 tokens 78 and 99; 128 experts of 2048x768, 16 tokens 36 and 30), or
+    // half of them where an expert's tokens would take the other kernel several passes (2 experts of 1024x2048, 64
+    // tokens: 12 and 19; 10 of 640x5984, 17 tokens of f32 each: 62 and 50).
+    const double inner_columns = (double)pairs / a.experts * xp, outer_columns = (double)pairs / a.experts * hp;
+    const bool stream_inner = tokens > 1 && inner && a.cols > (inner_columns > 32 ? 768 : 2048) && near_rows(a.gate) &&
+                              near_rows(a.up) && a.gate.codes.stride == a.up.codes.stride &&
+                              a.gate.scales.stride == a.up.scales.stride && chunks_of(m.p.x_len, 1, 4, m);
     m.routed = tokens > kFusedTokens || pairs > kFusedPairs || stream_inner;
     if (e == hipSuccess && m.routed) e = launch(moe_route_kernel, tokens, 64, m, stream);
     if (e != hipSuccess) return e;
@@ -1089,8 +1092,8 @@ hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
     // (8 experts of 4096x14336, 64 tokens: 72 us and 131; 32 of 4096x2048, 16 tokens 27 and 30; 11 of 1120x1504, 7
     // tokens 8.0 and 6.0).
     const uint64_t outer_groups = (pairs < a.experts ? pairs : a.experts) * ((a.cols + 63) / 64);
-    if (outer && a.inner > (outer_groups > 2 * kComputeUnits ? 1024 : 2048) && near_rows(a.down) &&
-        chunks_of(m.p.h_len, kChunks, 1, m))
+    const uint32_t least = outer_columns > 32 ? 768 : outer_groups > 2 * kComputeUnits ? 1024 : 2048;
+    if (outer && a.inner > least && near_rows(a.down) && chunks_of(m.p.h_len, kChunks, 1, m))
       e = stream_of<false, 1, 4>(m, stream);
     else
       e = product_of<false, false, 4, 1, 16, 3>(m, outer, stream);
