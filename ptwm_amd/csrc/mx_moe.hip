@@ -663,10 +663,18 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
     static_assert(sizeof(sums) >= kMoeMaxExperts * 4);
     for (uint32_t e = threadIdx.x; e < a.experts; e += 512) counts[e] = 0;
     __syncthreads();
-    for (uint32_t p = threadIdx.x; p < pairs; p += 512) {
-      const int32_t e = g_ld<int32_t>(m.p.chosen + p * 4);
+    const auto count = [&](uint32_t p, int32_t e) {
       chosen[p] = (int16_t)e;
       if (e >= 0) atomicAdd(&counts[e], 1u);
+    };
+    if (!INNER || m.routed) {
+      for (uint32_t p = threadIdx.x; p < pairs; p += 512) count(p, g_ld<int32_t>(m.p.chosen + p * 4));
+    } else {
+      for (uint32_t t = wave; t < a.tokens; t += 8) {
+        const Chosen c = choose(m, t);
+        if (lane < a.top_k) count(t * a.top_k + lane, c.expert);
+        if (blockIdx.x == 0) store_choice(m, t, c);
+      }
     }
     __syncthreads();
     if (wave == 0) {
@@ -1069,7 +1077,7 @@ hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
     const bool stream_inner = tokens > 1 && inner && a.cols > (inner_columns > 32 ? 768 : 2048) && near_rows(a.gate) &&
                               near_rows(a.up) && a.gate.codes.stride == a.up.codes.stride &&
                               a.gate.scales.stride == a.up.scales.stride && chunks_of(m.p.x_len, 1, 4, m);
-    m.routed = tokens > kFusedTokens || pairs > kFusedPairs || stream_inner;
+    m.routed = tokens > kFusedTokens || pairs > kFusedPairs;
     if (e == hipSuccess && m.routed) e = launch(moe_route_kernel, tokens, 64, m, stream);
     if (e != hipSuccess) return e;
     // 16 rows a workgroup, four wavefronts along them, where 64 would leave compute units idle (8 of 128 experts of
