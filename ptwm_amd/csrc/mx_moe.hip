@@ -238,6 +238,16 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
+// The sum of a lane's and the lower lanes' values.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t plus_by(uint32_t v) {
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ uint32_t wave_up_to(uint32_t v) {
+  v = plus_by<0x111, 0xF>(v), v = plus_by<0x112, 0xF>(v), v = plus_by<0x114, 0xF>(v), v = plus_by<0x118, 0xF>(v);
+  return plus_by<0x143, 0xC>(plus_by<0x142, 0xA>(v));
+}
+
 // Chooses a token's experts: the largest that is left, the lowest expert of equal ones.  One wavefront, N logits a
 // lane; lane k returns the k-th, with its weight.  An expert at minus infinity has none, not even among its like.
 struct Chosen {
@@ -626,12 +636,15 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
 // experts.  A tile's sums are added up over the wavefronts through LDS, while the next tile's products run.  INNER: of
 // whole rows; else of a chunk of them, each chunk a sum of its own, which the combining kernel adds.
 //
-// 8 experts of 4096x14336, 64 tokens: inner 97 us (499 MB, 5.1 TB/s: memory), outer 72 us (250 MB, 3.5 TB/s; 49 without
-// the products and 63 without the loads: a tile's 16 products a wavefront and 16 columns, its two barriers and the sums'
-// way through LDS take as long as its bytes).  With columns through LDS they took 120 and 101.  Weights that stayed in L2
+// 8 experts of 4096x14336, 64 tokens: inner 97 us (499 MB, 5.1 TB/s: memory), outer 69 us (250 MB, 3.6 TB/s; 44 without
+// products and sums: a tile's 16 products a wavefront and 16 columns, its two barriers and the sums' way through LDS
+// take longer than its bytes).  With columns through LDS they took 120 and 101.  Weights that stayed in L2
 // as others do (no "once") took 114 and 75: lines of h and y, of which a tile writes 32 or 64 bytes, left L2 in pieces.
 constexpr uint32_t kStreamGroups = kComputeUnits;
 constexpr uint32_t kStreamSlots = 16;    // experts of a workgroup, see below
+// What a tile costs beside its groups of columns, in the like of one: 64 tokens' outer products take 74 us by equal tiles
+// and 70, 69, 68.7 with 8, 6, 2.
+constexpr uint32_t kInnerWeight = 8, kOuterWeight = 2;
 
 template <bool INNER, int S, int NC>
 __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
@@ -643,7 +656,7 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
   __shared__ f32x2 sums[8 * M * NC * 128];
   __shared__ int16_t chosen[kTokens * kMoeMaxTopK];
   __shared__ u32x4 none[8];
-  __shared__ uint32_t slots[kStreamSlots], share[2];
+  __shared__ uint32_t slots[kStreamSlots], share[4];
   __shared__ int32_t list[kTokens];
   __shared__ float biases[M][INNER ? kBiasTiles * 16 : 1];
   const MxMoeArgs& a = m.a;
@@ -654,10 +667,10 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
   const uint32_t span = m.span, chunks = m.chunks;
   const uint32_t parts = INNER ? parts_of(a.x_type) : inner_parts(a.out_type), each = 16 / parts, most = each * NC;
   const uint32_t pairs = (uint32_t)a.tokens * a.top_k;
-  auto scalar = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
-
-  // A slot is an expert's up to `most` tokens.  There are at most 2048 / 5 + 1024 (three parts, one group of columns),
-  // so of the 256 workgroups' equal shares none meets more than eight.
+  // A slot is an expert's up to `most` tokens; a tile of it weighs kTileWeight + its groups of columns, and every
+  // workgroup has an equal share of that.  There are at most 2048 / 5 + 1024 slots (three parts, one group of columns),
+  // and one weighs twice another at most, so no share meets more than thirteen.
+  constexpr uint32_t kTileWeight = INNER ? kInnerWeight : kOuterWeight;
   {
     uint32_t* const counts = reinterpret_cast<uint32_t*>(sums);
     static_assert(sizeof(sums) >= kMoeMaxExperts * 4);
@@ -678,35 +691,43 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
     }
     __syncthreads();
     if (wave == 0) {
-      const uint64_t of_slot = (uint64_t)chunks * tiles;
-      auto slots_of = [&](uint32_t e) { return e < a.experts ? (counts[e] + most - 1) / most : 0; };
-      auto up_to = [&](uint32_t v) {  // the lane's and lower lanes' together
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-          const uint32_t other = __shfl_up(v, d, 64);
-          if (lane >= d) v += other;
+      const uint32_t of_slot = chunks * tiles;
+      // for 64 experts at a time, one a lane: its slots, their weight (of a tile each), and both with the ones before
+      uint32_t all = 0, weight = 0, n = 0, own = 0, n_to = 0, to = 0;
+      const auto each_slot = [&](auto f) {
+        all = weight = 0;
+        for (uint32_t e = lane; e - lane < a.experts; e += 64) {
+          const uint32_t count = e < a.experts ? counts[e] : 0;
+          n = (count + most - 1) / most;
+          own = n ? n * (kTileWeight + NC) - (n * most - count) / each : 0;
+          n_to = wave_up_to(n), to = wave_up_to(own);
+          for (uint32_t j = 0; j < n; ++j)
+            f(e, j, all + n_to - n + j, weight + to - own + j * (kTileWeight + NC),
+              j + 1 < n ? kTileWeight + NC : own - j * (kTileWeight + NC));
+          all += (uint32_t)__builtin_amdgcn_readlane((int)n_to, 63);
+          weight += (uint32_t)__builtin_amdgcn_readlane((int)to, 63);
         }
-        return v;
       };
-      uint32_t all = 0;
-      for (uint32_t e = 0; e < a.experts; e += 64) all += __shfl(up_to(slots_of(e + lane)), 63, 64);
-      const uint64_t first = all * of_slot * blockIdx.x / kStreamGroups;
-      const uint64_t end = all * of_slot * (blockIdx.x + 1) / kStreamGroups;
-      const uint32_t slot0 = (uint32_t)(first / of_slot);
-      uint32_t at = 0;
-      for (uint32_t e = 0; e < a.experts; e += 64) {
-        const uint32_t n = slots_of(e + lane), to = up_to(n);
-        for (uint32_t j = 0; j < n; ++j) {
-          const uint32_t slot = at + to - n + j - slot0;
-          if (slot < kStreamSlots) slots[slot] = (e + lane) | j << 16;
-        }
-        at += __shfl(to, 63, 64);
-      }
-      if (lane == 0) share[0] = (uint32_t)(end - first), share[1] = (uint32_t)(first - slot0 * of_slot);
+      each_slot([](uint32_t, uint32_t, uint32_t, uint32_t, uint32_t) {});
+      const uint64_t total = (uint64_t)weight * of_slot;
+      const uint64_t first = total * blockIdx.x / kStreamGroups, end = total * (blockIdx.x + 1) / kStreamGroups;
+      if (lane < 4) share[lane] = lane % 2 ? 0 : all;
+      each_slot([&](uint32_t, uint32_t, uint32_t slot, uint32_t before, uint32_t w) {
+        const uint64_t from = (uint64_t)before * of_slot, past = from + (uint64_t)w * of_slot;
+        if (first >= from && first < past) share[0] = slot, share[1] = (uint32_t)(first - from) / w;
+        if (end >= from && end < past) share[2] = slot, share[3] = (uint32_t)(end - from) / w;
+      });
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      const uint32_t slot0 = share[0];
+      each_slot([&](uint32_t e, uint32_t j, uint32_t slot, uint32_t, uint32_t) {
+        if (slot - slot0 < kStreamSlots) slots[slot - slot0] = e | j << 16;
+      });
     }
     __syncthreads();
   }
-  uint32_t left = scalar(share[0]), slot = 0, chunk = scalar(share[1]) / tiles, tile = scalar(share[1]) % tiles;
+  auto scalar = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
+  uint32_t left = scalar((share[2] - share[0]) * (chunks * tiles) + share[3] - share[1]), slot = 0;
+  uint32_t chunk = scalar(share[1]) / tiles, tile = scalar(share[1]) % tiles;
   if (left == 0) return;
   auto steps_of = [&](uint32_t chunk) {  // of this wavefront
     const uint32_t have = min(span, steps - chunk * span);
@@ -1097,7 +1118,7 @@ hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
     if (tokens * hp <= 4 && pairs <= 64 && (a.cols >= 2048 || pairs * (m.p.h_len / kStep) <= 64))
       return product_of<false, true, 1, 8, 4, 3>(m, outer, stream);
     // As above, and shorter rows too where there are more of them than the other kernel's workgroups do in one round
-    // (8 experts of 4096x14336, 64 tokens: 72 us and 131; 32 of 4096x2048, 16 tokens 27 and 30; 11 of 1120x1504, 7
+    // (8 experts of 4096x14336, 64 tokens: 69 us and 131; 32 of 4096x2048, 16 tokens 27 and 30; 11 of 1120x1504, 7
     // tokens 8.0 and 6.0).
     const uint64_t outer_groups = (pairs < a.experts ? pairs : a.experts) * ((a.cols + 63) / 64);
     const uint32_t least = outer_columns > 32 ? 768 : outer_groups > 2 * kComputeUnits ? 1024 : 2048;
