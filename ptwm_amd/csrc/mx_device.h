@@ -105,21 +105,18 @@ __device__ __forceinline__ void dma16_once(uint64_t from, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(to), "v"(from) : "memory", "m0");
 }
 
+// DMA of 4 bytes a lane, from multiples of 4.
 __device__ __forceinline__ void dma4(GlobalBytes from, uint32_t offset, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(from)
                : "memory", "m0");
 }
-__device__ __forceinline__ void dma4(uint64_t from, uint32_t to) {  // 4 bytes a lane, from multiples of 4
+__device__ __forceinline__ void dma4(uint64_t from, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "memory", "m0");
-}
-__device__ __forceinline__ void dma1(uint64_t from, uint32_t to) {  // a byte a lane, to words
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off" ::"s"(to), "v"(from) : "memory", "m0");
 }
 
 // LDS by its byte address, which takes a known offset along in the instruction.
 typedef __attribute__((address_space(3))) u32x4* LdsChunks;
 typedef __attribute__((address_space(3))) u32x2* LdsPairs;
-typedef __attribute__((address_space(3))) uint32_t* LdsWord;
 template <typename T>
 __device__ __forceinline__ uint32_t lds_address(T* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) T*)p;
