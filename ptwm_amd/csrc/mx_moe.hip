@@ -643,17 +643,17 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
   }
 }
 
-// The same products where an expert has several tokens and its codes lie at multiples of 16 bytes: the columns stay
-// in registers.  A workgroup walks along consecutive tiles of 16 rows, of one expert after the other; of a tile's rows
-// wavefront w of eight has steps w, w + 8, ... of a chunk of the rows, S at most, and keeps the values of 16 * NC
-// columns there.  So LDS is for the weights, NS steps of each wavefront on their way, across the ends of tiles and of
-// experts.  A tile's sums are added up over the wavefronts through LDS, while the next tile's products run.  INNER: of
-// whole rows; else of a chunk of them, each chunk a sum of its own, which the combining kernel adds.
+// The same products where an expert has several tokens and its codes lie at multiples of 16 bytes: the columns stay in
+// registers.  A workgroup walks along consecutive tiles (16 rows of gate and of up, or 32 of down), of one expert after
+// the other; of a tile's rows wavefront w of eight has steps w, w + 8, ... of a chunk of the rows, S at most, and keeps
+// the values of 16 * NC columns there.  So LDS is for the weights, NS steps of each wavefront on their way, across the
+// ends of tiles and of experts.  A tile's sums are added up over the wavefronts through LDS, read before the next tile's
+// products and stored after them.  INNER: sums of whole rows; else of a chunk of them, which the combining kernel adds.
 //
 // 8 experts of 4096x14336, 64 tokens: inner 97 us (499 MB, 5.1 TB/s: memory), outer 69 us (250 MB, 3.6 TB/s; 44 without
 // products and sums: a tile's 16 products a wavefront and 16 columns, its two barriers and the sums' way through LDS
-// take longer than its bytes).  With columns through LDS they took 120 and 101.  Weights that stayed in L2
-// as others do (no "once") took 114 and 75: lines of h and y, of which a tile writes 32 or 64 bytes, left L2 in pieces.
+// take longer than its bytes).  With columns through LDS they took 120 and 101.  Weights that stayed in L2 as others do
+// (no "once") took 114 and 75: lines of h and y, of which a tile writes 32 or 64 bytes, left L2 in pieces.
 constexpr uint32_t kStreamGroups = kComputeUnits;
 constexpr uint32_t kStreamSlots = 16;    // experts of a workgroup, see below
 // What a tile costs beside its groups of columns, in the like of one: 64 tokens' outer products take 74 us by equal tiles
@@ -748,11 +748,11 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
     return wave < have ? (have - wave + 7) / 8 : 0;
   };
 
-  // The tile to be requested next, T ahead: of it `n` steps, `run` tiles to the end of the expert's or the chunk's,
-  // `left` to the end of all.  Rows come by 32, so all of a tile's are there.
   auto part_of = [&](uint32_t chunk, uint32_t n) {  // which of n steps is only part of one
     return length % kStep && chunk * span + wave + (n - 1) * 8 == steps - 1 ? n - 1 : ~0u;
   };
+  // The tile to be requested next: of it `n` steps, `run` tiles to the end of the expert's or the chunk's, `left` to the
+  // end of all.  Rows come by 32, so all of a tile's are there.
   struct {
     uint32_t left, run, slot, chunk, tile, n, part;
     uint64_t codes[M], scales[M];  // the first row, at the wavefront's first step; scales at words
@@ -1004,6 +1004,7 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
     left -= run, tile = 0;
     if (++chunk == chunks) chunk = 0, ++slot;
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // for requests to nowhere, while the workgroup's LDS is its own
 }
 
 // The weighted sums of each token's experts, the largest weight first.  64 tokens of 4096, two experts in seven chunks:
