@@ -487,7 +487,9 @@ typedef struct ptwm_mi355x_experts {
  * workspace: device memory of at least workspace_bytes >=
  * ptwm_mi355x_mxfp4_moe_workspace() bytes at a multiple of 256, which the call
  * overwrites and which nothing else may use until it is done: calls that may
- * run at the same time (on two streams, from two graphs) take one each. */
+ * run at the same time (on two streams, from two graphs) take one each.
+ * Scales are read by words of 4 bytes, those that hold a byte of the row: up
+ * to three bytes beside it are read too, and not used. */
 typedef struct ptwm_mi355x_mxfp4_moe {
   uint64_t x, x_stride, router, router_stride, router_bias, out, out_stride;
   ptwm_mi355x_experts gate, up, down;
