@@ -18,7 +18,7 @@
 // launch, whose columns stay in registers.
 //
 // The products are of bf16 on the matrix unit.  Weights are widened to bf16,
-// which is exact; x, and h, are the sum of one to three bf16 values (parts),
+// which is exact; x is the sum of one to three bf16 values (parts), h of three,
 // each of which is a column of the product of its own, summed with its like at
 // the end.  So an instruction's 16 columns are one to three columns a token,
 // whatever the types, and few tokens in two parts cost no more than in one.
@@ -37,8 +37,8 @@ constexpr uint32_t kComputeUnits = 256;
 constexpr uint32_t kTokens = 64;  // of a launch; longer calls run in several
 constexpr uint32_t kStep = 256;   // values of a row that go through LDS together: a cache line of codes
 
-// h's parts: 24 significant bits where the outputs have 24, else 16, whose rounding is 2^-8 or 2^-5 of the output's own.
-constexpr uint32_t inner_parts(uint32_t out_type) { return out_type == kTypeF32 ? 3 : 2; }
+// h's parts: all 24 bits of a sum in 32, whatever the outputs' type.
+constexpr uint32_t kInnerParts = 3;
 
 // Where a launch's intermediate results lie in the workspace.  A pair is a token's k-th expert, token * top_k + k.
 struct MoePlaces {
@@ -64,7 +64,7 @@ MoePlaces places_of(const MxMoeArgs& a) {
   p.x_len = (a.cols + kStep - 1) / kStep * kStep, p.h_len = (a.inner + kStep - 1) / kStep * kStep;
   p.logits = take(t * a.experts * 8);
   p.x = take(parts_of(a.x_type) * t * p.x_len * 2);
-  p.h = take(inner_parts(a.out_type) * pairs * p.h_len * 2);
+  p.h = take(kInnerParts * pairs * p.h_len * 2);
   const uint64_t chunks = (p.h_len / kStep + 7) / 8;
   p.y = take((chunks <= kChunks ? chunks : 1) * pairs * a.cols * 4);
   p.chosen = take(pairs * 4), p.weights = take(pairs * 4);
@@ -139,12 +139,12 @@ __device__ __forceinline__ void store_out(const MxMoeArgs& a, uint64_t t, uint32
 
 __device__ __forceinline__ float activated(float g, float u) { return g / (1.0f + expf(-g)) * u; }
 
-// Two neighbours of a pair's h, the parts `apart` bytes apart: as x's, but for the last, which is rounded.
-__device__ __forceinline__ void store_h(uint32_t out_type, uint64_t to, uint64_t apart, f32x2 h) {
-  const uint32_t hp = inner_parts(out_type);
-  for (uint32_t p = 0; p < hp; ++p, to += apart) {
+// Two neighbours of a pair's h, the parts `apart` bytes apart: as x.s; the last is exact too, down to 2^-133.
+__device__ __forceinline__ void store_h(uint64_t to, uint64_t apart, f32x2 h) {
+#pragma unroll
+  for (uint32_t p = 0; p < kInnerParts; ++p, to += apart) {
     uint32_t b;
-    if (p + 1 < hp) {
+    if (p + 1 < kInnerParts) {
       const uint32_t low = f32_bits(__builtin_amdgcn_fmed3f(h[0], -kBf16Max, kBf16Max)) & 0xFFFF0000u;
       const uint32_t high = f32_bits(__builtin_amdgcn_fmed3f(h[1], -kBf16Max, kBf16Max)) & 0xFFFF0000u;
       h -= f32x2{bits_f32(low), bits_f32(high)};
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(kLogitThreads) void moe_logits_kernel(MoeArgs m) {
 #pragma unroll
       for (int j = 0; j < parts_of(T); ++j) st16(m.p.x + (j * a.tokens + t) * m.p.x_len * 2 + chunk_at(k / 8) * 16, p[j]);
     }
-    const uint32_t none = (m.p.h_len - a.inner) / 8, rows = a.top_k * inner_parts(a.out_type);  // chunks of a row
+    const uint32_t none = (m.p.h_len - a.inner) / 8, rows = a.top_k * kInnerParts;  // chunks of a row
     for (uint32_t j = threadIdx.x; j < none * rows; j += kLogitThreads) {
       const uint32_t row = j / none, part = row / a.top_k, pair = t * a.top_k + row % a.top_k;
       st16(m.p.h + (part * a.tokens * a.top_k + pair) * m.p.h_len * 2 + chunk_at(a.inner / 8 + j % none) * 16, u32x4{});
@@ -392,7 +392,7 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
   const uint32_t x_len = INNER ? m.p.x_len : m.p.h_len, steps = x_len / kStep;
   const uint32_t tiles = (rows + kRows - 1) / kRows;
   const uint32_t slot = blockIdx.x / tiles, n0 = blockIdx.x % tiles * kRows;
-  const uint32_t parts = INNER ? parts_of(a.x_type) : inner_parts(a.out_type), each = XC / parts;  // tokens of XC columns
+  const uint32_t parts = INNER ? parts_of(a.x_type) : kInnerParts, each = XC / parts;  // tokens of XC columns
   const uint32_t pairs = (uint32_t)a.tokens * a.top_k;
 
   // The expert and the pairs that chose it (every wavefront writes the same to LDS); ALL: the experts that any pair
@@ -622,7 +622,7 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
         for (uint32_t j = 0; j < 4; ++j) h[j] = activated(g[j] + gb[j], u[j] + ub[j]);
         const uint64_t to = m.p.h + pair * m.p.h_len * 2 + chunk_at(n / 8) * 16 + n % 8 * 2;
         const uint64_t apart = pairs * (uint64_t)m.p.h_len * 2;
-        store_h(a.out_type, to, apart, f32x2{h[0], h[1]}), store_h(a.out_type, to + 4, apart, f32x2{h[2], h[3]});
+        store_h(to, apart, f32x2{h[0], h[1]}), store_h(to + 4, apart, f32x2{h[2], h[3]});
       } else if (n < rows) {
         f32x4 v = sum_of(w, 0, in % 4, t);
         if constexpr (ALL) {
@@ -679,7 +679,7 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
   const uint32_t rows = INNER ? a.inner : a.cols, length = INNER ? a.cols : a.inner, tiles = rows / (INNER ? 16 : 32);
   const uint32_t x_len = INNER ? m.p.x_len : m.p.h_len, steps = x_len / kStep;
   const uint32_t span = m.span, chunks = m.chunks;
-  const uint32_t parts = INNER ? parts_of(a.x_type) : inner_parts(a.out_type), each = 16 / parts, most = each * NC;
+  const uint32_t parts = INNER ? parts_of(a.x_type) : kInnerParts, each = 16 / parts, most = each * NC;
   const uint32_t pairs = (uint32_t)a.tokens * a.top_k;
   // A slot is an expert's up to `most` tokens; a tile of it weighs kTileWeight + its groups of columns, and every
   // workgroup has an equal share of that.  There are at most 2048 / 5 + 1024 slots (three parts, one group of columns),
@@ -912,7 +912,7 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
           const uint32_t at = (tile - bias0) * 16 + n_in;
           v[0] += f32x2{biases[0][at], biases[0][at + 1]}, v[1] += f32x2{biases[1][at], biases[1][at + 1]};
         }
-        store_h(m.a.out_type, out + chunk_at(tile * 2) * 16, (uint64_t)pairs * m.p.h_len * 2,
+        store_h(out + chunk_at(tile * 2) * 16, (uint64_t)pairs * m.p.h_len * 2,
                 f32x2{activated(v[0][0], v[1][0]), activated(v[0][1], v[1][1])});
       } else {
 #pragma unroll
@@ -1104,12 +1104,12 @@ hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
     if (a.weights_out) m.a.weights_out += first * a.top_k * 4;
     hipError_t e = logits_of(m, stream);
     const uint64_t pairs = tokens * a.top_k;
-    const uint32_t xp = parts_of(a.x_type), hp = inner_parts(a.out_type);
+    const uint32_t xp = parts_of(a.x_type);
     // Rows that keep most of eight wavefronts busy (2 of 8 experts of 4096x14336, 8 tokens: 79 us, 88 by the other
     // kernel; 64 tokens 97 and 134; 8192 columns, 64 tokens 78 and 99; 128 experts of 2048x768, 16 tokens 36 and 30), or
     // half of them where an expert's tokens would take the other kernel several passes (2 experts of 1024x2048, 64
     // tokens: 12 and 19; 10 of 640x5984, 17 tokens of f32 each: 62 and 50).
-    const double inner_columns = (double)pairs / a.experts * xp, outer_columns = (double)pairs / a.experts * hp;
+    const double inner_columns = (double)pairs / a.experts * xp, outer_columns = (double)pairs / a.experts * kInnerParts;
     const bool stream_inner = tokens > 1 && inner && a.cols > (inner_columns > 32 ? 768 : 2048) && near_rows(a.gate) &&
                               near_rows(a.up) && a.gate.codes.stride == a.up.codes.stride &&
                               a.gate.scales.stride == a.up.scales.stride && chunks_of(m.p.x_len, 1, 4, m);
@@ -1130,8 +1130,9 @@ hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
     if (e != hipSuccess) return e;
     // The weighted sums at once, without a launch of their own of 4 us, unless few workgroups have much to do (2 of 8
     // experts of 4096x14336, 1 token: 15.0 us, 17.4 before the sums; 6 of 53 of 512x6080: 17.9 and 9.6).
-    if (tokens * hp <= 4 && pairs <= 64 && (a.cols >= 2048 || pairs * (m.p.h_len / kStep) <= 64))
-      return product_of<false, true, 1, 8, 4, 3>(m, outer, stream);
+    if (tokens <= 2 && pairs <= 64 && (a.cols >= 2048 || pairs * (m.p.h_len / kStep) <= 64))
+      return tokens == 1 ? product_of<false, true, 1, 8, 4, 3>(m, outer, stream)
+                         : product_of<false, true, 1, 8, 6, 3>(m, outer, stream);
     // As above, and shorter rows too where there are more of them than the other kernel's workgroups do in one round
     // (8 experts of 4096x14336, 64 tokens: 69 us and 131; 32 of 4096x2048, 16 tokens 27 and 30; 11 of 1120x1504, 7
     // tokens 8.0 and 6.0).
