@@ -390,7 +390,10 @@ int64_t ptwm_mi355x_last_kernel_ms(uint32_t device_ordinal, float *out3);
  *
  * These calls differ from the codec's in one way: they queue their work on
  * `stream` (a hipStream_t of the device, 0 = the null stream) and return
-X strides are between rows, in elements
+ * without waiting for it.  They hold no state, lock or workspace of their
+ * own, allocate nothing, and may be captured into a graph; the experts' layer
+ * works in memory that the caller gives it.  Addresses need the alignment of
+ * their elements only (that memory: 256); strides are between rows, in elements
  * (weights and scales: bytes).  dtypes are public dtype codes (dtype.rs:79-103):
  * 1 float32, 4 float16, 6 bfloat16, 29 float8_e4m3fn.  cols is a multiple of
  * 32.  Returns 0; -1 for arguments that do not fit together (nothing is
