@@ -137,7 +137,13 @@ __device__ __forceinline__ void store_out(const MxMoeArgs& a, uint64_t t, uint32
     st16(a.out.ptr + to * 4, __builtin_bit_cast(u32x4, v));
 }
 
-__device__ __forceinline__ float activated(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+// silu(g) * u.  Below g = -64 the 1 is nothing beside exp(-g), which 32 bits do not hold from -88.8 on though its quotient
+// with a large u may be a value: there four times exp(g / 4), the first one with g and u, each a number down to g = -349.
+__device__ __forceinline__ float activated(float g, float u) {
+  const bool deep = g < -64.0f;
+  const float e = expf(deep ? 0.25f * g : -g);
+  return deep ? g * e * u * e * e * e : g / (1.0f + e) * u;
+}
 
 // Two neighbours of a pair's h, the parts `apart` bytes apart: as x.s; the last is exact too, down to 2^-133.
 __device__ __forceinline__ void store_h(uint64_t to, uint64_t apart, f32x2 h) {
