@@ -1139,11 +1139,12 @@ hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
     if (tokens <= 2 && pairs <= 64 && (a.cols >= 2048 || pairs * (m.p.h_len / kStep) <= 64))
       return tokens == 1 ? product_of<false, true, 1, 8, 4, 3>(m, outer, stream)
                          : product_of<false, true, 1, 8, 6, 3>(m, outer, stream);
-    // As above, and shorter rows too where there are more of them than the other kernel's workgroups do in one round
-    // (8 experts of 4096x14336, 64 tokens: 69 us and 131; 32 of 4096x2048, 16 tokens 27 and 30; 11 of 1120x1504, 7
-    // tokens 8.0 and 6.0).
+    // As above, and shorter rows too where there are more of them than the other kernel's workgroups do in one round, or
+    // where an expert's tokens would take the other kernel four passes (8 experts of 4096x14336, 64 tokens: 105 us and 222;
+    // 2 of 8, 8 tokens 47 and 51; 34 of 256x12096, 9 tokens 17 and 26; 32 of 2048x1536, 64 tokens with eight each 35 and
+    // 55; 8 of 2048x1536, 64 tokens 19 and 17; 11 of 1120x1504, 7 tokens 9.3 and 6.0; 4 of 2048x800, 64 tokens 15 and 22).
     const uint64_t outer_groups = (pairs < a.experts ? pairs : a.experts) * ((a.cols + 63) / 64);
-    const uint32_t least = outer_columns > 32 ? 768 : outer_groups > 2 * kComputeUnits ? 1024 : 2048;
+    const uint32_t least = outer_columns > 48 ? 768 : outer_groups > 2 * kComputeUnits ? 1024 : 2048;
     if (outer && a.inner > least && near_rows(a.down) && chunks_of(m.p.h_len, kChunks, 1, m))
       e = stream_of<false, 1, 4>(m, stream);
     else
