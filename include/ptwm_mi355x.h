@@ -479,7 +479,10 @@ typedef struct ptwm_mi355x_experts {
  * `inner` values.  An expert whose logit is minus infinity takes no part and
  * has the weight 0 (a token with no other expert: zeros).  Logits are summed
  * in 64 bits, so that the choice does not depend on an order of additions;
- * other sums are in 32 bits, and all of h's go into the last product.  x, router and out are float32, float16 or bfloat16 each;
+ * other sums are in 32 bits, and all of h's go into the last product.  The
+ * order of their additions depends on the sizes, the codes' alignment and the
+ * strides, and, of two tokens, on the experts that both chose.
+ * x, router and out are float32, float16 or bfloat16 each;
  * router_bias has router_dtype.  out may be x itself.
  * experts_out (int32) and weights_out (float32), tokens x top_k each and 0
  * where not wanted, receive the choice, largest logits first, and p.

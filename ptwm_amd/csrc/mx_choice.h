@@ -1,6 +1,7 @@
-// mx_choice.h -- which kernel takes a product with MXFP4 weights, and of two
-// MXFP4 matrices: rules on sizes, types and alignment, on the host.  The times beside them are
-// microseconds on an MI355X.
+// mx_choice.h -- which kernel takes a product with MXFP4 weights, of two MXFP4
+// matrices, and the products of a mixture-of-experts layer: rules on sizes,
+// types and alignment, on the host.  The times beside them are microseconds on
+// an MI355X.
 #pragma once
 
 #include "mx_ops.h"
@@ -142,6 +143,77 @@ inline MxMatmulChoice choose_mxfp4_matmul(const MxLinearArgs& a) {
   // 64x14336x4096 (224 tiles of 64x64, 112 of 128x64) 8.7 and 10.0, 128x14336x4096 (448, 224) 11.6 and 10.7.
   if (count(64, 64) <= 256) return tile(MxMatmulChoice::k64x64, 64, 64);
   return tile(MxMatmulChoice::k128x64, 128, 64);
+}
+
+constexpr uint32_t kMoeUnits = 256;   // compute units
+constexpr uint32_t kMoeChunks = 16;   // that the outer products' rows are cut into at most
+constexpr uint32_t kMoeFusedPairs = 32;
+
+// How the products of a mixture-of-experts layer are made, for up to kMoeTokens tokens.
+struct MxMoeChoice {
+  // gate and up: 16 rows a workgroup, four wavefronts along them; 64 rows; columns in registers, two or four steps of a
+  // row a wavefront
+  enum Inner : uint32_t { kRows16, kRows64, kStream2, kStream4 } inner;
+  // down: 16 rows a workgroup and the weighted sums of one or two tokens at once; 64 rows; columns in registers, by chunks
+  enum Outer : uint32_t { kSums1, kSums2, kRows, kChunks } outer;
+  bool inner_dma, outer_dma;  // codes lie at multiples of 16 bytes; else they go through registers
+  bool routed;                // the choice of experts is a launch of its own, not the inner products' workgroups'
+  uint32_t span, chunks;      // kChunks: steps of a chunk, chunks of a row; else one
+};
+
+inline MxMoeChoice choose_mxfp4_moe(const MxMoeArgs& a) {
+  const auto whole = [&](const MxExperts& w) {
+    return w.codes.ptr % 16 == 0 && w.codes.stride % 16 == 0 && (a.experts == 1 || w.codes_expert % 16 == 0);
+  };
+  // 16 rows as 32-bit offsets
+  const auto near = [](const MxExperts& w) { return w.codes.stride < 1ull << 27 && w.scales.stride < 1ull << 27; };
+  const auto steps_of = [](uint32_t length) { return (length + kMoeStep - 1) / kMoeStep; };
+  const uint64_t tokens = a.tokens, pairs = tokens * a.top_k, served = pairs < a.experts ? pairs : a.experts;
+  const uint32_t x_steps = steps_of(a.cols), h_steps = steps_of(a.inner), parts = parts_of(a.x_type);
+  // columns of the matrix instruction that an expert's tokens take, on average
+  const double inner_columns = (double)pairs / a.experts * parts, outer_columns = (double)pairs / a.experts * kMoeInnerParts;
+  MxMoeChoice k{};
+  k.inner_dma = whole(a.gate) && whole(a.up), k.outer_dma = whole(a.down);
+  k.span = k.chunks = 1;
+  // Few tokens are chosen for by the inner products' workgroups themselves, each for all of them, a wavefront two tokens:
+  // 16 experts of 1024x2048, 4 tokens 22 and 26 with a launch for the choice; 64 experts, 32 tokens 49 and 37.
+  k.routed = tokens > 8 || pairs > kMoeFusedPairs;
+  // Columns in registers where rows keep most of eight wavefronts busy: measured (so, and by 64 rows) 8 experts of
+  // 4096x14336, 64 tokens 97 and 134, 8 tokens 86 and 95; 32 of 4096x2048, 16 tokens 51 and 59; 8192 columns, 64 tokens
+  // 78 and 99; 128 of 2048x768, 16 tokens 36 and 30.  Or half of them where an expert's tokens would take the other
+  // kernel several passes: 2 experts of 1024x2048, 64 tokens 12 and 19; 10 of 640x5984, 17 tokens of f32 each 62 and 50.
+  if (tokens > 1 && k.inner_dma && a.cols > (inner_columns > 32 ? 768 : 2048) && x_steps <= 32 && near(a.gate) &&
+      near(a.up) && a.gate.codes.stride == a.up.codes.stride && a.gate.scales.stride == a.up.scales.stride)
+    k.inner = x_steps <= 16 ? MxMoeChoice::kStream2 : MxMoeChoice::kStream4;
+  // 16 rows where 64 would leave compute units idle, for the four columns that they hold: measured (16 rows, 64)
+  // 128 experts of 2048x768, one token 10.2 and 14.3, two 12.6 and 14.5, two of f16 13.1 and 14.9, one of f32 11.6 and
+  // 14.5; 16 of 1024x2048, three tokens 9.0 and 10.2; 8 of 1024x512, four 6.7 and 10.0; 8 of 4096x14336, one (448 of 64)
+  // 31 and 27.
+  else if (tokens * parts <= 4 && served * ((a.inner + 63) / 64) < kMoeUnits)
+    k.inner = MxMoeChoice::kRows16;
+  else
+    k.inner = MxMoeChoice::kRows64;
+  // The weighted sums at once, without a launch of their own of 3 to 4, unless few workgroups have much to do: measured
+  // (at once, before the sums) 8 experts of 4096x14336, one token 15.0 and 17.4, two 23.9 and 22.6; 16 of 1024x2048, one
+  // 5.4 and 6.8, two 7.2 and 6.8; 128 of 2048x768, two 9.3 and 5.4; 6 of 53 of 512x6080, one 17.9 and 9.6.
+  if (tokens <= 2 && pairs <= 64 && (a.cols >= 2048 || pairs * h_steps <= 64)) {
+    k.outer = tokens == 1 ? MxMoeChoice::kSums1 : MxMoeChoice::kSums2;
+    return k;
+  }
+  // Columns in registers as above, and for shorter rows where there are more of them than the other kernel's workgroups
+  // do in one round, or where an expert's tokens would take the other kernel four passes: measured (so, and by 64 rows)
+  // 8 experts of 4096x14336, 64 tokens 105 and 222, 8 tokens 47 and 51; 34 of 256x12096, 9 tokens 17 and 26; 32 of
+  // 2048x1536, 64 tokens with eight each 35 and 55; 8 of 2048x1536, 64 tokens 19 and 17; 11 of 1120x1504, 7 tokens 9.3 and
+  // 6.0; 4 of 2048x800, 64 tokens 15 and 22.
+  const uint32_t least = outer_columns > 48 ? 768 : served * ((a.cols + 63) / 64) > 2 * kMoeUnits ? 1024 : 2048;
+  const uint32_t chunks = (h_steps + 7) / 8;  // a wavefront of eight has one step of each
+  if (k.outer_dma && a.inner > least && chunks <= kMoeChunks && near(a.down)) {
+    k.outer = MxMoeChoice::kChunks;
+    k.span = (h_steps + chunks - 1) / chunks, k.chunks = (h_steps + k.span - 1) / k.span;
+  } else {
+    k.outer = MxMoeChoice::kRows;
+  }
+  return k;
 }
 
 }  // namespace ptwm

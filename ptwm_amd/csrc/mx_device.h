@@ -238,9 +238,6 @@ __device__ __forceinline__ uint32_t quantise8(const float (&v)[8], uint32_t& lo,
   return broken ? 255u : (uint32_t)b;
 }
 
-// bf16 parts that hold a value of type T exactly.
-constexpr int parts_of(uint32_t type) { return type == kTypeF32 ? 3 : type == kTypeF16 ? 2 : 1; }
-
 __device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t w, float scale, bool high) {
   return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))
               : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));

@@ -26,19 +26,13 @@
 
 #include <type_traits>
 
+#include "mx_choice.h"
 #include "mx_device.h"
 
 namespace ptwm {
 namespace {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-
-constexpr uint32_t kComputeUnits = 256;
-constexpr uint32_t kTokens = 64;  // of a launch; longer calls run in several
-constexpr uint32_t kStep = 256;   // values of a row that go through LDS together: a cache line of codes
-
-// h's parts: all 24 bits of a sum in 32, whatever the outputs' type.
-constexpr uint32_t kInnerParts = 3;
 
 // Where a launch's intermediate results lie in the workspace.  A pair is a token's k-th expert, token * top_k + k.
 struct MoePlaces {
@@ -51,9 +45,8 @@ struct MoePlaces {
   uint64_t end;
   uint32_t x_len, h_len;  // cols and inner in whole steps, zeros past their ends
 };
-constexpr uint32_t kChunks = 16;  // that the outer products' rows are cut into at most
 MoePlaces places_of(const MxMoeArgs& a) {
-  const uint64_t t = a.tokens < kTokens ? a.tokens : kTokens, pairs = t * a.top_k;
+  const uint64_t t = a.tokens < kMoeTokens ? a.tokens : kMoeTokens, pairs = t * a.top_k;
   uint64_t at = a.workspace;
   const auto take = [&](uint64_t bytes) {
     const uint64_t here = at;
@@ -61,12 +54,12 @@ MoePlaces places_of(const MxMoeArgs& a) {
     return here;
   };
   MoePlaces p;
-  p.x_len = (a.cols + kStep - 1) / kStep * kStep, p.h_len = (a.inner + kStep - 1) / kStep * kStep;
+  p.x_len = (a.cols + kMoeStep - 1) / kMoeStep * kMoeStep, p.h_len = (a.inner + kMoeStep - 1) / kMoeStep * kMoeStep;
   p.logits = take(t * a.experts * 8);
   p.x = take(parts_of(a.x_type) * t * p.x_len * 2);
-  p.h = take(kInnerParts * pairs * p.h_len * 2);
-  const uint64_t chunks = (p.h_len / kStep + 7) / 8;
-  p.y = take((chunks <= kChunks ? chunks : 1) * pairs * a.cols * 4);
+  p.h = take(kMoeInnerParts * pairs * p.h_len * 2);
+  const uint64_t chunks = (p.h_len / kMoeStep + 7) / 8;
+  p.y = take((chunks <= kMoeChunks ? chunks : 1) * pairs * a.cols * 4);
   p.chosen = take(pairs * 4), p.weights = take(pairs * 4);
   p.end = at;
   return p;
@@ -148,9 +141,9 @@ __device__ __forceinline__ float activated(float g, float u) {
 // Two neighbours of a pair's h, the parts `apart` bytes apart: as x.s; the last is exact too, down to 2^-133.
 __device__ __forceinline__ void store_h(uint64_t to, uint64_t apart, f32x2 h) {
 #pragma unroll
-  for (uint32_t p = 0; p < kInnerParts; ++p, to += apart) {
+  for (uint32_t p = 0; p < kMoeInnerParts; ++p, to += apart) {
     uint32_t b;
-    if (p + 1 < kInnerParts) {
+    if (p + 1 < kMoeInnerParts) {
       const uint32_t low = f32_bits(__builtin_amdgcn_fmed3f(h[0], -kBf16Max, kBf16Max)) & 0xFFFF0000u;
       const uint32_t high = f32_bits(__builtin_amdgcn_fmed3f(h[1], -kBf16Max, kBf16Max)) & 0xFFFF0000u;
       h -= f32x2{bits_f32(low), bits_f32(high)};
@@ -200,7 +193,7 @@ __global__ __launch_bounds__(kLogitThreads) void moe_logits_kernel(MoeArgs m) {
 #pragma unroll
       for (int j = 0; j < parts_of(T); ++j) st16(m.p.x + (j * a.tokens + t) * m.p.x_len * 2 + chunk_at(k / 8) * 16, p[j]);
     }
-    const uint32_t none = (m.p.h_len - a.inner) / 8, rows = a.top_k * kInnerParts;  // chunks of a row
+    const uint32_t none = (m.p.h_len - a.inner) / 8, rows = a.top_k * kMoeInnerParts;  // chunks of a row
     for (uint32_t j = threadIdx.x; j < none * rows; j += kLogitThreads) {
       const uint32_t row = j / none, part = row / a.top_k, pair = t * a.top_k + row % a.top_k;
       st16(m.p.h + (part * a.tokens * a.top_k + pair) * m.p.h_len * 2 + chunk_at(a.inner / 8 + j % none) * 16, u32x4{});
@@ -345,11 +338,6 @@ __device__ __forceinline__ void store_choice(const MoeArgs& m, uint32_t t, const
 
 __global__ __launch_bounds__(64) void moe_route_kernel(MoeArgs m) { store_choice(m, blockIdx.x, choose(m, blockIdx.x)); }
 
-// Up to so many, the inner products' workgroups choose the experts for themselves, each all of them: a wavefront two
-// tokens.  (16 experts of 1024x2048, 4 tokens: 22 us, 26 with a launch for the choice; 64 experts, 32 tokens: 49 and 37.)
-constexpr uint32_t kFusedTokens = 8;
-constexpr uint32_t kFusedPairs = 32;
-
 // Rows of one expert's products for its tokens (or, ALL, of the outer products
 // of all experts of up to 64 pairs, weighted and added up).  WR wavefronts hold
 // 16 rows each, of gate and up (INNER) or of down, and share the XC columns; KG
@@ -387,7 +375,7 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
   static_assert(kColumns % G == 0 && (NS - 2) * N < 64, "whole requests, and a wait that counts them");
   __shared__ u32x4 columns[KG * NS * kColumns], codes[KG * WR * NS * kCodes];
   __shared__ u32x4 scales[KG * WR * NS * kScales / 4];
-  __shared__ int32_t list[64], table[ALL ? 64 * XC : 1], fused[INNER ? kFusedPairs : 1];
+  __shared__ int32_t list[64], table[ALL ? 64 * XC : 1], fused[INNER ? kMoeFusedPairs : 1];
   __shared__ float weights[ALL ? 64 : 1];
   const MxMoeArgs& a = m.a;
   const uint32_t lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
@@ -395,10 +383,10 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t group = wave / WR, wr = wave % WR, gi = wr * 64 + lane;
   const uint32_t rows = INNER ? a.inner : a.cols, length = INNER ? a.cols : a.inner, blocks = length / kMxBlock;
-  const uint32_t x_len = INNER ? m.p.x_len : m.p.h_len, steps = x_len / kStep;
+  const uint32_t x_len = INNER ? m.p.x_len : m.p.h_len, steps = x_len / kMoeStep;
   const uint32_t tiles = (rows + kRows - 1) / kRows;
   const uint32_t slot = blockIdx.x / tiles, n0 = blockIdx.x % tiles * kRows;
-  const uint32_t parts = INNER ? parts_of(a.x_type) : kInnerParts, each = XC / parts;  // tokens of XC columns
+  const uint32_t parts = INNER ? parts_of(a.x_type) : kMoeInnerParts, each = XC / parts;  // tokens of XC columns
   const uint32_t pairs = (uint32_t)a.tokens * a.top_k;
 
   // The expert and the pairs that chose it (every wavefront writes the same to LDS); ALL: the experts that any pair
@@ -521,7 +509,7 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
       }
 #pragma unroll
       for (int j = 0; j < JX; ++j) {
-        uint32_t from = x_at[j] + u.step * (kStep * 2);
+        uint32_t from = x_at[j] + u.step * (kMoeStep * 2);
         if constexpr (ALL) {
           // a token that did not choose the expert has another's h here, whose sums are left out
           const int32_t pair = table[u.k * XC + x_token[j]];
@@ -660,7 +648,7 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
 // products and sums: a tile's 16 products a wavefront and 16 columns, its two barriers and the sums' way through LDS
 // take longer than its bytes).  With columns through LDS they took 120 and 101.  Weights that stayed in L2 as others do
 // (no "once") took 114 and 75: lines of h and y, of which a tile writes 32 or 64 bytes, left L2 in pieces.
-constexpr uint32_t kStreamGroups = kComputeUnits;
+constexpr uint32_t kStreamGroups = kMoeUnits;
 constexpr uint32_t kStreamSlots = 16;    // experts of a workgroup, see below
 // What a tile costs beside its groups of columns, in the like of one: 64 tokens' outer products take 74 us by equal tiles
 // and 70, 69, 68.7 with 8, 6, 2.
@@ -674,18 +662,18 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
   __shared__ u32x4 codes[8 * NS * kCodes];
   __shared__ uint32_t scales[8 * NS * kWords];
   __shared__ f32x2 sums[8 * M * NC * 128];
-  __shared__ int16_t chosen[kTokens * kMoeMaxTopK];
+  __shared__ int16_t chosen[kMoeTokens * kMoeMaxTopK];
   __shared__ u32x4 none[8];
   __shared__ uint32_t slots[kStreamSlots], share[4];
-  __shared__ int32_t list[kTokens];
+  __shared__ int32_t list[kMoeTokens];
   __shared__ float biases[M][INNER ? kBiasTiles * 16 : 1];
   const MxMoeArgs& a = m.a;
   const uint32_t lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t rows = INNER ? a.inner : a.cols, length = INNER ? a.cols : a.inner, tiles = rows / (INNER ? 16 : 32);
-  const uint32_t x_len = INNER ? m.p.x_len : m.p.h_len, steps = x_len / kStep;
+  const uint32_t x_len = INNER ? m.p.x_len : m.p.h_len, steps = x_len / kMoeStep;
   const uint32_t span = m.span, chunks = m.chunks;
-  const uint32_t parts = INNER ? parts_of(a.x_type) : kInnerParts, each = 16 / parts, most = each * NC;
+  const uint32_t parts = INNER ? parts_of(a.x_type) : kMoeInnerParts, each = 16 / parts, most = each * NC;
   const uint32_t pairs = (uint32_t)a.tokens * a.top_k;
   // A slot is an expert's up to `most` tokens; a tile of it weighs kTileWeight + its groups of columns, and every
   // workgroup has an equal share of that.  There are at most 2048 / 5 + 1024 slots (three parts, one group of columns),
@@ -755,7 +743,7 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
   };
 
   auto part_of = [&](uint32_t chunk, uint32_t n) {  // which of n steps is only part of one
-    return length % kStep && chunk * span + wave + (n - 1) * 8 == steps - 1 ? n - 1 : ~0u;
+    return length % kMoeStep && chunk * span + wave + (n - 1) * 8 == steps - 1 ? n - 1 : ~0u;
   };
   // The tile to be requested next: of it `n` steps, `run` tiles to the end of the expert's or the chunk's, `left` to the
   // end of all.  Rows come by 32, so all of a tile's are there.
@@ -872,12 +860,12 @@ __global__ __launch_bounds__(512) void moe_stream_kernel(MoeArgs m) {
         if (i >= each * parts || t >= tokens) t = 0, p = 0;
         const uint32_t pair = (uint32_t)list[t0 + t];
         const uint32_t row = INNER ? p * (uint32_t)a.tokens + pair / a.top_k : p * pairs + pair;
-        const uint32_t at = row * x_len * 2 + (chunk * span + wave) * (kStep * 2) + q * 16;
+        const uint32_t at = row * x_len * 2 + (chunk * span + wave) * (kMoeStep * 2) + q * 16;
 #pragma unroll
         for (int s = 0; s < S; ++s)
           if (s < mine)
 #pragma unroll
-            for (int u = 0; u < 8; ++u) x[s][c][u] = ld16(x0, at + s * 8 * (kStep * 2) + u * 64);
+            for (int u = 0; u < 8; ++u) x[s][c][u] = ld16(x0, at + s * 8 * (kMoeStep * 2) + u * 64);
       }
     }
     // where this lane's sums go: of the first part's column
@@ -1056,11 +1044,6 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs m) {
   store_out(a, t, n, v);
 }
 
-// Codes at multiples of 16 bytes.
-bool dma_of(const MxExperts& w, uint64_t experts) {
-  return w.codes.ptr % 16 == 0 && w.codes.stride % 16 == 0 && (experts == 1 || w.codes_expert % 16 == 0);
-}
-
 template <bool INNER, bool ALL, int WR, int KG, int XC, int NS>
 hipError_t product_of(const MoeArgs& m, bool dma, hipStream_t stream) {
   constexpr uint32_t kRows = 16 * WR;
@@ -1071,16 +1054,6 @@ hipError_t product_of(const MoeArgs& m, bool dma, hipStream_t stream) {
                 items * tiles, 64 * WR * KG, m, stream);
 }
 
-// 16 rows as 32-bit offsets.
-bool near_rows(const MxExperts& w) { return w.codes.stride < 1ull << 27 && w.scales.stride < 1ull << 27; }
-
-// Cuts rows into chunks, at most `most` of them, of which a wavefront has s steps at most.
-bool chunks_of(uint32_t len, uint32_t most, uint32_t s, MoeArgs& m) {
-  const uint32_t steps = len / kStep, chunks = (steps + 8 * s - 1) / (8 * s);
-  if (chunks > most) return false;
-  m.span = (steps + chunks - 1) / chunks, m.chunks = (steps + m.span - 1) / m.span;
-  return true;
-}
 template <bool INNER, int S, int NC>
 hipError_t stream_of(const MoeArgs& m, hipStream_t stream) {
   return launch(moe_stream_kernel<INNER, S, NC>, kStreamGroups, 512, m, stream);
@@ -1101,54 +1074,32 @@ hipError_t logits_of(const MoeArgs& m, hipStream_t stream) {
 uint64_t mxfp4_moe_workspace(const MxMoeArgs& a) { return places_of(a).end - a.workspace; }
 
 hipError_t launch_mxfp4_moe(const MxMoeArgs& a, hipStream_t stream) {
-  const bool inner = dma_of(a.gate, a.experts) && dma_of(a.up, a.experts), outer = dma_of(a.down, a.experts);
-  return in_parts(a.tokens, kTokens, [&](uint64_t first, uint64_t tokens) {
+  return in_parts(a.tokens, kMoeTokens, [&](uint64_t first, uint64_t tokens) {
     MoeArgs m{a, places_of(a), 1, 1, false};
     m.a.tokens = tokens;
     m.a.x = rows_from(a.x, first, type_bytes(a.x_type)), m.a.out = rows_from(a.out, first, type_bytes(a.out_type));
     if (a.experts_out) m.a.experts_out += first * a.top_k * 4;
     if (a.weights_out) m.a.weights_out += first * a.top_k * 4;
+    const MxMoeChoice k = choose_mxfp4_moe(m.a);
+    m.routed = k.routed;
     hipError_t e = logits_of(m, stream);
-    const uint64_t pairs = tokens * a.top_k;
-    const uint32_t xp = parts_of(a.x_type);
-    // Rows that keep most of eight wavefronts busy (2 of 8 experts of 4096x14336, 8 tokens: 79 us, 88 by the other
-    // kernel; 64 tokens 97 and 134; 8192 columns, 64 tokens 78 and 99; 128 experts of 2048x768, 16 tokens 36 and 30), or
-    // half of them where an expert's tokens would take the other kernel several passes (2 experts of 1024x2048, 64
-    // tokens: 12 and 19; 10 of 640x5984, 17 tokens of f32 each: 62 and 50).
-    const double inner_columns = (double)pairs / a.experts * xp, outer_columns = (double)pairs / a.experts * kInnerParts;
-    const bool stream_inner = tokens > 1 && inner && a.cols > (inner_columns > 32 ? 768 : 2048) && near_rows(a.gate) &&
-                              near_rows(a.up) && a.gate.codes.stride == a.up.codes.stride &&
-                              a.gate.scales.stride == a.up.scales.stride && chunks_of(m.p.x_len, 1, 4, m);
-    m.routed = tokens > kFusedTokens || pairs > kFusedPairs;
-    if (e == hipSuccess && m.routed) e = launch(moe_route_kernel, tokens, 64, m, stream);
+    if (e == hipSuccess && k.routed) e = launch(moe_route_kernel, tokens, 64, m, stream);
     if (e != hipSuccess) return e;
-    // 16 rows a workgroup, four wavefronts along them, where 64 would leave compute units idle (8 of 128 experts of
-    // 2048x768, 1 token: 9.2 us and 12.7; 2 of 8 of 4096x14336: 31 and 27)
-    const uint64_t groups = (pairs < a.experts ? pairs : a.experts) * ((a.inner + 63) / 64);
-    if (tokens * xp <= 4 && groups < kComputeUnits && !stream_inner)
-      e = product_of<true, false, 1, 4, 4, 2>(m, inner, stream);
-    else if (stream_inner && m.p.x_len <= 16 * kStep)
-      e = stream_of<true, 2, 2>(m, stream);
-    else if (stream_inner)
-      e = stream_of<true, 4, 1>(m, stream);
-    else
-      e = product_of<true, false, 4, 1, 16, 2>(m, inner, stream);
+    m.span = m.p.x_len / kMoeStep;
+    switch (k.inner) {
+      case MxMoeChoice::kRows16: e = product_of<true, false, 1, 4, 4, 2>(m, k.inner_dma, stream); break;
+      case MxMoeChoice::kRows64: e = product_of<true, false, 4, 1, 16, 2>(m, k.inner_dma, stream); break;
+      case MxMoeChoice::kStream2: e = stream_of<true, 2, 2>(m, stream); break;
+      case MxMoeChoice::kStream4: e = stream_of<true, 4, 1>(m, stream); break;
+    }
     if (e != hipSuccess) return e;
-    // The weighted sums at once, without a launch of their own of 4 us, unless few workgroups have much to do (2 of 8
-    // experts of 4096x14336, 1 token: 15.0 us, 17.4 before the sums; 6 of 53 of 512x6080: 17.9 and 9.6).
-    if (tokens <= 2 && pairs <= 64 && (a.cols >= 2048 || pairs * (m.p.h_len / kStep) <= 64))
-      return tokens == 1 ? product_of<false, true, 1, 8, 4, 3>(m, outer, stream)
-                         : product_of<false, true, 1, 8, 6, 3>(m, outer, stream);
-    // As above, and shorter rows too where there are more of them than the other kernel's workgroups do in one round, or
-    // where an expert's tokens would take the other kernel four passes (8 experts of 4096x14336, 64 tokens: 105 us and 222;
-    // 2 of 8, 8 tokens 47 and 51; 34 of 256x12096, 9 tokens 17 and 26; 32 of 2048x1536, 64 tokens with eight each 35 and
-    // 55; 8 of 2048x1536, 64 tokens 19 and 17; 11 of 1120x1504, 7 tokens 9.3 and 6.0; 4 of 2048x800, 64 tokens 15 and 22).
-    const uint64_t outer_groups = (pairs < a.experts ? pairs : a.experts) * ((a.cols + 63) / 64);
-    const uint32_t least = outer_columns > 48 ? 768 : outer_groups > 2 * kComputeUnits ? 1024 : 2048;
-    if (outer && a.inner > least && near_rows(a.down) && chunks_of(m.p.h_len, kChunks, 1, m))
-      e = stream_of<false, 1, 4>(m, stream);
-    else
-      e = product_of<false, false, 4, 1, 16, 3>(m, outer, stream);
+    m.span = k.span, m.chunks = k.chunks;
+    switch (k.outer) {
+      case MxMoeChoice::kSums1: return product_of<false, true, 1, 8, 4, 3>(m, k.outer_dma, stream);
+      case MxMoeChoice::kSums2: return product_of<false, true, 1, 8, 6, 3>(m, k.outer_dma, stream);
+      case MxMoeChoice::kRows: e = product_of<false, false, 4, 1, 16, 3>(m, k.outer_dma, stream); break;
+      case MxMoeChoice::kChunks: e = stream_of<false, 1, 4>(m, stream); break;
+    }
     if (e == hipSuccess) e = launch(moe_combine_kernel, (tokens * (a.cols / 4) + 255) / 256, 256, m, stream);
     return e;
   });

@@ -18,6 +18,8 @@ constexpr uint32_t kMxBlock = 32;
 __host__ __device__ constexpr uint32_t type_bytes(uint32_t type) {
   return type == kTypeF32 ? 4 : type == kTypeE4m3 ? 1 : 2;
 }
+// bf16 parts that hold a value of type T exactly.
+constexpr int parts_of(uint32_t type) { return type == kTypeF32 ? 3 : type == kTypeF16 ? 2 : 1; }
 
 // A row-major operand: device address and row stride in elements (of scales:
 // in bytes).  Addresses need no alignment beyond the element's.
@@ -77,6 +79,10 @@ struct MxMoeArgs {
   uint32_t x_type, router_type, out_type;
 };
 constexpr uint64_t kMoeMaxExperts = 1024, kMoeMaxTopK = 32, kMoeMaxWidth = 1 << 17;
+constexpr uint32_t kMoeTokens = 64;  // of a launch; longer calls run in several
+constexpr uint32_t kMoeStep = 256;   // values of a row that go through LDS together: a cache line of codes
+// h's parts: all 24 bits of a sum in 32, whatever the outputs' type.
+constexpr uint32_t kMoeInnerParts = 3;
 // Bytes of workspace, at a multiple of 256, that a call takes.
 uint64_t mxfp4_moe_workspace(const MxMoeArgs& a);
 
