@@ -674,15 +674,16 @@ __global__ __launch_bounds__(64 * kFewWaves) void mxfp4_linear_few_kernel(MxLine
 
 template <uint32_t T, int ROWS, int CT, int RG, int KG, bool RAW>
 hipError_t tiles_of(const MxLinearArgs& a, bool aligned, hipStream_t stream) {
-  return launch_tiles<type_bytes(T), ROWS * RG, 32 * CT>(aligned ? mxfp4_linear_tiles_kernel<T, ROWS, CT, RG, KG, RAW, true>
-                                                     : mxfp4_linear_tiles_kernel<T, ROWS, CT, RG, KG, RAW, false>,
-                                             64 * RG * KG, a, stream);
+  return launch_tiles<type_bytes(T), ROWS * RG, 32 * CT>(
+      aligned ? mxfp4_linear_tiles_kernel<T, ROWS, CT, RG, KG, RAW, true>
+              : mxfp4_linear_tiles_kernel<T, ROWS, CT, RG, KG, RAW, false>,
+      64 * RG * KG, a, stream);
 }
 
 template <uint32_t T, int NT>
 hipError_t few_of(const MxLinearArgs& a, hipStream_t stream) {
   return launch_tiles<type_bytes(T), 16, NT>(mxfp4_linear_few_kernel<T, NT>, 64 * kFewWaves, a, stream,
-                                 (uint32_t)mx_few_bytes(a.cols, NT));
+                                             (uint32_t)mx_few_bytes(a.cols, NT));
 }
 
 template <uint32_t T>
