@@ -137,6 +137,7 @@ decltype(&ptwm_mi355x_mxfp4_moe_cuda) g_moe;
 
 PyObject* g_stream;  // torch's current stream of a device
 PyObject* g_error;   // NativeError
+PyObject* g_memory;  // torch.OutOfMemoryError
 
 uint64_t stream_of(int64_t device) {
   PyObject* d = PyLong_FromLongLong(device);
@@ -166,6 +167,9 @@ PyObject* guarded(F&& f) {
   try {
     return f();
   } catch (const Failed&) {
+    return nullptr;
+  } catch (const c10::OutOfMemoryError& e) {
+    PyErr_SetString(g_memory, e.what_without_backtrace());
     return nullptr;
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
@@ -478,8 +482,9 @@ PyMODINIT_FUNC PyInit__mx(void) {
   PyObject* torch_c = PyImport_ImportModule("torch._C");
   if (!torch_c) return nullptr;
   g_stream = PyObject_GetAttrString(torch_c, "_cuda_getCurrentRawStream");
+  g_memory = g_stream ? PyObject_GetAttrString(torch_c, "OutOfMemoryError") : nullptr;
   Py_DECREF(torch_c);
-  PyObject* native = g_stream ? PyImport_ImportModule("ptwm_amd._native") : nullptr;
+  PyObject* native = g_memory ? PyImport_ImportModule("ptwm_amd._native") : nullptr;
   if (!native) return nullptr;
   g_error = PyObject_GetAttrString(native, "NativeError");
   PyObject* path = g_error ? PyObject_GetAttrString(native, "LIB_PATH") : nullptr;
