@@ -123,11 +123,14 @@ struct Scales16 {
 // through registers to the same places, so results do not depend on how
 // operands lie.  Offsets within a tile are 32 bits on top of uniform addresses.
 //
-// What bounds the largest tile, 256 x 256 by 2 x 4 wavefronts, is the matrix
-// unit at the clock that it holds: 2048x8192x4096, a tile a CU, 39 us, and 38
-// without any request to memory (3.5 PFLOP/s); one tile alone takes 1.25 us for
-// a step of 256 values, 2.2 us with all CUs at work.  LDS gives 96 of its 128
-// bytes a cycle.  Steps of 64 bytes of a row instead of 128 took every cache
+// What bounds the largest tile, 256 x 256 by 2 x 4 wavefronts, is the clock
+// under full load, and then waits within the tile.  2048x8192x4096, a tile a
+// CU: 32768 cycles of the matrix unit within 57000 to 65000 (48000 to 55000 in
+// the loop, the rest for the first bytes and the stores), at 1.8 GHz in a
+// launch alone and 1.3 to 1.6 GHz in launches one after the other (2.3 with a
+// single tile at work): 37 to 43 us, 38 without any request to memory.  While
+// the matrix unit is busy, LDS gives 96 of its 128 bytes a cycle and takes the
+// requests' 32.  Steps of 64 bytes of a row instead of 128 took every cache
 // line twice: 2048x14336x4096 86 us, 77 this way.  Smaller tiles are bound by
 // the way to memory; four stages shorten it (128x14336x4096, 128 x 64 tiles:
 // 13.7 us with two stages, 10.7 with four).
