@@ -357,9 +357,10 @@ __global__ __launch_bounds__(64) void moe_route_kernel(MoeArgs m) { store_choice
 // those come that hold one of the row's own; four lanes a row.  kDma: codes lie
 // at multiples of 16 bytes; else they go through registers.
 //
-// Memory's latency bounds it: a workgroup ends after 1 to 56 steps, of which
-// NS - 1 are on their way, and the chip's bytes on their way are what its
-// workgroups have.  8 experts of 4096x14336, 1 token: inner 27 us (125 MB, 4.6
+// Memory's latency bounds it: a workgroup ends after 1 to 56 steps at the
+// measured sizes (512 at most, and that of each where it walks along several
+// experts), of which NS - 1 are on their way, and the chip's bytes on their way
+// are what its workgroups have.  8 experts of 4096x14336, 1 token: inner 27 us (125 MB, 4.6
 // TB/s), outer 14.6 us (62 MB, 4.3 TB/s).  Three stages of the inner products,
 // two workgroups a compute unit instead of three, 30.6 us.
 template <bool INNER, bool ALL, int WR, int KG, int XC, int NS, bool kDma>
@@ -644,14 +645,15 @@ __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
 // ends of tiles and of experts.  A tile's sums are added up over the wavefronts through LDS, read before the next tile's
 // products and stored after them.  INNER: sums of whole rows; else of a chunk of them, which the combining kernel adds.
 //
-// 8 experts of 4096x14336, 64 tokens: inner 97 us (499 MB, 5.1 TB/s: memory), outer 69 us (250 MB, 3.6 TB/s; 44 without
+// 8 experts of 4096x14336, 64 tokens: inner 97 us (499 MB, 5.1 TB/s: memory), outer 86 us (250 MB, 2.9 TB/s; 44 without
 // products and sums: a tile's 16 products a wavefront and 16 columns, its two barriers and the sums' way through LDS
-// take longer than its bytes).  With columns through LDS they took 120 and 101.  Weights that stayed in L2 as others do
-// (no "once") took 114 and 75: lines of h and y, of which a tile writes 32 or 64 bytes, left L2 in pieces.
+// take longer than its bytes, and experts of more than 20 tokens go by twice).  With h in two parts, 69; so with columns
+// through LDS they took 120 and 101, and weights that stayed in L2 as others do (no "once") 114 and 75: lines of h and
+// y, of which a tile writes 32 or 64 bytes, left L2 in pieces.
 constexpr uint32_t kStreamGroups = kMoeUnits;
 constexpr uint32_t kStreamSlots = 16;    // experts of a workgroup, see below
-// What a tile costs beside its groups of columns, in the like of one: 64 tokens' outer products take 74 us by equal tiles
-// and 70, 69, 68.7 with 8, 6, 2.
+// What a tile costs beside its groups of columns, in the like of one: 64 tokens' outer products took 74 us by equal tiles
+// and 70, 69, 68.7 with 8, 6, 2 (h in two parts); the call with three takes 197, 197, 196, 195 with 9, 6, 4, 2.
 constexpr uint32_t kInnerWeight = 8, kOuterWeight = 2;
 
 template <bool INNER, int S, int NC>
