@@ -138,7 +138,7 @@ __device__ __forceinline__ float activated(float g, float u) {
   return deep ? g * e * u * e * e * e : g / (1.0f + e) * u;
 }
 
-// Two neighbours of a pair's h, the parts `apart` bytes apart: as x.s; the last is exact too, down to 2^-133.
+// Two neighbours of a pair's h, the parts `apart` bytes apart: as x's; the last is exact too, down to 2^-133.
 __device__ __forceinline__ void store_h(uint64_t to, uint64_t apart, f32x2 h) {
 #pragma unroll
   for (uint32_t p = 0; p < kMoeInnerParts; ++p, to += apart) {
@@ -360,9 +360,9 @@ __global__ __launch_bounds__(64) void moe_route_kernel(MoeArgs m) { store_choice
 // Memory's latency bounds it: a workgroup ends after 1 to 56 steps at the
 // measured sizes (512 at most, and that of each where it walks along several
 // experts), of which NS - 1 are on their way, and the chip's bytes on their way
-// are what its workgroups have.  8 experts of 4096x14336, 1 token: inner 27 us (125 MB, 4.6
-// TB/s), outer 14.6 us (62 MB, 4.3 TB/s).  Three stages of the inner products,
-// two workgroups a compute unit instead of three, 30.6 us.
+// are what its workgroups have.  8 experts of 4096x14336, 1 token: inner 27 us
+// (125 MB, 4.6 TB/s), outer 15 us (62 MB, 4.2 TB/s).  Three stages of the inner
+// products, two workgroups a compute unit instead of three, 30.6 us.
 template <bool INNER, bool ALL, int WR, int KG, int XC, int NS, bool kDma>
 __global__ __launch_bounds__(64 * WR * KG) void moe_product_kernel(MoeArgs m) {
   static_assert(WR == 1 || KG == 1, "groups of several wavefronts meet at barriers of the whole workgroup");
